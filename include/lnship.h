@@ -365,6 +365,126 @@ int lnship16_rope_attn_decode_seqs(int mode, const lnship_qkv_store_args *store,
  * (checked before any device call). */
 int lnship32_attn_decode(const lnship_attn_args *args, void *stream);
 
+/* ---- a paged KV cache of several sequences (xlns16) --------------------------
+ * Pages of `page` cells (a power of two, 16 to 256), each holding every kv
+ * head's keys or values of its cells in the cache layouts of
+ * lnship16_store_kv: page i's kv head g starts (i * n_head_kv + g) * page *
+ * head_dim codes into k_pages / v_pages; its cell c, dim d lies at
+ * ((d/8) * page + c) * 8 + d % 8 (keys) and ((c/8) * head_dim + d) * 8 + c % 8
+ * (values).  head_dim a multiple of 8, up to 256; both pointers 16-byte
+ * aligned.  Cell p of sequence s is cell p % page of page
+ * table[s * table_ld + p / page] (table_ld: the pages a row of the table
+ * holds; entries past a sequence's last cell are not read).
+ * The new tokens of a call lie behind each other: rows q_start[s] to
+ * q_start[s+1] - 1 of its ntok rows are sequence s's, and kv_len[s] counts the
+ * sequence's cells, those of its new tokens included, so row t has position
+ * kv_len[s] - q_start[s+1] + t.  q_start (n_seq + 1 non-decreasing entries),
+ * kv_len and table live on the device: a captured graph replays with the
+ * lengths and pages of its replay.  Rows before q_start[0] and from
+ * q_start[n_seq] on belong to no sequence: nothing is read or written for
+ * them.
+ * No counterpart in the reference, whose KV cache is ggml's contiguous one
+ * per sequence. */
+typedef struct lnship_paged_kv {
+    uint16_t *k_pages, *v_pages;
+    int64_t n_pages, page, n_head_kv, head_dim;
+    const int32_t *table;
+    int64_t table_ld;
+    int64_t ntok, n_seq;
+    const int32_t *q_start, *kv_len;
+} lnship_paged_kv;
+
+/* ROPE of the new tokens' query and key heads and the stores of their keys
+ * and values: q_dst holds what lnship16_rope writes, the cells the codes that
+ * lnship16_store_kv stores (keys rotated; through IEEE half), bit for bit.
+ * Row t's heads start at q + t * q_ld, k + t * k_ld and v + t * v_ld (floats),
+ * head_dim floats each: the three parts of a fused q|k|v product, or arrays of
+ * their own.  n_head 0: no queries.  rope_n_dims (even, up to head_dim; 0: none
+ * are rotated, and the keys are stored as the values are) dims are rotated, in
+ * neighbouring pairs or, with neox, in pairs half of them apart, by cos_sin
+ * (lnship_rope_table's layout, n_pos positions).  A position below 0, past the
+ * table's cells or (rotating) not below n_pos, and a page outside
+ * [0, n_pages), is recorded (lnship_index_error) and its row, or what it has
+ * in that page, is skipped.  Two rows of one call never have the same cell
+ * unless the table names a page twice; then which of them stays is not said. */
+typedef struct lnship_paged_store_args {
+    const float *q, *k, *v;
+    int64_t q_ld, k_ld, v_ld;
+    int64_t n_head;
+    int rope_n_dims, neox;
+    const float *cos_sin;
+    int64_t n_pos;
+    float *q_dst;        /* [ntok][n_head][head_dim], row t at t * q_dst_ld */
+    int64_t q_dst_ld;    /* 0: n_head * head_dim */
+} lnship_paged_store_args;
+int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_store_args *a, void *stream);
+
+/* Attention of the new tokens over their sequences' cells: for row t at
+ * position p and query head h (kv head h / (n_head / n_head_kv))
+ *   dst = sum_j e^(s_j - m) V_j / sum_j e^(s_j - m),  s_j = scale q . K_j,
+ * over the cells j <= p and, with window > 0, j > p - window; zeros where
+ * there are none.  Codes stand for their real numbers 2^(log/128 - 128) (as
+ * the stores make them, up to the largest half: larger ones count as
+ * 2^(2047/128)); q and dst are F32, and every sum is a sum of real numbers in
+ * 32 bits, not a chain of LNS additions: such a chain takes two dependent
+ * steps a cell (lnship16_attn_decode runs them), which a long cache cannot
+ * afford, and its result is what the chain rounds.  Keys and values are read
+ * as pairs of IEEE halves on the matrix cores, 22 bits of each operand; the
+ * relative error is about 1e-6.
+ * Cells of a page outside [0, n_pages) or past the table's end count as
+ * hidden and are recorded (lnship_index_error).  dst may be q.
+ * work: lnship16_attn_paged_work bytes of device memory, 16-byte aligned,
+ * that nothing else uses until the call has run (calls on two streams, or
+ * graphs that may replay side by side, need one each); it may be null where
+ * that is 0. */
+typedef struct lnship_paged_attn_args {
+    const float *q;
+    float *dst;
+    int64_t q_ld, dst_ld;   /* floats between rows; 0: n_head * head_dim */
+    int64_t n_head;
+    float scale;
+    int64_t window;
+    void *work;
+    size_t work_bytes;
+} lnship_paged_attn_args;
+int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args *a, void *stream);
+/* the bytes of work that lnship16_attn_paged takes for these sizes on the
+ * current device (pointers are not read); negative: a lnship_error */
+int64_t lnship16_attn_paged_work(const lnship_paged_kv *kv, int64_t n_head);
+
+/* ---- drawing tokens ------------------------------------------------------------
+ * For each of n_rows rows of n_vocab F32 logits (row r at logits + r * ld) one
+ * token, from the uniform random number u[r] in [0, 1).  With x_max the row's
+ * largest logit and T its temperature, token i weighs e^((x_i - x_max) / T).
+ * Tokens are ranked by logit, equal ones by index.  Kept are: the first
+ * top_k; of these the shortest beginning whose weights sum to at least top_p
+ * of theirs all; of these the ones that weigh at least min_p; the first token
+ * always.  Drawn is the first token, by index, at which the running sum of the
+ * kept weights exceeds u times their sum; probs (optional) receives its weight
+ * over that sum.  T not above 0: the first token by rank, with probability 1.
+ * temperature, top_k, top_p, min_p: n_rows values on the device, or null (1,
+ * and no limits); top_k <= 0, top_p >= 1, min_p <= 0 and NaN set no limit.  u
+ * outside [0, 1) counts as the nearer end, NaN as 0.  A NaN logit is never
+ * drawn; with an infinite largest logit only its equals weigh anything; a row
+ * without any logit above -inf gets token -1 and probability 0.  Weights are
+ * summed as integers (units of 2^-40), so the draw does not depend on an order
+ * of additions.  n_vocab up to 2^22.  No LNS arithmetic, and no counterpart in
+ * the reference, which samples on the host.
+ * work: lnship_sample_work bytes, as in lnship_paged_attn_args. */
+typedef struct lnship_sample_args {
+    const float *logits;
+    int64_t ld, n_rows, n_vocab;   /* ld 0: n_vocab */
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p, *u;
+    int32_t *tokens;
+    float *probs;
+    void *work;
+    size_t work_bytes;
+} lnship_sample_args;
+int lnship_sample(const lnship_sample_args *a, void *stream);
+int64_t lnship_sample_work(int64_t n_rows, int64_t n_vocab);
+
 /* ggml views on the device (tensors in the ggml device buffer type): the
  * elements of a 4-D strided view (byte strides nb, as ggml_tensor::nb)
  * gathered into a contiguous F32 array in ggml element order, from F32

@@ -207,4 +207,62 @@ __device__ __forceinline__ float x32_to_f32(uint32_t v) {
     return (v & k32_sign) ? -f : f;
 }
 
+// ---- shared by the kernel files ------------------------------------------
+
+// Records an index out of range: err[0] = 1, err[1] = the first such index.
+__device__ __forceinline__ void index_fault(unsigned long long *err, int64_t idx) {
+    if (atomicCAS(&err[0], 0ull, 1ull) == 0ull) err[1] = (unsigned long long)idx;
+}
+
+// The float -> xlns16 conversion from a 512-entry table in LDS: the code of a
+// normal float is its exponent times 128 plus a function of the top eight
+// mantissa bits (floor or ceil of 128 log2(1 + m / 256), as the exponent is
+// positive or negative: the conversion truncates toward zero).  Zeros,
+// denormals, infinities and NaN read the whole table in global memory.  A
+// gather from that 256 KB table costs a wave a cache line per lane; this one
+// a few LDS cycles.
+struct cvt16_lds {
+    const uint16_t *t;     // LDS: [0, 256) exponents below 127, [256, 512) from 127 on; less 127 * 128
+    const uint16_t *cvt;   // the whole table
+    __device__ __forceinline__ uint32_t operator()(float f) const {
+        const uint32_t b = f32_bits(f), ex = __builtin_amdgcn_ubfe(b, 23, 8);
+        const uint32_t m = __builtin_amdgcn_ubfe(b, 15, 8);
+        const uint32_t l = ((uint32_t)t[m + (ex < 127u ? 0u : 256u)] + (ex << 7)) & k16_logmask;
+        uint32_t c = l | ((b >> 16) & k16_sign);
+        if (__builtin_expect(ex - 1u >= 254u, 0)) c = x16_from_f32(cvt, f);
+        return c;
+    }
+};
+constexpr int k_cvt_lds = 512;
+__device__ __forceinline__ cvt16_lds stage_cvt16(const uint16_t *cvt, uint16_t *t) {
+    for (int i = threadIdx.x; i < k_cvt_lds; i += blockDim.x)
+        t[i] = (uint16_t)(cvt[((i < 256 ? 126u : 127u) << 8) | (uint32_t)(i & 255)] - (i < 256 ? 126 : 127) * 128);
+    return {t, cvt};
+}
+
+// xlns16 through the conversion, decode, Gaussian-log and sigmoid tables
+struct fmt16 {
+    using code_t = uint16_t;
+    const dev_tables &T;
+    __device__ __forceinline__ uint32_t from(float v) const { return x16_from_f32(T.cvt16, v); }
+    __device__ __forceinline__ float to(uint32_t c) const { return T.rev16[c]; }
+    __device__ __forceinline__ uint32_t add(uint32_t x, uint32_t y) const { return x16_add_g(T.gauss16, x, y); }
+    __device__ __forceinline__ uint32_t mul(uint32_t x, uint32_t y) const { return x16_mul(x, y); }
+    __device__ __forceinline__ uint32_t neg(uint32_t x) const { return x ^ k16_sign; }
+    // xlns16_silu: x times the table sigmoid of x
+    __device__ __forceinline__ uint32_t silu(uint32_t x) const { return x16_mul(x, T.sig16[x]); }
+};
+
+// the rotation of one pair
+template <class F>
+__device__ __forceinline__ void rope_pair(const F &f, const float *xr, int64_t j, int n_dims, int neox, const float *cs,
+                                          int64_t &i0, int64_t &i1, uint32_t &r0, uint32_t &r1) {
+    const uint32_t c = f.from(cs[j * 2]), sn = f.from(cs[j * 2 + 1]);
+    i0 = neox ? j : 2 * j;
+    i1 = neox ? j + n_dims / 2 : 2 * j + 1;
+    const uint32_t x0 = f.from(xr[i0]), x1 = f.from(xr[i1]);
+    r0 = f.add(f.mul(x0, c), f.neg(f.mul(x1, sn)));
+    r1 = f.add(f.mul(x0, sn), f.mul(x1, c));
+}
+
 }  // namespace lnship

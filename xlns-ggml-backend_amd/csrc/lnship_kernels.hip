@@ -20,12 +20,11 @@
 
 #include "lnship.h"
 #include "lnship_device.h"
+#include "lnship_host.h"
 #include "lnship_tables.h"
 
 namespace lnship {
 
-constexpr int k_block = 256;
-constexpr int k_max_devices = 64;
 // LDS budget of a workgroup on gfx950 (160 KiB per CU)
 constexpr int k_lds_bytes = 160 * 1024;
 // what the row kernels' static shared arrays may take beside their dynamic LDS
@@ -75,40 +74,21 @@ static_assert((k32_sb_end & ((1u << k32_sb_fsh) - 1)) == 0, "the far grid starts
 
 static thread_local std::string t_err;
 
-static int fail(int code, const char *fmt, const char *what = "") {
+int fail(int code, const char *fmt, const char *what) {
     char buf[256];
     std::snprintf(buf, sizeof buf, fmt, what);
     t_err = buf;
     return code;
 }
 
-static int hip_fail(hipError_t e, const char *where) {
+int hip_fail(hipError_t e, const char *where) {
     char buf[256];
     std::snprintf(buf, sizeof buf, "%s: %s", where, hipGetErrorString(e));
     t_err = buf;
     return LNSHIP_EDEVICE;
 }
 
-#define LNSHIP_HIP(call)                                          \
-    do {                                                          \
-        hipError_t e_ = (call);                                   \
-        if (e_ != hipSuccess) return hip_fail(e_, #call);         \
-    } while (0)
-
 // ---- per-device state -----------------------------------------------------
-
-struct device_state {
-    bool ready = false;
-    int cus = 0;   // compute units
-    dev_tables T{};
-    void *scratch = nullptr;   // grow-only
-    size_t scratch_size = 0;
-    std::vector<void *> retired;   // outgrown scratch blocks, kept for captured graphs
-    void *fixed_scratch = nullptr;  // this device's copy of `scratch` (below), from hipGetSymbolAddress
-    // index check of get_rows / set_rows: [0] set to 1 by the first
-    // out-of-range index since the last lnship_index_error, [1] that index
-    unsigned long long *index_err = nullptr;
-};
 
 static device_state g_devices[k_max_devices];
 
@@ -122,7 +102,7 @@ static __device__ __align__(256) unsigned char scratch[k_fixed_scratch_bytes];
 static std::mutex g_mutex;
 static host_tables *g_host = nullptr;
 
-static int current_device(int *dev) {
+int current_device(int *dev) {
     LNSHIP_HIP(hipGetDevice(dev));
     if (*dev < 0 || *dev >= k_max_devices) return fail(LNSHIP_EDEVICE, "device index out of range%s");
     return 0;
@@ -137,7 +117,7 @@ static int upload(const T *src, size_t n, const T **dst) {
     return 0;
 }
 
-static device_state *state() {
+device_state *state() {
     int dev = 0;
     if (current_device(&dev) != 0) return nullptr;
     device_state *s = &g_devices[dev];
@@ -212,25 +192,6 @@ __global__ void k_to_f32_32(const uint32_t *__restrict__ src, float *__restrict_
         dst[i] = x32_to_f32(src[i]);
 }
 
-// The float -> xlns16 conversion from a 512-entry table in LDS: the code of a
-// normal float is its exponent times 128 plus a function of the top eight
-// mantissa bits (floor or ceil of 128 log2(1 + m / 256), as the exponent is
-// positive or negative: the conversion truncates toward zero).  Zeros,
-// denormals, infinities and NaN read the whole table in global memory.  A
-// gather from that 256 KB table costs a wave a cache line per lane; this one
-// a few LDS cycles.
-struct cvt16_lds {
-    const uint16_t *t;     // LDS: [0, 256) exponents below 127, [256, 512) from 127 on; less 127 * 128
-    const uint16_t *cvt;   // the whole table
-    __device__ __forceinline__ uint32_t operator()(float f) const {
-        const uint32_t b = f32_bits(f), ex = __builtin_amdgcn_ubfe(b, 23, 8);
-        const uint32_t m = __builtin_amdgcn_ubfe(b, 15, 8);
-        const uint32_t l = ((uint32_t)t[m + (ex < 127u ? 0u : 256u)] + (ex << 7)) & k16_logmask;
-        uint32_t c = l | ((b >> 16) & k16_sign);
-        if (__builtin_expect(ex - 1u >= 254u, 0)) c = x16_from_f32(cvt, f);
-        return c;
-    }
-};
 // a batch of values: one branch for the batch's special values
 template <int B>
 __device__ __forceinline__ void cvt16_batch(const cvt16_lds &C, const float (&f)[B], uint32_t (&c)[B]) {
@@ -246,13 +207,6 @@ __device__ __forceinline__ void cvt16_batch(const cvt16_lds &C, const float (&f)
         for (int q = 0; q < B; q++) c[q] = x16_from_f32(C.cvt, f[q]);
     }
 }
-constexpr int k_cvt_lds = 512;
-__device__ __forceinline__ cvt16_lds stage_cvt16(const uint16_t *cvt, uint16_t *t) {
-    for (int i = threadIdx.x; i < k_cvt_lds; i += blockDim.x)
-        t[i] = (uint16_t)(cvt[((i < 256 ? 126u : 127u) << 8) | (uint32_t)(i & 255)] - (i < 256 ? 126 : 127) * 128);
-    return {t, cvt};
-}
-
 // rows x cols row-major -> k8-interleaved (k = col, m = row), one slice per
 // blockIdx.y; padding columns (cols..Kp) get code 0.  TY: 0 F32, 1 IEEE half,
 // 2 xlns16 codes.  Bound by HBM (xlns32: by its FP64 logarithms): a thread
@@ -1289,11 +1243,6 @@ struct mm_args16 {
     // workgroup x works (as block x >> xcd_sh) iff x is a multiple of 2^xcd_sh
     uint32_t xcd_sh;
 };
-
-// Records an index out of range: err[0] = 1, err[1] = the first such index.
-__device__ __forceinline__ void index_fault(unsigned long long *err, int64_t idx) {
-    if (atomicCAS(&err[0], 0ull, 1ull) == 0ull) err[1] = (unsigned long long)idx;
-}
 
 // The weight slice and activation slice of grid slice (i12, i13): ggml's
 // broadcast for MUL_MAT, the expert of the slot for MUL_MAT_ID.  Returns
@@ -3199,20 +3148,9 @@ __global__ __launch_bounds__(4 * k_block) void k_softmax16(sm_args a, dev_tables
 
 // ---- elementwise ops of the Llama graph ---------------------------------------
 
-// The elementwise ops in either format: fmt16 (xlns16 through the
+// The elementwise ops in either format: fmt16 (lnship_device.h; xlns16 through the
 // conversion, decode, Gaussian-log and sigmoid tables) or fmt32 (xlns32,
 // converted arithmetically, adder over the global xlns32 tables).
-struct fmt16 {
-    using code_t = uint16_t;
-    const dev_tables &T;
-    __device__ __forceinline__ uint32_t from(float v) const { return x16_from_f32(T.cvt16, v); }
-    __device__ __forceinline__ float to(uint32_t c) const { return T.rev16[c]; }
-    __device__ __forceinline__ uint32_t add(uint32_t x, uint32_t y) const { return x16_add_g(T.gauss16, x, y); }
-    __device__ __forceinline__ uint32_t mul(uint32_t x, uint32_t y) const { return x16_mul(x, y); }
-    __device__ __forceinline__ uint32_t neg(uint32_t x) const { return x ^ k16_sign; }
-    // xlns16_silu: x times the table sigmoid of x
-    __device__ __forceinline__ uint32_t silu(uint32_t x) const { return x16_mul(x, T.sig16[x]); }
-};
 struct fmt32 {
     using code_t = uint32_t;
     const dev_tables &T;
@@ -3270,18 +3208,6 @@ __global__ void k_get_rows_packed(const uint16_t *__restrict__ w, int64_t K, int
         const int64_t m = rows[r];
         dst[i] = rev[w[((k >> 3) * M + m) * 8 + (k & 7)]];
     }
-}
-
-// one thread per rotated pair (or passthrough element)
-template <class F>
-__device__ __forceinline__ void rope_pair(const F &f, const float *xr, int64_t j, int n_dims, int neox, const float *cs,
-                                          int64_t &i0, int64_t &i1, uint32_t &r0, uint32_t &r1) {
-    const uint32_t c = f.from(cs[j * 2]), sn = f.from(cs[j * 2 + 1]);
-    i0 = neox ? j : 2 * j;
-    i1 = neox ? j + n_dims / 2 : 2 * j + 1;
-    const uint32_t x0 = f.from(xr[i0]), x1 = f.from(xr[i1]);
-    r0 = f.add(f.mul(x0, c), f.neg(f.mul(x1, sn)));
-    r1 = f.add(f.mul(x0, sn), f.mul(x1, c));
 }
 
 // item i of a rope: a rotated pair (j < n_dims / 2) or a passthrough element

@@ -65,6 +65,29 @@ class AttnSeqs(ctypes.Structure):
                 ("monte_offset", ctypes.c_uint64 * 3)]
 
 
+class PagedKV(ctypes.Structure):
+    _fields_ = [("k_pages", c_p), ("v_pages", c_p), ("n_pages", c_i64), ("page", c_i64), ("n_head_kv", c_i64),
+                ("head_dim", c_i64), ("table", c_p), ("table_ld", c_i64), ("ntok", c_i64), ("n_seq", c_i64),
+                ("q_start", c_p), ("kv_len", c_p)]
+
+
+class PagedStoreArgs(ctypes.Structure):
+    _fields_ = [("q", c_p), ("k", c_p), ("v", c_p), ("q_ld", c_i64), ("k_ld", c_i64), ("v_ld", c_i64),
+                ("n_head", c_i64), ("rope_n_dims", ctypes.c_int), ("neox", ctypes.c_int), ("cos_sin", c_p),
+                ("n_pos", c_i64), ("q_dst", c_p), ("q_dst_ld", c_i64)]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [("q", c_p), ("dst", c_p), ("q_ld", c_i64), ("dst_ld", c_i64), ("n_head", c_i64),
+                ("scale", ctypes.c_float), ("window", c_i64), ("work", c_p), ("work_bytes", ctypes.c_size_t)]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [("logits", c_p), ("ld", c_i64), ("n_rows", c_i64), ("n_vocab", c_i64), ("temperature", c_p),
+                ("top_k", c_p), ("top_p", c_p), ("min_p", c_p), ("u", c_p), ("tokens", c_p), ("probs", c_p),
+                ("work", c_p), ("work_bytes", ctypes.c_size_t)]
+
+
 def attn_seqs(n_seq, seeds=(0, 0, 0)):
     """lnship_attn_seqs for n_seq sequences; seeds: the kq, soft_max and kqv
     nodes' Monte seed arguments (seed_fields forms: all three 16-bit states,
@@ -170,6 +193,11 @@ def lib():
                                          c_p]),
         "lnship32_store_kv": (ctypes.c_int, [c_p, c_i64, c_p, c_i64, c_i64, c_i64, ctypes.c_int, c_p, c_p, c_i64,
                                              c_i64, ctypes.c_int, c_p, c_i64, c_p]),
+        "lnship16_rope_store_kv_paged": (ctypes.c_int, [ctypes.POINTER(PagedKV), ctypes.POINTER(PagedStoreArgs), c_p]),
+        "lnship16_attn_paged": (ctypes.c_int, [ctypes.POINTER(PagedKV), ctypes.POINTER(PagedAttnArgs), c_p]),
+        "lnship16_attn_paged_work": (c_i64, [ctypes.POINTER(PagedKV), c_i64]),
+        "lnship_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), c_p]),
+        "lnship_sample_work": (c_i64, [c_i64, c_i64]),
         "lnship_causal_mask": (ctypes.c_int, [c_p, c_i64, c_i64, c_p, c_p]),
         "lnship_rope_table": (ctypes.c_int, [ctypes.c_float, ctypes.c_int, c_i64, c_p]),
     }
@@ -445,3 +473,45 @@ def lfsr_advance(state, draws):
     """state (a device uint16 tensor) <- lfsr_jump(state, draws), in stream order."""
     init()
     check(lib().lnship_lfsr_advance(_p(state), draws, _stream()))
+
+
+# ---- drawing tokens ----------------------------------------------------------
+
+def _row_values(t, rows, dtype, name, device):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != (rows,) or t.device != device or not t.is_contiguous():
+        raise LnshipError(f"sample: {name} must be a contiguous {dtype} tensor of {rows} on the logits' device")
+    return t.data_ptr()
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+    """One token for each row of logits [n_rows, n_vocab] (float32; rows may be
+    strided): temperature, then top_k, top_p and min_p (each None or one value
+    a row on the device; top_k int32, the others float32), drawn by the uniform
+    numbers u [n_rows].  Returns (tokens int32, probs float32), or fills the
+    pair out; a row that holds no number above -inf gets token -1."""
+    import torch
+    init()
+    dev = logits.device
+    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1 or not logits.is_cuda:
+        raise LnshipError("sample: logits must be float32 [n_rows, n_vocab] on the GPU, a row's values together")
+    if dev.index != torch.cuda.current_device():
+        raise LnshipError("sample: logits are not on the current device")
+    rows, vocab = logits.shape
+    tokens, probs = out if out is not None else (torch.empty(rows, dtype=torch.int32, device=dev),
+                                                 torch.empty(rows, dtype=torch.float32, device=dev))
+    need = lib().lnship_sample_work(rows, vocab)
+    if need < 0:
+        check(need)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    a = SampleArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
+                   _row_values(temperature, rows, torch.float32, "temperature", dev),
+                   _row_values(top_k, rows, torch.int32, "top_k", dev),
+                   _row_values(top_p, rows, torch.float32, "top_p", dev),
+                   _row_values(min_p, rows, torch.float32, "min_p", dev),
+                   _row_values(u, rows, torch.float32, "u", dev),
+                   _row_values(tokens, rows, torch.int32, "tokens", dev),
+                   _row_values(probs, rows, torch.float32, "probs", dev), _p(work), need)
+    check(lib().lnship_sample(ctypes.byref(a), _stream()))
+    return tokens, probs
