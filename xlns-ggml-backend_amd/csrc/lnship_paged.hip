@@ -90,20 +90,24 @@ __global__ __launch_bounds__(k_block) void k_store_paged(store_args s, dev_table
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
 
 struct attn_paged_args {
     lnship_paged_kv kv;
     const float *q;
     float *dst;
-    int64_t q_ld, dst_ld, window;
+    int64_t q_ld, dst_ld;
     float scale;          // times log2 e
-    int n_head, rep, page_sh, splits;
+    int window;           // 0: none
+    int n_head, rep, page_sh, splits, tile_rows;
     float *work;          // [splits][ntok][n_head] rows of head_dim sums, maximum and total
 };
 
 constexpr int k_lo_sh = 11;             // the low halves are scaled by 2^11
 constexpr float k_lo = 2048.0f, k_lo_inv = 1.0f / 2048.0f;
-constexpr float k_p_scale = 16384.0f;   // of the weights as halves
+// the weights as halves are scaled by 2^k_p_sh; a running maximum may lag by
+// k_p_lag binades, so they stay below the largest half
+constexpr int k_p_sh = 10, k_p_lag = 5;
 
 // x, y to a pair of halves, and what the rounding leaves, times 2^11, to
 // another: together 22 bits of each
@@ -120,15 +124,21 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
 // Log 0 (zero) becomes 2^-117, which rounds to zero in both halves.
 __device__ __forceinline__ void decode2(uint32_t w, uint32_t &hi, uint32_t &lo) {
     constexpr uint32_t magic = 0x4b000000u, top = 0x47ffu;   // 2^23; the largest log of a half
-    const uint32_t l0 = min(w & k16_logmask, top), l1 = min((w >> 16) & k16_logmask, top);
+    typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+    const uint32_t l = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(
+        __builtin_bit_cast(ushort2v, w & (k16_logmask << 16 | k16_logmask)), ushort2v{top, top}));
     constexpr float off = -(8388608.0f / 128 + 128 - k_lo_sh);
-    const float x0 = __builtin_amdgcn_exp2f(fmaf(__uint_as_float(magic | l0), 1.0f / 128, off));
-    const float x1 = __builtin_amdgcn_exp2f(fmaf(__uint_as_float(magic | l1), 1.0f / 128, off));
-    const half2v h = {(_Float16)(x0 * k_lo_inv), (_Float16)(x1 * k_lo_inv)};
-    const half2v l = {(_Float16)fmaf((float)h[0], -k_lo, x0), (_Float16)fmaf((float)h[1], -k_lo, x1)};
+    const float x0 = __builtin_amdgcn_exp2f(fmaf(__uint_as_float((l & 0xffffu) | magic), 1.0f / 128, off));
+    const float x1 = __builtin_amdgcn_exp2f(
+        fmaf(__uint_as_float(__builtin_amdgcn_perm(magic, l, 0x07060302u)), 1.0f / 128, off));
+    const half2v h0 = {(_Float16)(x0 * k_lo_inv), (_Float16)(x1 * k_lo_inv)};
+    uint32_t hw = __builtin_bit_cast(uint32_t, h0);
+    asm("" : "+v"(hw));   // one packed conversion, read back as halves
+    const half2v h = __builtin_bit_cast(half2v, hw);
+    const half2v r = {(_Float16)fmaf((float)h[0], -k_lo, x0), (_Float16)fmaf((float)h[1], -k_lo, x1)};
     const uint32_t sg = w & (k16_sign << 16 | k16_sign);
-    hi = __builtin_bit_cast(uint32_t, h) ^ sg;
-    lo = __builtin_bit_cast(uint32_t, l) ^ sg;
+    hi = hw ^ sg;
+    lo = __builtin_bit_cast(uint32_t, r) ^ sg;
 }
 
 union frag {   // a lane's eight halves of a matrix operand
@@ -144,51 +154,104 @@ __device__ __forceinline__ void decode8(uint4 c, frag &hi, frag &lo) {
     decode2(c.w, hi.u[3], lo.u[3]);
 }
 
+// eight weights (scaled by 2^k_p_sh) to their halves, the rest of those, and
+// the halves less the low halves' scale (for the values' low halves)
+__device__ __forceinline__ void split_p(const float *p, frag &ph, frag &pl, frag &pc) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const half2v h0 = {(_Float16)p[j], (_Float16)p[j + 1]};
+        uint32_t hw = __builtin_bit_cast(uint32_t, h0);
+        asm("" : "+v"(hw));
+        const half2v h = __builtin_bit_cast(half2v, hw);
+        const half2v r = {(_Float16)(p[j] - (float)h[0]), (_Float16)(p[j + 1] - (float)h[1])};
+        const half2v c = h * half2v{(_Float16)k_lo_inv, (_Float16)k_lo_inv};
+        ph.u[j / 2] = hw;
+        pl.u[j / 2] = __builtin_bit_cast(uint32_t, r);
+        pc.u[j / 2] = __builtin_bit_cast(uint32_t, c);
+    }
+}
+
 __device__ __forceinline__ float4v mma(const frag &a, const frag &b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b.h, c, 0, 0, 0);
 }
+__device__ __forceinline__ float16v mma(const frag &a, const frag &b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
+}
 
-// A wave takes 16 rows (token and head of one kv head's group) and, of their
-// visible cells, every fourth block of 32; the four waves of a workgroup and
-// the workgroups of a split are joined by their maxima.  Scores are formed
-// transposed, S^T = K Q^T, with the cells dealt to the rows of two 16 x 16
-// products so that a lane's eight scores are eight neighbouring cells of one
-// row: as such they are the operand of O^T = V^T P^T, and both caches' layouts
-// give a lane's share of K and V in 16-byte loads.
-template <int NB>   // 32-wide groups of head_dim
-__global__ __launch_bounds__(256) void k_attn_paged(attn_paged_args a, unsigned long long *err) {
+// A tile of R rows of one sequence (row r: token r / rep, head r % rep of the
+// kv head's group) and the cells that it sees.  Sequence s's tiles start at
+// q_start[s] rep / R + s, which leaves each as many as it may need.
+struct row_tile {
+    int sq, t0, rows, r0;   // its sequence, that one's first token and rows, the tile's first row
+    int pos0;               // position of token t0
+    int c0, c1;             // cells [c0, c1) may be seen, c0 a multiple of 64
+    int blocks, per;        // blocks of 64 of them, and of a split
+};
+// r0 < 0: the tile has no rows.
+__device__ __forceinline__ row_tile find_tile(const attn_paged_args &a, int tile, unsigned long long *err) {
+    const lnship_paged_kv &kv = a.kv;
+    const uint32_t R = (uint32_t)a.tile_rows, rep = (uint32_t)a.rep;
+    auto first_tile = [&](int i) { return (int)((uint32_t)min(max(kv.q_start[i], 0), (int)kv.ntok) * rep / R) + i; };
+    row_tile t;
+    t.sq = last_at_most((int)kv.n_seq, tile, first_tile);
+    t.t0 = min(max(kv.q_start[t.sq], 0), (int)kv.ntok);
+    const int64_t end = kv.q_start[t.sq + 1];
+    t.rows = (int)max(min(end, kv.ntok) - t.t0, (int64_t)0) * a.rep;
+    t.r0 = (tile - first_tile(t.sq)) * a.tile_rows;
+    if (t.r0 >= t.rows) t.r0 = -1;
+    if (t.r0 < 0) return t;
+    const int64_t pos0 = max((int64_t)kv.kv_len[t.sq] - end + t.t0, -((int64_t)1 << 30));
+    const int last = (int)((uint32_t)(min(t.r0 + a.tile_rows, t.rows) - 1) / rep), first = (int)((uint32_t)t.r0 / rep);
+    const int64_t cells = kv.table_ld << a.page_sh;
+    if (err && pos0 + last >= cells && threadIdx.x == 0) index_fault(err, pos0 + last);
+    t.pos0 = (int)min(pos0, ((int64_t)1 << 31) - 1 - t.rows);
+    t.c1 = (int)max(min((int64_t)t.pos0 + last + 1, cells), (int64_t)0);
+    t.c0 = a.window > 0 ? max(0, min(t.pos0 + first - a.window + 1, t.c1)) & ~63 : 0;
+    t.blocks = (t.c1 - t.c0 + 63) >> 6;
+    t.per = max((t.blocks + a.splits - 1) / a.splits, 4);
+    return t;
+}
+
+// A row's finished sums: divided into dst, or (splits) into its part of work.
+struct row_out {
+    float *dst;
+    float f;   // what the sums are multiplied by
+};
+__device__ __forceinline__ row_out out_row(const attn_paged_args &a, int split, int64_t tok, int head, float m, float l) {
+    const int hd = (int)a.kv.head_dim;
+    if (a.splits == 1) return {a.dst + tok * a.dst_ld + (int64_t)head * hd, m == -INFINITY ? 0.0f : 1.0f / l};
+    return {a.work + ((split * a.kv.ntok + tok) * a.n_head + head) * (hd + 2), 1.0f};
+}
+
+// Few rows a sequence (single tokens): a wave takes 16 rows and, of their
+// split's cells, every fourth block of 32; the four waves of a workgroup are
+// joined at the end.  Scores are formed transposed, S^T = K Q^T, with the cells
+// dealt to the rows of two 16 x 16 products so that a lane's eight scores are
+// eight neighbouring cells of one row: as such they are the operand of
+// O^T = V^T P^T, and both caches' layouts give a lane's share of K and V in
+// 16-byte loads, straight from memory.  The next block's keys are loaded while
+// this one's weights are formed, its values once this one's are decoded.
+template <int NB, bool FULL>   // 32-wide groups of head_dim; whether it fills them
+#ifndef LNSHIP_W
+#define LNSHIP_W 2
+#endif
+__global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_attn_paged(attn_paged_args a, unsigned long long *err) {
     const lnship_paged_kv &kv = a.kv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int rep = a.rep, kvh = blockIdx.y, split = blockIdx.z, hd = (int)kv.head_dim;
+    const int rep = a.rep, kvh = blockIdx.y, split = blockIdx.z, hd = (int)kv.head_dim, page = (int)kv.page;
     __shared__ float s_m[4][16], s_l[4][16];
     __shared__ float s_o[16][NB * 32 + 1];
 
-    // the tile's sequence: sequence s's tiles start at q_start[s] rep / 16 + s
-    const int64_t tile = blockIdx.x;
-    const int sq = last_at_most((int)kv.n_seq, tile,
-                                [&](int i) { return (int64_t)max(kv.q_start[i], 0) * rep / 16 + i; });
-    const int64_t t0 = max(kv.q_start[sq], 0), t1 = min((int64_t)kv.q_start[sq + 1], kv.ntok);
-    const int64_t r0 = (tile - (t0 * rep / 16 + sq)) * 16, rows = (t1 - t0) * rep;
-    if (r0 < 0 || r0 >= rows) return;
-    const int64_t pos0 = (int64_t)kv.kv_len[sq] - kv.q_start[sq + 1] + t0;
-    const int64_t cells = kv.table_ld << a.page_sh;
-    const int64_t last = pos0 + (min(r0 + 16, rows) - 1) / rep, first = pos0 + r0 / rep;
-    if (last >= cells && threadIdx.x == 0) index_fault(err, last);
-    const int64_t c1 = min(last + 1, cells);
-    const int64_t c0 = a.window > 0 ? max((int64_t)0, first - a.window + 1) & ~(int64_t)31 : 0;
-    // this split's blocks of 32 cells, at least 8 a split
-    const int64_t blocks = c1 > c0 ? (c1 - c0 + 31) / 32 : 0;
-    const int64_t per = max((blocks + a.splits - 1) / a.splits, (int64_t)8);
-    const int64_t b0 = split * per, b1 = min(b0 + per, blocks);
-    if (split > 0 && b0 >= blocks) return;
+    const row_tile T = find_tile(a, blockIdx.x, err);
+    if (T.r0 < 0 || (split > 0 && split * T.per >= T.blocks)) return;
+    const int cend = min(T.c1, T.c0 + (split + 1) * T.per * 64);
 
     // the lane's row
-    const int64_t row = r0 + n;
-    const bool have = row < rows;
-    const int64_t tok = t0 + (have ? row / rep : 0);
-    const int head = kvh * rep + (have ? (int)(row % rep) : 0);
-    const int64_t pos = pos0 + tok - t0;
-    const int64_t lo_cell = a.window > 0 ? pos - a.window : -1;   // cells at and below are hidden
+    const bool have = T.r0 + n < T.rows;
+    const int row = have ? T.r0 + n : T.r0, tok = T.t0 + (int)((uint32_t)row / (uint32_t)rep);
+    const int head = kvh * rep + (int)((uint32_t)row % (uint32_t)rep);
+    const int pos = min(T.pos0 + tok - T.t0, T.c1 - 1);
+    const int lo_cell = a.window > 0 ? T.pos0 + tok - T.t0 - a.window : -1;   // cells at and below are hidden
 
     // the queries as halves, scaled by the row's largest to at most 2
     frag qh[NB], ql[NB];
@@ -201,7 +264,7 @@ __global__ __launch_bounds__(256) void k_attn_paged(attn_paged_args a, unsigned 
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int d = b * 32 + g * 8 + j;
-                x[b][j] = have && d < hd ? q[d] : 0.0f;
+                x[b][j] = have && (FULL || d < hd) ? q[d] : 0.0f;
                 mx = fmaxf(mx, fabsf(x[b][j]));
             }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
@@ -215,84 +278,105 @@ __global__ __launch_bounds__(256) void k_attn_paged(attn_paged_args a, unsigned 
         qs = ldexpf(a.scale, e);
     }
 
+    const int32_t *table = kv.table + (int64_t)T.sq * kv.table_ld;
+    const int64_t head_codes = (int64_t)page * hd, page_codes = kv.n_head_kv * head_codes;
+    const uint16_t *kbase = kv.k_pages + kvh * head_codes, *vbase = kv.v_pages + kvh * head_codes;
+    // the lane's cells of a block: as a row of the key products (4 of each of
+    // the two), and of its eight scores
+    const int kcell = 8 * (n >> 2), vcell = 8 * g;
+    // a page of cell c, or page 0 (hidden cells: whatever it holds is finite)
+    auto page_of = [&](int c) { return c < cend ? table[c >> a.page_sh] : 0; };
+    auto sound = [&](int id) { return (uint32_t)id < (uint32_t)kv.n_pages; };
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    uint4 kc[2][NB], vc[2 * NB];
+    auto load_k = [&](int cb, int id) {
+        const int c = (cb + kcell) & (page - 1);
+        const uint16_t *k = kbase + (sound(id) ? id : 0) * page_codes + (c + (n & 3)) * 8;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                const int d8 = FULL ? i * 4 + g : min(i * 4 + g, hd / 8 - 1);
+                kc[t][i] = *reinterpret_cast<const uint4 *>(k + (d8 * page + 4 * t) * 8);
+                if (!FULL && (i * 4 + g) * 8 >= hd) kc[t][i] = zero;
+            }
+    };
+    auto load_v = [&](int cb, int id) {
+        const uint16_t *v = vbase + (sound(id) ? id : 0) * page_codes + ((cb + vcell) & (page - 1)) * hd;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            const int d = FULL ? i * 16 + n : min(i * 16 + n, hd - 1);
+            vc[i] = *reinterpret_cast<const uint4 *>(v + d * 8);
+            if (!FULL && i * 16 + n >= hd) vc[i] = zero;
+        }
+    };
+
     float4v o[2 * NB];
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) o[i] = float4v{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
-    const int32_t *table = kv.table + sq * kv.table_ld;
-    for (int64_t b = b0 + wave; b < b1; b += 4) {
-        const int64_t cb = c0 + b * 32;
-        // the lane's cells: as a row of K^T's products, and of its eight scores
-        int64_t kpg = -1, vpg = -1;
-        const int64_t kc = cb + 8 * (n >> 2), vc = cb + 8 * g;
-        if (kc < c1) kpg = table[kc >> a.page_sh];
-        if (vc < c1) vpg = table[vc >> a.page_sh];
-        const bool kok = kc < c1 && kpg >= 0 && kpg < kv.n_pages, vok = vc < c1 && vpg >= 0 && vpg < kv.n_pages;
-        if (vc < c1 && !vok) index_fault(err, vpg);
-        const uint4 zero = make_uint4(0, 0, 0, 0);
+    int cb = T.c0 + split * T.per * 64 + wave * 32;
+    int vid = page_of(cb + vcell), kid = page_of(cb + kcell);
+    if (cb < cend) {
+        load_k(cb, kid);
+        load_v(cb, vid);
+    }
+    for (; cb < cend; cb += 128) {
+        const int vid1 = page_of(cb + 128 + vcell), kid1 = page_of(cb + 128 + kcell);
+        const bool vok = cb + vcell < cend && sound(vid);
+        if (cb + vcell < cend && !vok) index_fault(err, vid);
         float4v sh[2], sx[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             sh[t] = sx[t] = float4v{0, 0, 0, 0};
-            const int64_t cell = (kc & (kv.page - 1)) + 4 * t + (n & 3);
-            const uint16_t *k = kv.k_pages + ((kok ? kpg : 0) * kv.n_head_kv + kvh) * kv.page * hd;
 #pragma unroll
             for (int i = 0; i < NB; i++) {
-                uint4 c = zero;
-                if (kok && i * 32 + g * 8 < hd)
-                    c = *reinterpret_cast<const uint4 *>(k + ((int64_t)(i * 4 + g) * kv.page + cell) * 8);
                 frag kh, kl;
-                decode8(c, kh, kl);
+                decode8(kc[t][i], kh, kl);
                 sh[t] = mma(kh, qh[i], sh[t]);
                 sx[t] = mma(kl, qh[i], sx[t]);
                 sx[t] = mma(kh, ql[i], sx[t]);
             }
         }
+        load_k(min(cb + 128, cend - 1), kid1);
         float s[8], mb = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const int64_t cell = vc + j;
+            const int cell = cb + vcell + j;
             s[j] = (sh[j >> 2][j & 3] + k_lo_inv * sx[j >> 2][j & 3]) * qs;
             if (!vok || cell > pos || cell <= lo_cell) s[j] = -INFINITY;
             mb = fmaxf(mb, s[j]);
         }
-        mb = fmaxf(mb, __shfl_xor(mb, 16));
-        mb = fmaxf(mb, __shfl_xor(mb, 32));
-        const float mn = fmaxf(m, mb), ms = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - ms);
-        m = mn;
+        if (__any(mb > m + k_p_lag)) {   // the first block, and where the maximum has grown far
+            mb = fmaxf(mb, __shfl_xor(mb, 16));
+            mb = fmaxf(mb, __shfl_xor(mb, 32));
+            const float mn = fmaxf(m, mb);
+            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) o[i] *= alpha;
+        }
+        const float ms = (m == -INFINITY ? 0.0f : m) - k_p_sh;
         float p[8];
-        frag ph, pl, pc;
-        l *= alpha;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             p[j] = __builtin_amdgcn_exp2f(s[j] - ms);
             l += p[j];
         }
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const float x = p[j] * k_p_scale, y = p[j + 1] * k_p_scale;
-            const half2v h = {(_Float16)x, (_Float16)y};
-            const half2v r = {(_Float16)(x - (float)h[0]), (_Float16)(y - (float)h[1])};
-            const half2v f = {(_Float16)k_lo_inv, (_Float16)k_lo_inv};
-            const half2v c = h * f;
-            ph.u[j / 2] = __builtin_bit_cast(uint32_t, h);
-            pl.u[j / 2] = __builtin_bit_cast(uint32_t, r);
-            pc.u[j / 2] = __builtin_bit_cast(uint32_t, c);
-        }
-        const uint16_t *v = kv.v_pages + ((vok ? vpg : 0) * kv.n_head_kv + kvh) * kv.page * hd +
-                            ((vc & (kv.page - 1)) >> 3) * hd * 8;
+        frag ph, pl, pc;
+        split_p(p, ph, pl, pc);
 #pragma unroll
         for (int i = 0; i < 2 * NB; i++) {
-            uint4 c = zero;
-            if (vok && i * 16 + n < hd) c = *reinterpret_cast<const uint4 *>(v + (i * 16 + n) * 8);
             frag vh, vl;
-            decode8(c, vh, vl);
-            o[i] *= alpha;
+            decode8(vc[i], vh, vl);
             o[i] = mma(vh, ph, o[i]);
             o[i] = mma(vh, pl, o[i]);
             o[i] = mma(vl, pc, o[i]);
         }
+        load_v(min(cb + 128, cend - 1), vid1);
+        kid = kid1;
+        vid = vid1;
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -304,8 +388,7 @@ __global__ __launch_bounds__(256) void k_attn_paged(attn_paged_args a, unsigned 
     }
     __syncthreads();
     const float M = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
-    const float Ms = M == -INFINITY ? 0.0f : M;
-    const float f = __builtin_amdgcn_exp2f(m - Ms) * (1.0f / k_p_scale);
+    const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
     for (int w = 0; w < 4; w++) {
         if (wave == w) {
 #pragma unroll
@@ -319,62 +402,299 @@ __global__ __launch_bounds__(256) void k_attn_paged(attn_paged_args a, unsigned 
         __syncthreads();
     }
     // a row's elements, on 16 threads
-    const int rr = threadIdx.x >> 4;
-    const int64_t row2 = r0 + rr;
-    if (row2 >= rows) return;
-    const int64_t tok2 = t0 + row2 / rep;
-    const int head2 = kvh * rep + (int)(row2 % rep);
+    const int rr = threadIdx.x >> 4, row2 = T.r0 + rr;
+    if (row2 >= T.rows) return;
+    const int tok2 = T.t0 + (int)((uint32_t)row2 / (uint32_t)rep), head2 = kvh * rep + (int)((uint32_t)row2 % (uint32_t)rep);
     float M2 = -INFINITY, L2 = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; w++) M2 = fmaxf(M2, s_m[w][rr]);
-    const float Ms2 = M2 == -INFINITY ? 0.0f : M2;
+    if (M2 != -INFINITY)
 #pragma unroll
-    for (int w = 0; w < 4; w++) L2 += s_l[w][rr] * __builtin_amdgcn_exp2f(s_m[w][rr] - Ms2);
-    if (a.splits == 1) {
-        const float inv = M2 == -INFINITY ? 0.0f : 1.0f / L2;
-        float *dst = a.dst + tok2 * a.dst_ld + (int64_t)head2 * hd;
-        for (int d = threadIdx.x & 15; d < hd; d += 16) dst[d] = s_o[rr][d] * inv;
-    } else {
-        float *dst = a.work + ((split * kv.ntok + tok2) * a.n_head + head2) * (hd + 2);
-        for (int d = threadIdx.x & 15; d < hd; d += 16) dst[d] = s_o[rr][d];
-        if ((threadIdx.x & 15) == 0) {
-            dst[hd] = M2;
-            dst[hd + 1] = L2;
-        }
+        for (int w = 0; w < 4; w++) L2 += s_l[w][rr] * __builtin_amdgcn_exp2f(s_m[w][rr] - M2);
+    const row_out out = out_row(a, split, tok2, head2, M2, L2);
+    for (int d = threadIdx.x & 15; d < hd; d += 16) out.dst[d] = s_o[rr][d] * out.f;
+    if (a.splits > 1 && (threadIdx.x & 15) == 0) {
+        out.dst[hd] = M2;
+        out.dst[hd + 1] = L2;
     }
 }
 
-// The splits' parts of a row joined, in the splits' order.
-__global__ __launch_bounds__(64) void k_attn_paged_join(attn_paged_args a) {
+// Many rows a sequence (prompts, chunks): NW waves of 32 rows each go over the
+// cells together, 64 at a time.  Every code is decoded once a workgroup, by the
+// thread that loaded it, into split halves in LDS, in the order in which the
+// products read them: each operand is one 16-byte read a lane of consecutive
+// addresses.  Products are 32 x 32 x 16, transposed as above; a lane has 16
+// scores of one row.  Two LDS buffers: while one is multiplied the next tile's
+// codes are in flight; they are decoded into the other before the barrier.
+template <int NB, int NW>   // 32-wide groups of head_dim; waves
+__global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsigned long long *err) {
+    constexpr int HD = NB * 32, NT = NW * 64, KK = HD / 16;
+    constexpr int U = 64 * HD / 8;        // 16-byte units of a tile's keys, and of its values
+    constexpr int UT = (U + NT - 1) / NT; // of a thread
+    extern __shared__ uint4 s_tile[];     // [2][keys high, low, values high, low][U]
+    __shared__ alignas(16) int s_ok[2][8];   // whether a tile's groups of eight cells lie in a page
     const lnship_paged_kv &kv = a.kv;
-    const int64_t tok = blockIdx.x;
-    const int head = blockIdx.y, hd = (int)kv.head_dim, n_seq = (int)kv.n_seq;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, h = lane >> 5;
+    const int rep = a.rep, nkv = (int)kv.n_head_kv, hd = (int)kv.head_dim, page = (int)kv.page;
+    // kv heads side by side (on the XCDs' L2s), the last tiles (most cells) first
+    const int kvh = (int)(blockIdx.x % (uint32_t)nkv), split = blockIdx.y;
+    const int tile = (int)(gridDim.x / (uint32_t)nkv) - 1 - (int)(blockIdx.x / (uint32_t)nkv);
+    const row_tile T = find_tile(a, tile, err);
+    if (T.r0 < 0 || (split > 0 && split * T.per >= T.blocks)) return;
+    const int cbeg = T.c0 + split * T.per * 64, cend = min(T.c1, cbeg + T.per * 64);
+
+    const int wrow = T.r0 + wave * 32;   // the wave's rows
+    const bool have = wrow + n < T.rows;
+    const int row = have ? wrow + n : min(wrow, T.rows - 1), tok = T.t0 + (int)((uint32_t)row / (uint32_t)rep);
+    const int head = kvh * rep + (int)((uint32_t)row % (uint32_t)rep);
+    const int pos = min(T.pos0 + tok - T.t0, T.c1 - 1);
+    const int lo_cell = a.window > 0 ? T.pos0 + tok - T.t0 - a.window : -1;
+    // what all of the wave's rows see, and any does
+    const int wfirst = T.pos0 + (int)((uint32_t)min(wrow, T.rows - 1) / (uint32_t)rep);
+    const int wlast = T.pos0 + (int)((uint32_t)(min(wrow + 32, T.rows) - 1) / (uint32_t)rep);
+    const int all_lo = a.window > 0 ? wlast - a.window : -1, any_lo = a.window > 0 ? wfirst - a.window : -1;
+    const bool wave_has = wrow < T.rows;
+
+    frag qh[KK], ql[KK];
+    float qs;
+    {
+        float mx = 0.0f;
+        const float *q = a.q + tok * a.q_ld + (int64_t)head * hd;
+        auto load = [&](int kk, int j) {
+            const int d = kk * 16 + h * 8 + j;
+            return have && d < hd ? q[d] : 0.0f;
+        };
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(load(kk, j)));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const int e = (int)(f32_bits(mx) >> 23) - 127;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+                split2(ldexpf(load(kk, j), -e), ldexpf(load(kk, j + 1), -e), qh[kk].u[j / 2], ql[kk].u[j / 2]);
+        qs = ldexpf(a.scale, e);
+    }
+
+    const int32_t *table = kv.table + (int64_t)T.sq * kv.table_ld;
+    const int64_t head_codes = (int64_t)page * hd, page_codes = nkv * head_codes;
+    const uint16_t *kbase = kv.k_pages + kvh * head_codes, *vbase = kv.v_pages + kvh * head_codes;
+    auto page_of = [&](int c) { return c < cend ? table[c >> a.page_sh] : 0; };
+    auto sound = [&](int id) { return (uint32_t)id < (uint32_t)kv.n_pages; };
+    // unit u of the keys: dims u / 64 * 8.., cell u % 64 of the tile (the same
+    // for all of a thread's); of the values: cells u / HD * 8.., dim u % HD
+    uint4 kc[UT], vc[UT];
+    int kid, vid[UT];
+    auto has = [&](int i) { return (i + 1) * NT <= U || tid + i * NT < U; };   // the thread's last unit may not be one
+    auto pages = [&](int cb) {
+        kid = page_of(cb + (tid & 63));
+#pragma unroll
+        for (int i = 0; i < UT; i++) vid[i] = has(i) ? page_of(cb + (tid + i * NT) / HD * 8) : 0;
+    };
+    auto load = [&](int cb) {
+        const uint16_t *k = kbase + (sound(kid) ? kid : 0) * page_codes + ((cb + (tid & 63)) & (page - 1)) * 8;
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            const int d8 = (tid + i * NT) >> 6;
+            kc[i] = *reinterpret_cast<const uint4 *>(k + min(d8, hd / 8 - 1) * page * 8);
+            if (d8 * 8 >= hd) kc[i] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            const int c8 = (tid + i * NT) / HD, d = (tid + i * NT) % HD;
+            const uint16_t *v = vbase + (sound(vid[i]) ? vid[i] : 0) * page_codes + ((cb + c8 * 8) & (page - 1)) * hd;
+            vc[i] = *reinterpret_cast<const uint4 *>(v + min(d, hd - 1) * 8);
+            if (d >= hd) vc[i] = make_uint4(0, 0, 0, 0);
+        }
+    };
+    // the cell's row of its block's key product: a lane's 16 results are then
+    // cells 8 h + 0..7 and 16 + 8 h + 0..7 of the block
+    const int kcell = tid & 63, kin = kcell & 31;
+    const int krow = 8 * ((kin >> 4) * 2 + ((kin >> 2) & 1)) + 4 * ((kin >> 3) & 1) + (kin & 3);
+    auto store = [&](int buf, int cb, const int *ids) {
+        uint4 *s = s_tile + buf * 4 * U;
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            frag hi, lo;
+            decode8(kc[i], hi, lo);
+            if (!has(i)) continue;
+            const int d8 = (tid + i * NT) >> 6;
+            const int at = (kcell >> 5) * (U / 2) + (d8 >> 1) * 64 + (d8 & 1) * 32 + krow;
+            s[at] = hi.w;
+            s[U + at] = lo.w;
+        }
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            frag hi, lo;
+            decode8(vc[i], hi, lo);
+            if (!has(i)) continue;
+            const int c8 = (tid + i * NT) / HD, d = (tid + i * NT) % HD;
+            const int at = (c8 >> 2) * (U / 2) + (d >> 5) * 128 + ((c8 >> 1) & 1) * 64 + (c8 & 1) * 32 + (d & 31);
+            s[2 * U + at] = hi.w;
+            s[3 * U + at] = lo.w;
+            if (d == 0) {
+                const int c = cb + c8 * 8;
+                s_ok[buf][c8] = c < cend && sound(ids[i]);
+                if (c < cend && !sound(ids[i])) index_fault(err, ids[i]);
+            }
+        }
+    };
+
+    float16v o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) o[i] = float16v{};
+    float m = -INFINITY, l = 0.0f;
+    int ids[UT];
+    if (cbeg < cend) {
+        pages(cbeg);
+        load(cbeg);
+#pragma unroll
+        for (int i = 0; i < UT; i++) ids[i] = vid[i];
+        pages(cbeg + 64);
+        store(0, cbeg, ids);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
+        const bool more = cb + 64 < cend;
+        if (more) {
+            load(cb + 64);
+#pragma unroll
+            for (int i = 0; i < UT; i++) ids[i] = vid[i];
+            pages(cb + 128);
+        }
+        if (wave_has) {
+            const frag *s = reinterpret_cast<const frag *>(s_tile + buf * 4 * U) + lane;
+#pragma unroll 1
+            for (int blk = 0; blk < 2; blk++) {
+                const int b0 = cb + blk * 32;
+                if (b0 > wlast || b0 + 31 <= any_lo) continue;
+                float16v sh{}, sx{};
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++) {
+                    const frag kh = s[blk * (U / 2) + kk * 64], kl = s[U + blk * (U / 2) + kk * 64];
+                    sh = mma(kh, qh[kk], sh);
+                    sx = mma(kl, qh[kk], sx);
+                    sx = mma(kh, ql[kk], sx);
+                }
+                const int4 ok = *reinterpret_cast<const int4 *>(&s_ok[buf][blk * 4]);
+                float p[16], mb = -INFINITY;
+                const float sub = (m == -INFINITY ? 0.0f : m) - k_p_sh;
+#pragma unroll
+                for (int j = 0; j < 16; j++) p[j] = fmaf(sx[j], qs * k_lo_inv, fmaf(sh[j], qs, -sub));
+                if (b0 + 31 > wfirst || b0 + 31 >= T.c1 || b0 <= all_lo || !(ok.x & ok.y & ok.z & ok.w)) {
+                    const bool ok0 = h ? ok.y : ok.x, ok1 = h ? ok.w : ok.z;
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const int cell = b0 + (j >> 3) * 16 + h * 8 + (j & 7);
+                        if (!(j < 8 ? ok0 : ok1) || cell > pos || cell <= lo_cell) p[j] = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j++) mb = fmaxf(mb, p[j]);
+                // p holds the scores less sub: the first block, and where the maximum has grown far
+                if (__any(m == -INFINITY ? mb != -INFINITY : mb > (float)(k_p_sh + k_p_lag))) {
+                    mb = fmaxf(mb, __shfl_xor(mb, 32));
+                    const float mn = fmaxf(m, mb + sub);
+                    const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                    const float more_sub = (mn == -INFINITY ? 0.0f : mn) - k_p_sh - sub;
+#pragma unroll
+                    for (int j = 0; j < 16; j++) p[j] -= more_sub;
+                    m = mn;
+                    l *= alpha;
+#pragma unroll
+                    for (int i = 0; i < NB; i++) o[i] *= alpha;
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    p[j] = __builtin_amdgcn_exp2f(p[j]);
+                    l += p[j];
+                }
+                frag ph[2], pl[2], pc[2];
+                split_p(p, ph[0], pl[0], pc[0]);
+                split_p(p + 8, ph[1], pl[1], pc[1]);
+#pragma unroll
+                for (int i = 0; i < NB; i++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const int at = blk * (U / 2) + i * 128 + t * 64;
+                        const frag vh = s[2 * U + at], vl = s[3 * U + at];
+                        o[i] = mma(vh, ph[t], o[i]);
+                        o[i] = mma(vh, pl[t], o[i]);
+                        o[i] = mma(vl, pc[t], o[i]);
+                    }
+            }
+        }
+        if (more) store(buf ^ 1, cb + 64, ids);
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32);
+    if (!have) return;
+    const row_out out = out_row(a, split, tok, head, m, l);
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int d = i * 32 + 8 * (j >> 2) + 4 * h + (j & 3);
+            if (d < hd) out.dst[d] = o[i][j] * out.f;
+        }
+    if (a.splits > 1 && h == 0) {
+        out.dst[hd] = m;
+        out.dst[hd + 1] = l;
+    }
+}
+
+// The splits' parts of a row joined, in a fixed order: a wave takes every
+// fourth part.
+__global__ __launch_bounds__(256) void k_attn_paged_join(attn_paged_args a) {
+    __shared__ float s_f[256], s_o[4][256], s_red[4];
+    const lnship_paged_kv &kv = a.kv;
+    const int tok = blockIdx.x, head = blockIdx.y, hd = (int)kv.head_dim, n_seq = (int)kv.n_seq, tid = threadIdx.x;
+    const int lane = tid & 63, wave = tid >> 6;
     if (tok < kv.q_start[0] || tok >= kv.q_start[n_seq]) return;
     const int sq = last_at_most(n_seq, tok, [&](int i) { return kv.q_start[i]; });
-    const int64_t t0 = max(kv.q_start[sq], 0), t1 = min((int64_t)kv.q_start[sq + 1], kv.ntok);
-    const int64_t pos0 = (int64_t)kv.kv_len[sq] - kv.q_start[sq + 1] + t0;
-    // the splits that the row's tile had, as k_attn_paged finds them
-    const int64_t rows = (t1 - t0) * a.rep, r0 = ((tok - t0) * a.rep + head % a.rep) & ~(int64_t)15;
-    const int64_t last = pos0 + (min(r0 + 16, rows) - 1) / a.rep, first = pos0 + r0 / a.rep;
-    const int64_t c1 = min(last + 1, kv.table_ld << a.page_sh);
-    const int64_t c0 = a.window > 0 ? max((int64_t)0, first - a.window + 1) & ~(int64_t)31 : 0;
-    const int64_t blocks = c1 > c0 ? (c1 - c0 + 31) / 32 : 0;
-    const int64_t per = max((blocks + a.splits - 1) / a.splits, (int64_t)8);
-    const int used = (int)max((blocks + per - 1) / per, (int64_t)1);
+    const int t0 = min(max(kv.q_start[sq], 0), (int)kv.ntok);
+    const uint32_t R = (uint32_t)a.tile_rows, rep = (uint32_t)a.rep;
+    const int tile = (int)((uint32_t)t0 * rep / R) + sq + (int)((uint32_t)((tok - t0) * a.rep + head % a.rep) / R);
+    // (an unsound q_start may give no such tile; faults are recorded by then)
+    const row_tile T = find_tile(a, tile, nullptr);
+    if (T.r0 < 0) return;
+    const int used = max((T.blocks + T.per - 1) / T.per, 1);
     const int64_t step = kv.ntok * a.n_head * (hd + 2);
-    const float *w = a.work + (tok * a.n_head + head) * (hd + 2);
-    float M = -INFINITY;
-    for (int i = 0; i < used; i++) M = fmaxf(M, w[i * step + hd]);
-    const float Ms = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f;
-    for (int i = 0; i < used; i++) L += w[i * step + hd + 1] * __builtin_amdgcn_exp2f(w[i * step + hd] - Ms);
-    const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
-    float *dst = a.dst + tok * a.dst_ld + (int64_t)head * hd;
-    for (int d = threadIdx.x; d < hd; d += 64) {
-        float s = 0.0f;
-        for (int i = 0; i < used; i++) s += w[i * step + d] * __builtin_amdgcn_exp2f(w[i * step + hd] - Ms);
-        dst[d] = s * inv;
+    const float *w = a.work + ((int64_t)tok * a.n_head + head) * (hd + 2);
+    const float mi = tid < used ? w[tid * step + hd] : -INFINITY;
+    const float li = tid < used ? w[tid * step + hd + 1] : 0.0f;
+    auto reduce = [&](float v, bool sum) {
+        for (int d = 32; d; d >>= 1) {
+            const float y = __shfl_xor(v, d);
+            v = sum ? v + y : fmaxf(v, y);
+        }
+        __syncthreads();
+        if (lane == 0) s_red[wave] = v;
+        __syncthreads();
+        return sum ? s_red[0] + s_red[1] + s_red[2] + s_red[3]
+                   : fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    };
+    const float M = reduce(mi, false);
+    const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - M);
+    s_f[tid] = f;
+    const float L = reduce(li * f, true);
+    float s[4] = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int i = wave; i < used; i += 4) {
+        const float fi = s_f[i];
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            if (q * 64 + lane < hd) s[q] = fmaf(w[i * step + q * 64 + lane], fi, s[q]);
     }
+#pragma unroll
+    for (int q = 0; q < 4; q++) s_o[wave][q * 64 + lane] = s[q];
+    __syncthreads();
+    if (tid < hd)
+        a.dst[tok * a.dst_ld + (int64_t)head * hd + tid] =
+            (s_o[0][tid] + s_o[1][tid] + s_o[2][tid] + s_o[3][tid]) * (M == -INFINITY ? 0.0f : 1.0f / L);
 }
 
 // ---- host -----------------------------------------------------------------------
@@ -389,7 +709,7 @@ static int check_paged(const lnship_paged_kv *kv, bool ptrs) {
         return fail(LNSHIP_EINVAL, "paged cache: head_dim not a multiple of 8 up to 256%s");
     // (a grid's threads along x are counted in 32 bits)
     if (kv->ntok > 0xffffff || kv->n_seq > 0x7fffff || kv->n_head_kv > 65535 || kv->n_pages > 0x7fffffff ||
-        kv->table_ld > 0x7fffffff / kv->page)
+        kv->table_ld > 0x3fffffff / kv->page)
         return fail(LNSHIP_ERANGE, "paged cache: too large%s");
     if (ptrs && kv->ntok && kv->n_seq) {
         if (!kv->k_pages || !kv->v_pages || !kv->q_start || !kv->kv_len || (!kv->table && kv->table_ld))
@@ -406,18 +726,58 @@ static int log2_of(int64_t page) {
     return sh;
 }
 
-static int64_t attn_tiles(const lnship_paged_kv *kv, int64_t rep) { return kv->ntok * rep / 16 + kv->n_seq; }
-
-// Parts that a row's cells are split into: where there are few tiles, as many
-// as give every CU two workgroups, each of at least 8 blocks of 32 cells.
-static int attn_splits(const lnship_paged_kv *kv, int64_t rep, int cus) {
-    const int64_t wgs = std::max<int64_t>(1, attn_tiles(kv, rep) * kv->n_head_kv);
-    const int64_t most = (kv->table_ld * kv->page + 255) / 256;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + wgs - 1) / wgs, most, 256}));
+// How a call runs: k_attn_chunk with `waves` waves, or (0) k_attn_paged; rows
+// of a tile, tiles, and the parts that a row's cells are split into.
+struct attn_plan {
+    int waves, tile_rows, splits;
+    int64_t tiles;
+};
+#ifndef LNSHIP_TGT
+#define LNSHIP_TGT 16
+#define LNSHIP_TGT2 2
+#endif
+#ifndef LNSHIP_CHUNK_ROWS
+#define LNSHIP_CHUNK_ROWS 64
+#define LNSHIP_CHUNK_ROWS8 384
+#endif
+static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
+    attn_plan p;
+    const int64_t rows = kv->ntok * rep, of_seq = kv->n_seq ? rows / kv->n_seq : 0;
+    p.waves = kv->head_dim > 128 || of_seq < LNSHIP_CHUNK_ROWS ? 0 : of_seq < LNSHIP_CHUNK_ROWS8 ? 4 : 8;
+    p.tile_rows = p.waves ? p.waves * 32 : 16;
+    p.tiles = rows / p.tile_rows + kv->n_seq;
+    const int64_t wgs = std::max<int64_t>(1, p.tiles * kv->n_head_kv);
+    const int64_t most = (kv->table_ld * kv->page + 255) / 256, want = p.waves ? LNSHIP_TGT2 : LNSHIP_TGT;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want * cus + wgs - 1) / wgs, most, 256}));
+    return p;
 }
 
 static int64_t attn_work(const lnship_paged_kv *kv, int64_t n_head, int splits) {
     return splits > 1 ? (int64_t)splits * kv->ntok * n_head * (kv->head_dim + 2) * 4 : 0;
+}
+
+template <int NB, int NW>
+static int launch_chunk(const attn_paged_args &m, const attn_plan &p, hipStream_t s, unsigned long long *err) {
+    const int lds = 2 * 4 * 64 * NB * 32 * 2;
+    LNSHIP_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_chunk<NB, NW>),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL((k_attn_chunk<NB, NW>), dim3((unsigned)(p.tiles * m.kv.n_head_kv), (unsigned)p.splits),
+                       dim3(NW * 64), lds, s, m, err);
+    LNSHIP_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int NB>
+static int launch_attn(const attn_paged_args &m, const attn_plan &p, hipStream_t s, unsigned long long *err) {
+    if constexpr (NB <= 4) {
+        if (p.waves == 4) return launch_chunk<NB, 4>(m, p, s, err);
+        if (p.waves == 8) return launch_chunk<NB, 8>(m, p, s, err);
+    }
+    const dim3 grid((unsigned)p.tiles, (unsigned)m.kv.n_head_kv, (unsigned)p.splits);
+    if (m.kv.head_dim == NB * 32) hipLaunchKernelGGL((k_attn_paged<NB, true>), grid, dim3(256), 0, s, m, err);
+    else hipLaunchKernelGGL((k_attn_paged<NB, false>), grid, dim3(256), 0, s, m, err);
+    LNSHIP_HIP(hipGetLastError());
+    return 0;
 }
 
 }  // namespace lnship
@@ -453,7 +813,7 @@ int64_t lnship16_attn_paged_work(const lnship_paged_kv *kv, int64_t n_head) {
         return fail(LNSHIP_EINVAL, "attn_paged: n_head not a multiple of n_head_kv%s");
     device_state *st = state();
     if (!st) return LNSHIP_ENOINIT;
-    return attn_work(kv, n_head, attn_splits(kv, n_head / kv->n_head_kv, st->cus));
+    return attn_work(kv, n_head, plan_attn(kv, n_head / kv->n_head_kv, st->cus).splits);
 }
 
 int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args *a, void *stream) {
@@ -468,34 +828,31 @@ int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args 
     device_state *st = state();
     if (!st) return LNSHIP_ENOINIT;
     const int64_t rep = a->n_head / kv->n_head_kv;
-    const int splits = attn_splits(kv, rep, st->cus);
-    const int64_t need = attn_work(kv, a->n_head, splits), tiles = attn_tiles(kv, rep);
+    const attn_plan p = plan_attn(kv, rep, st->cus);
+    const int64_t need = attn_work(kv, a->n_head, p.splits);
     if (need && (!a->work || a->work_bytes < (size_t)need || ((uintptr_t)a->work & 15)))
         return fail(LNSHIP_EINVAL, "attn_paged: work smaller than lnship16_attn_paged_work or not aligned%s");
-    if (tiles > 0xffffff) return fail(LNSHIP_ERANGE, "attn_paged: grid too large%s");
-    attn_paged_args m{*kv, a->q, a->dst, q_ld, dst_ld, std::min<int64_t>(a->window, (int64_t)1 << 40),
-                      a->scale * 1.44269504088896341f, (int)a->n_head, (int)rep, log2_of(kv->page), splits,
-                      (float *)a->work};
-    const dim3 grid((unsigned)tiles, (unsigned)kv->n_head_kv, (unsigned)splits), block(256);
+    if (kv->ntok * rep > 0xfffffff || p.tiles * kv->n_head_kv > 0x7fffff)
+        return fail(LNSHIP_ERANGE, "attn_paged: grid too large%s");
+    attn_paged_args m{*kv, a->q, a->dst, q_ld, dst_ld, a->scale * 1.44269504088896341f,
+                      a->window > 0x3fffffff ? 0 : (int)a->window, (int)a->n_head, (int)rep, log2_of(kv->page), p.splits,
+                      p.tile_rows, (float *)a->work};
+    if (kv->n_pages == 0) m.kv.table_ld = 0;   // no page to read: no cells
     hipStream_t s = (hipStream_t)stream;
+    int rc;
     switch ((kv->head_dim + 31) / 32) {
-#define LNSHIP_ATTN(NB) \
-    case NB: hipLaunchKernelGGL(k_attn_paged<NB>, grid, block, 0, s, m, st->index_err); break
-        LNSHIP_ATTN(1);
-        LNSHIP_ATTN(2);
-        LNSHIP_ATTN(3);
-        LNSHIP_ATTN(4);
-        LNSHIP_ATTN(5);
-        LNSHIP_ATTN(6);
-        LNSHIP_ATTN(7);
-        default: hipLaunchKernelGGL(k_attn_paged<8>, grid, block, 0, s, m, st->index_err);
-#undef LNSHIP_ATTN
+        case 1: rc = launch_attn<1>(m, p, s, st->index_err); break;
+        case 2: rc = launch_attn<2>(m, p, s, st->index_err); break;
+        case 3: rc = launch_attn<3>(m, p, s, st->index_err); break;
+        case 4: rc = launch_attn<4>(m, p, s, st->index_err); break;
+        case 5: rc = launch_attn<5>(m, p, s, st->index_err); break;
+        case 6: rc = launch_attn<6>(m, p, s, st->index_err); break;
+        case 7: rc = launch_attn<7>(m, p, s, st->index_err); break;
+        default: rc = launch_attn<8>(m, p, s, st->index_err);
     }
+    if (rc || p.splits == 1) return rc;
+    hipLaunchKernelGGL(k_attn_paged_join, dim3((unsigned)kv->ntok, (unsigned)a->n_head), dim3(256), 0, s, m);
     LNSHIP_HIP(hipGetLastError());
-    if (splits > 1) {
-        hipLaunchKernelGGL(k_attn_paged_join, dim3((unsigned)kv->ntok, (unsigned)a->n_head), dim3(64), 0, s, m);
-        LNSHIP_HIP(hipGetLastError());
-    }
     return 0;
 }
 
