@@ -99,8 +99,13 @@ struct attn_paged_args {
     int64_t q_ld, dst_ld;
     float scale;          // times log2 e
     int window;           // 0: none
-    int n_head, rep, page_sh, splits, tile_rows;
-    float *work;          // [splits][ntok][n_head] rows of head_dim sums, maximum and total
+    int n_head, rep, page_sh, splits, tile_rows, min_per;
+    bool vec;             // the queries' rows are 16-byte aligned
+    // splits: sums [splits][ntok][n_head][head_dim], (maximum, total) [splits][ntok][n_head],
+    // parts that a row has [ntok][n_head]
+    float *sums;
+    float2 *stats;
+    int *used;
 };
 
 constexpr int k_lo_sh = 11;             // the low halves are scaled by 2^11
@@ -118,27 +123,40 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
+// (x k as a half, y k as a half) in a word, one rounding each
+__device__ __forceinline__ uint32_t scaled_halves(float x, float y, float k) {
+    uint32_t r;
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,0,0]" : "=v"(r) : "v"(x), "s"(k));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,0,0]" : "+v"(r) : "v"(y), "s"(k));
+    return r;
+}
+// the halves of h times k, less x and y: (x - k h0, y - k h1) as halves
+__device__ __forceinline__ uint32_t rest_halves(uint32_t h, float k, float x, float y) {
+    uint32_t r;
+    asm("v_fma_mixlo_f16 %0, %1, -%2, %3 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "s"(k), "v"(x));
+    asm("v_fma_mixhi_f16 %0, %1, -%2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(r) : "v"(h), "s"(k), "v"(y));
+    return r;
+}
+
 // Two xlns16 codes in a word to the split halves of their values.  The log
 // field goes into the mantissa of 2^23 + log, one FMA makes it the exponent;
 // 2^11 times the value stays within F32 and the split needs no other product.
-// Log 0 (zero) becomes 2^-117, which rounds to zero in both halves.
+// Log 0 (zero) becomes 2^-117, which rounds to zero in both halves.  Ten issue
+// slots a code, four of them the power.
 __device__ __forceinline__ void decode2(uint32_t w, uint32_t &hi, uint32_t &lo) {
     constexpr uint32_t magic = 0x4b000000u, top = 0x47ffu;   // 2^23; the largest log of a half
     typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
     const uint32_t l = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(
         __builtin_bit_cast(ushort2v, w & (k16_logmask << 16 | k16_logmask)), ushort2v{top, top}));
     constexpr float off = -(8388608.0f / 128 + 128 - k_lo_sh);
-    const float x0 = __builtin_amdgcn_exp2f(fmaf(__uint_as_float((l & 0xffffu) | magic), 1.0f / 128, off));
+    const float x0 = __builtin_amdgcn_exp2f(
+        fmaf(__uint_as_float(__builtin_amdgcn_perm(magic, l, 0x07060100u)), 1.0f / 128, off));
     const float x1 = __builtin_amdgcn_exp2f(
         fmaf(__uint_as_float(__builtin_amdgcn_perm(magic, l, 0x07060302u)), 1.0f / 128, off));
-    const half2v h0 = {(_Float16)(x0 * k_lo_inv), (_Float16)(x1 * k_lo_inv)};
-    uint32_t hw = __builtin_bit_cast(uint32_t, h0);
-    asm("" : "+v"(hw));   // one packed conversion, read back as halves
-    const half2v h = __builtin_bit_cast(half2v, hw);
-    const half2v r = {(_Float16)fmaf((float)h[0], -k_lo, x0), (_Float16)fmaf((float)h[1], -k_lo, x1)};
+    const uint32_t h = scaled_halves(x0, x1, k_lo_inv), r = rest_halves(h, k_lo, x0, x1);
     const uint32_t sg = w & (k16_sign << 16 | k16_sign);
-    hi = hw ^ sg;
-    lo = __builtin_bit_cast(uint32_t, r) ^ sg;
+    hi = h ^ sg;
+    lo = r ^ sg;
 }
 
 union frag {   // a lane's eight halves of a matrix operand
@@ -159,14 +177,11 @@ __device__ __forceinline__ void decode8(uint4 c, frag &hi, frag &lo) {
 __device__ __forceinline__ void split_p(const float *p, frag &ph, frag &pl, frag &pc) {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-        const half2v h0 = {(_Float16)p[j], (_Float16)p[j + 1]};
-        uint32_t hw = __builtin_bit_cast(uint32_t, h0);
-        asm("" : "+v"(hw));
-        const half2v h = __builtin_bit_cast(half2v, hw);
-        const half2v r = {(_Float16)(p[j] - (float)h[0]), (_Float16)(p[j + 1] - (float)h[1])};
+        const half2v h = {(_Float16)p[j], (_Float16)p[j + 1]};
+        const uint32_t hw = __builtin_bit_cast(uint32_t, h), r = rest_halves(hw, 1.0f, p[j], p[j + 1]);
         const half2v c = h * half2v{(_Float16)k_lo_inv, (_Float16)k_lo_inv};
         ph.u[j / 2] = hw;
-        pl.u[j / 2] = __builtin_bit_cast(uint32_t, r);
+        pl.u[j / 2] = r;
         pc.u[j / 2] = __builtin_bit_cast(uint32_t, c);
     }
 }
@@ -208,19 +223,41 @@ __device__ __forceinline__ row_tile find_tile(const attn_paged_args &a, int tile
     t.c1 = (int)max(min((int64_t)t.pos0 + last + 1, cells), (int64_t)0);
     t.c0 = a.window > 0 ? max(0, min(t.pos0 + first - a.window + 1, t.c1)) & ~63 : 0;
     t.blocks = (t.c1 - t.c0 + 63) >> 6;
-    t.per = max((t.blocks + a.splits - 1) / a.splits, 4);
+    t.per = max((t.blocks + a.splits - 1) / a.splits, a.min_per);
     return t;
 }
 
-// A row's finished sums: divided into dst, or (splits) into its part of work.
+// Where a row's sums go, and what they are multiplied by: divided into dst,
+// or (splits) as they are into their part of the workspace, with the row's
+// maximum and total (first: by the thread that writes those).
 struct row_out {
     float *dst;
-    float f;   // what the sums are multiplied by
+    float f;
 };
-__device__ __forceinline__ row_out out_row(const attn_paged_args &a, int split, int64_t tok, int head, float m, float l) {
+__device__ __forceinline__ row_out out_row(const attn_paged_args &a, const row_tile &t, int split, int64_t tok, int head,
+                                           float m, float l, bool first) {
     const int hd = (int)a.kv.head_dim;
     if (a.splits == 1) return {a.dst + tok * a.dst_ld + (int64_t)head * hd, m == -INFINITY ? 0.0f : 1.0f / l};
-    return {a.work + ((split * a.kv.ntok + tok) * a.n_head + head) * (hd + 2), 1.0f};
+    const int64_t row = tok * a.n_head + head, part = split * a.kv.ntok * a.n_head + row;
+    if (first) {
+        a.stats[part] = make_float2(m, l);
+        if (split == 0) a.used[row] = max((t.blocks + t.per - 1) / t.per, 1);
+    }
+    return {a.sums + part * hd, 1.0f};
+}
+
+// eight queries of a row from dim d on (zeros past head_dim)
+__device__ __forceinline__ void load_q(const float *q, int d, int hd, bool vec, float *x) {
+    if (d >= hd) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = 0.0f;
+    } else if (vec) {
+        const float4 u = *reinterpret_cast<const float4 *>(q + d), v = *reinterpret_cast<const float4 *>(q + d + 4);
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = q[d + j];
+    }
 }
 
 // Few rows a sequence (single tokens): a wave takes 16 rows and, of their
@@ -260,13 +297,11 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
         float x[NB][8], mx = 0.0f;
         const float *q = a.q + tok * a.q_ld + (int64_t)head * hd;
 #pragma unroll
+        for (int b = 0; b < NB; b++) load_q(q, b * 32 + g * 8, FULL ? NB * 32 : hd, a.vec, x[b]);
+#pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int d = b * 32 + g * 8 + j;
-                x[b][j] = have && (FULL || d < hd) ? q[d] : 0.0f;
-                mx = fmaxf(mx, fabsf(x[b][j]));
-            }
+            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[b][j]));
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const int e = (int)(f32_bits(mx) >> 23) - 127;   // -127 for zeros
@@ -411,12 +446,8 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
     if (M2 != -INFINITY)
 #pragma unroll
         for (int w = 0; w < 4; w++) L2 += s_l[w][rr] * __builtin_amdgcn_exp2f(s_m[w][rr] - M2);
-    const row_out out = out_row(a, split, tok2, head2, M2, L2);
+    const row_out out = out_row(a, T, split, tok2, head2, M2, L2, (threadIdx.x & 15) == 0);
     for (int d = threadIdx.x & 15; d < hd; d += 16) out.dst[d] = s_o[rr][d] * out.f;
-    if (a.splits > 1 && (threadIdx.x & 15) == 0) {
-        out.dst[hd] = M2;
-        out.dst[hd + 1] = L2;
-    }
 }
 
 // Many rows a sequence (prompts, chunks): NW waves of 32 rows each go over the
@@ -458,23 +489,21 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     frag qh[KK], ql[KK];
     float qs;
     {
-        float mx = 0.0f;
+        float x[KK][8], mx = 0.0f;
         const float *q = a.q + tok * a.q_ld + (int64_t)head * hd;
-        auto load = [&](int kk, int j) {
-            const int d = kk * 16 + h * 8 + j;
-            return have && d < hd ? q[d] : 0.0f;
-        };
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) load_q(q, kk * 16 + h * 8, hd, a.vec, x[kk]);
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(load(kk, j)));
+            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[kk][j]));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const int e = (int)(f32_bits(mx) >> 23) - 127;
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
 #pragma unroll
             for (int j = 0; j < 8; j += 2)
-                split2(ldexpf(load(kk, j), -e), ldexpf(load(kk, j + 1), -e), qh[kk].u[j / 2], ql[kk].u[j / 2]);
+                split2(ldexpf(x[kk][j], -e), ldexpf(x[kk][j + 1], -e), qh[kk].u[j / 2], ql[kk].u[j / 2]);
         qs = ldexpf(a.scale, e);
     }
 
@@ -584,7 +613,9 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
                 const float sub = (m == -INFINITY ? 0.0f : m) - k_p_sh;
 #pragma unroll
                 for (int j = 0; j < 16; j++) p[j] = fmaf(sx[j], qs * k_lo_inv, fmaf(sh[j], qs, -sub));
-                if (b0 + 31 > wfirst || b0 + 31 >= T.c1 || b0 <= all_lo || !(ok.x & ok.y & ok.z & ok.w)) {
+                const int ok_all = __builtin_amdgcn_readfirstlane(ok.x & ok.y & ok.z & ok.w);
+                if (b0 + 31 > wfirst || b0 + 31 >= T.c1 || b0 <= all_lo || !ok_all) {
+                    asm volatile("");   // a branch: few blocks need it
                     const bool ok0 = h ? ok.y : ok.x, ok1 = h ? ok.w : ok.z;
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
@@ -632,7 +663,7 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     }
     l += __shfl_xor(l, 32);
     if (!have) return;
-    const row_out out = out_row(a, split, tok, head, m, l);
+    const row_out out = out_row(a, T, split, tok, head, m, l, h == 0);
 #pragma unroll
     for (int i = 0; i < NB; i++)
 #pragma unroll
@@ -640,61 +671,67 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
             const int d = i * 32 + 8 * (j >> 2) + 4 * h + (j & 3);
             if (d < hd) out.dst[d] = o[i][j] * out.f;
         }
-    if (a.splits > 1 && h == 0) {
-        out.dst[hd] = m;
-        out.dst[hd + 1] = l;
-    }
 }
 
-// The splits' parts of a row joined, in a fixed order: a wave takes every
-// fourth part.
+// The splits' parts of a row joined, in a fixed order, by one wave (four rows a
+// workgroup) or, many parts, by the workgroup's four: head_dim / 4 lanes read a
+// part, the others other parts beside it.
+template <int W>   // waves of a row
 __global__ __launch_bounds__(256) void k_attn_paged_join(attn_paged_args a) {
-    __shared__ float s_f[256], s_o[4][256], s_red[4];
-    const lnship_paged_kv &kv = a.kv;
-    const int tok = blockIdx.x, head = blockIdx.y, hd = (int)kv.head_dim, n_seq = (int)kv.n_seq, tid = threadIdx.x;
-    const int lane = tid & 63, wave = tid >> 6;
-    if (tok < kv.q_start[0] || tok >= kv.q_start[n_seq]) return;
-    const int sq = last_at_most(n_seq, tok, [&](int i) { return kv.q_start[i]; });
-    const int t0 = min(max(kv.q_start[sq], 0), (int)kv.ntok);
-    const uint32_t R = (uint32_t)a.tile_rows, rep = (uint32_t)a.rep;
-    const int tile = (int)((uint32_t)t0 * rep / R) + sq + (int)((uint32_t)((tok - t0) * a.rep + head % a.rep) / R);
-    // (an unsound q_start may give no such tile; faults are recorded by then)
-    const row_tile T = find_tile(a, tile, nullptr);
-    if (T.r0 < 0) return;
-    const int used = max((T.blocks + T.per - 1) / T.per, 1);
-    const int64_t step = kv.ntok * a.n_head * (hd + 2);
-    const float *w = a.work + ((int64_t)tok * a.n_head + head) * (hd + 2);
-    const float mi = tid < used ? w[tid * step + hd] : -INFINITY;
-    const float li = tid < used ? w[tid * step + hd + 1] : 0.0f;
+    constexpr int S = W == 4 ? 256 : 64;   // parts at most
+    __shared__ float s_f[4 / W][S], s_red[2][4];
+    __shared__ float4 s_o[4][64];
+    const int hd = (int)a.kv.head_dim, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t rows = a.kv.ntok * a.n_head;
+    const int64_t row = W == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int64_t tok = row / a.n_head;
+    const bool in = row < rows && tok >= a.kv.q_start[0] && tok < a.kv.q_start[a.kv.n_seq];
+    if (W == 4 && !in) return;
+    const int used = in ? max(1, min(a.used[row], a.splits)) : 0;   // (an unsound q_start may leave rows out)
+    const int at = W == 4 ? tid : lane;
+    const float2 st = at < used ? a.stats[at * rows + row] : make_float2(-INFINITY, 0.0f);
     auto reduce = [&](float v, bool sum) {
         for (int d = 32; d; d >>= 1) {
             const float y = __shfl_xor(v, d);
             v = sum ? v + y : fmaxf(v, y);
         }
+        if (W == 1) return v;
+        float *r = s_red[sum];
+        if (lane == 0) r[wave] = v;
         __syncthreads();
-        if (lane == 0) s_red[wave] = v;
-        __syncthreads();
-        return sum ? s_red[0] + s_red[1] + s_red[2] + s_red[3]
-                   : fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+        return sum ? r[0] + r[1] + r[2] + r[3] : fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
     };
-    const float M = reduce(mi, false);
-    const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - M);
-    s_f[tid] = f;
-    const float L = reduce(li * f, true);
-    float s[4] = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int i = wave; i < used; i += 4) {
-        const float fi = s_f[i];
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-            if (q * 64 + lane < hd) s[q] = fmaf(w[i * step + q * 64 + lane], fi, s[q]);
-    }
-#pragma unroll
-    for (int q = 0; q < 4; q++) s_o[wave][q * 64 + lane] = s[q];
+    const float M = reduce(st.x, false);
+    const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.x - M);
+    float *sf = s_f[W == 4 ? 0 : wave];
+    if (at < S) sf[at] = f;
+    const float L = reduce(st.y * f, true);
     __syncthreads();
-    if (tid < hd)
-        a.dst[tok * a.dst_ld + (int64_t)head * hd + tid] =
-            (s_o[0][tid] + s_o[1][tid] + s_o[2][tid] + s_o[3][tid]) * (M == -INFINITY ? 0.0f : 1.0f / L);
+    const int lanes = hd >> 2, par = 64 / lanes, sub = lane / lanes, d4 = lane - sub * lanes;
+    float4 s = make_float4(0, 0, 0, 0);
+    if (sub < par) {
+        const int64_t step = rows * hd;
+        const float4 *w = reinterpret_cast<const float4 *>(a.sums + row * hd) + d4;
+        const int inc = par * W;
+#pragma unroll 8
+        for (int i = (W == 4 ? wave * par : 0) + sub; i < used; i += inc) {
+            const float4 v = w[i * (step >> 2)];
+            const float fi = sf[i];
+            s.x = fmaf(v.x, fi, s.x), s.y = fmaf(v.y, fi, s.y), s.z = fmaf(v.z, fi, s.z), s.w = fmaf(v.w, fi, s.w);
+        }
+    }
+    s_o[wave][lane] = s;
+    __syncthreads();
+    if (!in || (W == 4 && wave > 0) || lane >= lanes) return;
+    const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
+    float4 t = make_float4(0, 0, 0, 0);
+    for (int w = W == 4 ? 0 : wave; w <= (W == 4 ? 3 : wave); w++)
+        for (int q = 0; q < par; q++) {
+            const float4 v = s_o[w][q * lanes + lane];
+            t.x += v.x, t.y += v.y, t.z += v.z, t.w += v.w;
+        }
+    float *dst = a.dst + tok * a.dst_ld + (row - tok * a.n_head) * hd + lane * 4;
+    dst[0] = t.x * inv, dst[1] = t.y * inv, dst[2] = t.z * inv, dst[3] = t.w * inv;
 }
 
 // ---- host -----------------------------------------------------------------------
@@ -729,15 +766,25 @@ static int log2_of(int64_t page) {
 // How a call runs: k_attn_chunk with `waves` waves, or (0) k_attn_paged; rows
 // of a tile, tiles, and the parts that a row's cells are split into.
 struct attn_plan {
-    int waves, tile_rows, splits;
+    int waves, tile_rows, splits, min_per;
     int64_t tiles;
 };
 #ifndef LNSHIP_TGT
-#define LNSHIP_TGT 16
-#define LNSHIP_TGT2 2
+#define LNSHIP_TGT 4
+#endif
+#ifndef LNSHIP_TGT2
+#define LNSHIP_TGT2 1
+#endif
+#ifndef LNSHIP_MINP
+#define LNSHIP_MINP 8
+#endif
+#ifndef LNSHIP_MINP2
+#define LNSHIP_MINP2 8
 #endif
 #ifndef LNSHIP_CHUNK_ROWS
 #define LNSHIP_CHUNK_ROWS 64
+#endif
+#ifndef LNSHIP_CHUNK_ROWS8
 #define LNSHIP_CHUNK_ROWS8 384
 #endif
 static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
@@ -747,13 +794,15 @@ static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
     p.tile_rows = p.waves ? p.waves * 32 : 16;
     p.tiles = rows / p.tile_rows + kv->n_seq;
     const int64_t wgs = std::max<int64_t>(1, p.tiles * kv->n_head_kv);
-    const int64_t most = (kv->table_ld * kv->page + 255) / 256, want = p.waves ? LNSHIP_TGT2 : LNSHIP_TGT;
+    p.min_per = p.waves ? LNSHIP_MINP2 : LNSHIP_MINP;
+    const int64_t most = (kv->table_ld * kv->page / 64 + p.min_per - 1) / p.min_per;
+    const int64_t want = p.waves ? LNSHIP_TGT2 : LNSHIP_TGT;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want * cus + wgs - 1) / wgs, most, 256}));
     return p;
 }
 
 static int64_t attn_work(const lnship_paged_kv *kv, int64_t n_head, int splits) {
-    return splits > 1 ? (int64_t)splits * kv->ntok * n_head * (kv->head_dim + 2) * 4 : 0;
+    return splits > 1 ? kv->ntok * n_head * (splits * (kv->head_dim + 2) + 1) * 4 : 0;
 }
 
 template <int NB, int NW>
@@ -832,11 +881,18 @@ int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args 
     const int64_t need = attn_work(kv, a->n_head, p.splits);
     if (need && (!a->work || a->work_bytes < (size_t)need || ((uintptr_t)a->work & 15)))
         return fail(LNSHIP_EINVAL, "attn_paged: work smaller than lnship16_attn_paged_work or not aligned%s");
-    if (kv->ntok * rep > 0xfffffff || p.tiles * kv->n_head_kv > 0x7fffff)
+    // (a grid's threads along x are counted in 32 bits)
+    if (kv->ntok * rep > 0xfffffff || p.tiles * kv->n_head_kv > 0x7fffff || kv->ntok * a->n_head > 0xffffff)
         return fail(LNSHIP_ERANGE, "attn_paged: grid too large%s");
     attn_paged_args m{*kv, a->q, a->dst, q_ld, dst_ld, a->scale * 1.44269504088896341f,
                       a->window > 0x3fffffff ? 0 : (int)a->window, (int)a->n_head, (int)rep, log2_of(kv->page), p.splits,
-                      p.tile_rows, (float *)a->work};
+                      p.tile_rows, p.min_per, q_ld % 4 == 0 && ((uintptr_t)a->q & 15) == 0, nullptr, nullptr, nullptr};
+    const int64_t all = kv->ntok * a->n_head;
+    if (need) {
+        m.sums = (float *)a->work;
+        m.stats = (float2 *)(m.sums + p.splits * all * kv->head_dim);
+        m.used = (int *)(m.stats + p.splits * all);
+    }
     if (kv->n_pages == 0) m.kv.table_ld = 0;   // no page to read: no cells
     hipStream_t s = (hipStream_t)stream;
     int rc;
@@ -851,7 +907,8 @@ int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args 
         default: rc = launch_attn<8>(m, p, s, st->index_err);
     }
     if (rc || p.splits == 1) return rc;
-    hipLaunchKernelGGL(k_attn_paged_join, dim3((unsigned)kv->ntok, (unsigned)a->n_head), dim3(256), 0, s, m);
+    if (p.splits > 8) hipLaunchKernelGGL(k_attn_paged_join<4>, dim3((unsigned)all), dim3(256), 0, s, m);
+    else hipLaunchKernelGGL(k_attn_paged_join<1>, dim3((unsigned)((all + 3) / 4)), dim3(256), 0, s, m);
     LNSHIP_HIP(hipGetLastError());
     return 0;
 }
