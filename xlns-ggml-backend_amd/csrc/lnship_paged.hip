@@ -270,14 +270,15 @@ __device__ __forceinline__ void load_q(const float *q, int d, int hd, bool vec, 
 // this one's weights are formed, its values once this one's are decoded.
 template <int NB, bool FULL>   // 32-wide groups of head_dim; whether it fills them
 #ifndef LNSHIP_W
-#define LNSHIP_W 2
+#define LNSHIP_W 3
 #endif
 __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_attn_paged(attn_paged_args a, unsigned long long *err) {
     const lnship_paged_kv &kv = a.kv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int rep = a.rep, kvh = blockIdx.y, split = blockIdx.z, hd = (int)kv.head_dim, page = (int)kv.page;
-    __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ float s_m[4][16], s_l[4][16], s_qs[16];
     __shared__ float s_o[16][NB * 32 + 1];
+    __shared__ uint4 s_q[2][NB][64];   // the queries' split halves, as the products' operands
 
     const row_tile T = find_tile(a, blockIdx.x, err);
     if (T.r0 < 0 || (split > 0 && split * T.per >= T.blocks)) return;
@@ -289,29 +290,6 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
     const int head = kvh * rep + (int)((uint32_t)row % (uint32_t)rep);
     const int pos = min(T.pos0 + tok - T.t0, T.c1 - 1);
     const int lo_cell = a.window > 0 ? T.pos0 + tok - T.t0 - a.window : -1;   // cells at and below are hidden
-
-    // the queries as halves, scaled by the row's largest to at most 2
-    frag qh[NB], ql[NB];
-    float qs;
-    {
-        float x[NB][8], mx = 0.0f;
-        const float *q = a.q + tok * a.q_ld + (int64_t)head * hd;
-#pragma unroll
-        for (int b = 0; b < NB; b++) load_q(q, b * 32 + g * 8, FULL ? NB * 32 : hd, a.vec, x[b]);
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[b][j]));
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const int e = (int)(f32_bits(mx) >> 23) - 127;   // -127 for zeros
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int j = 0; j < 8; j += 2)
-                split2(ldexpf(x[b][j], -e), ldexpf(x[b][j + 1], -e), qh[b].u[j / 2], ql[b].u[j / 2]);
-        qs = ldexpf(a.scale, e);
-    }
 
     const int32_t *table = kv.table + (int64_t)T.sq * kv.table_ld;
     const int64_t head_codes = (int64_t)page * hd, page_codes = kv.n_head_kv * head_codes;
@@ -356,21 +334,50 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
         load_k(cb, kid);
         load_v(cb, vid);
     }
+    // the queries as halves, scaled by the row's largest to at most 2: by the
+    // first wave, for all
+    if (wave == 0) {
+        float x[NB][8], mx = 0.0f;
+        const float *q = a.q + tok * a.q_ld + (int64_t)head * hd;
+#pragma unroll
+        for (int b = 0; b < NB; b++) load_q(q, b * 32 + g * 8, FULL ? NB * 32 : hd, a.vec, x[b]);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[b][j]));
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const int e = (int)(f32_bits(mx) >> 23) - 127;   // -127 for zeros
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            frag hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) split2(ldexpf(x[b][j], -e), ldexpf(x[b][j + 1], -e), hi.u[j / 2], lo.u[j / 2]);
+            s_q[0][b][lane] = hi.w;
+            s_q[1][b][lane] = lo.w;
+        }
+        if (g == 0) s_qs[n] = ldexpf(a.scale, e);
+    }
+    __syncthreads();
+    const float qs = s_qs[n];
     for (; cb < cend; cb += 128) {
         const int vid1 = page_of(cb + 128 + vcell), kid1 = page_of(cb + 128 + kcell);
         const bool vok = cb + vcell < cend && sound(vid);
         if (cb + vcell < cend && !vok) index_fault(err, vid);
         float4v sh[2], sx[2];
+        sh[0] = sh[1] = sx[0] = sx[1] = float4v{0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            sh[t] = sx[t] = float4v{0, 0, 0, 0};
+        for (int i = 0; i < NB; i++) {
+            frag qh, ql;
+            qh.w = s_q[0][i][lane];
+            ql.w = s_q[1][i][lane];
 #pragma unroll
-            for (int i = 0; i < NB; i++) {
+            for (int t = 0; t < 2; t++) {
                 frag kh, kl;
                 decode8(kc[t][i], kh, kl);
-                sh[t] = mma(kh, qh[i], sh[t]);
-                sx[t] = mma(kl, qh[i], sx[t]);
-                sx[t] = mma(kh, ql[i], sx[t]);
+                sh[t] = mma(kh, qh, sh[t]);
+                sx[t] = mma(kl, qh, sx[t]);
+                sx[t] = mma(kh, ql, sx[t]);
             }
         }
         load_k(min(cb + 128, cend - 1), kid1);
@@ -770,7 +777,7 @@ struct attn_plan {
     int64_t tiles;
 };
 #ifndef LNSHIP_TGT
-#define LNSHIP_TGT 4
+#define LNSHIP_TGT 8
 #endif
 #ifndef LNSHIP_TGT2
 #define LNSHIP_TGT2 1
