@@ -468,7 +468,7 @@ int64_t lnship16_attn_paged_work(const lnship_paged_kv *kv, int64_t n_head);
  * drawn; with an infinite largest logit only its equals weigh anything; a row
  * without any logit above -inf gets token -1 and probability 0.  Weights are
  * summed as integers (units of 2^-40), so the draw does not depend on an order
- * of additions.  n_vocab up to 2^22.  No LNS arithmetic, and no counterpart in
+ * of additions.  n_vocab up to 2^19.  No LNS arithmetic, and no counterpart in
  * the reference, which samples on the host.
  * work: lnship_sample_work bytes, as in lnship_paged_attn_args. */
 typedef struct lnship_sample_args {
