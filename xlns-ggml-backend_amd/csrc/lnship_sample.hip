@@ -10,6 +10,9 @@
 
 namespace lnship {
 
+#ifndef LNSHIP_RES
+#define LNSHIP_RES 3
+#endif
 constexpr int k_draw_block = 1024;
 constexpr int k_draw_waves = k_draw_block / 64;
 constexpr int k_w_sh = 40;              // weights are integers in units of 2^-40
@@ -31,20 +34,22 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 constexpr uint32_t k_key_ninf = 0x007fffffu;   // order_key(-inf)
 
-// The weight e^((x - x_max) / T) in units of 2^-40.  The exponent is formed in
-// 64 bits (32 would lose what tells two sums apart), its fraction's power in
-// 32: 24 bits of every weight.
+// The weight e^((x - x_max) / T) in units of 2^-40, rounded.  The exponent is
+// formed in 64 bits (32 would lose what tells two sums apart), its fraction's
+// power in 32: 24 bits of every weight.  Integers come out of the low bits of
+// a sum with a power of two, which costs less than a conversion: 17 issue slots
+// a weight, four of them the power.
 struct weigher {
     double xmax, f;   // f = log2 e / T
     __device__ __forceinline__ uint64_t operator()(float x) const {
-        const double d = (double)x - xmax;
-        const double y = x == (float)xmax ? 0.0 : d * f;
-        if (!(y > -64.0)) return 0;
-        const double n = rint(y);
-        // 2^r in [2^-1/2, 2^1/2]: an integer in units of 2^-24
-        const uint64_t q = (uint64_t)(uint32_t)(__builtin_amdgcn_exp2f((float)(y - n)) * 16777216.0f);
-        const int sh = k_w_sh - 24 + (int)n;
-        return sh >= 0 ? q << sh : q >> -sh;
+        constexpr double whole = 6755399441055744.0;   // 1.5 2^52: a sum's low word is the integer
+        constexpr double unit = 4096.0;                // a sum's last place is 2^-40
+        const double y = fmax(((double)x - xmax) * f, -63.0);   // (-inf times an f of 0: -63)
+        const double t = y + whole;
+        // 2^r in [2^-1/2, 2^1/2]
+        const float p = __builtin_amdgcn_exp2f((float)(y - (t - whole)));
+        const double w = ldexp((double)p, (int)(uint32_t)__double_as_longlong(t));
+        return (uint64_t)__double_as_longlong(w + unit) - (uint64_t)__double_as_longlong(unit);
     }
 };
 
@@ -132,7 +137,9 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
     __shared__ uint64_t s_above_w;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n;
     const float *x = a.logits + r * a.ld;
-    const weigher W = d0.W;
+    // (an infinite largest logit, or 1 / T: only its equals weigh anything)
+    const bool sharp = !(fabsf(d0.xmax) < INFINITY) || !(d0.W.f < 1e300);
+    auto W = [&](float v) { return sharp ? (uint64_t)(v == d0.xmax) << k_w_sh : d0.W(v); };
     const int top_k = d0.top_k;
     const float top_p = d0.top_p;
     const double wmin = d0.wmin;
@@ -284,8 +291,9 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
     pass(draw_target(a.u[r], total), true, total);
 }
 
-// One workgroup a row; a wave goes through segments of 1024 logits.  The row is
-// held in registers (R segments a wave), or (R 0) read again for every pass.
+// One workgroup a row; a wave goes through segments of 1024 logits.  R segments
+// a wave are held in registers; the rest of a longer row (MORE) is read again
+// for every pass.
 // After its largest logit is known:
 // - without top_k and top_p the weights are summed by segment, the segment that
 //   holds u's share found, and that segment gone through again;
@@ -293,9 +301,9 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
 //   for top_k, of weights for top_p) names the bin of the border; with a top_k
 //   the tokens down to that bin, with top_p alone those of that bin, are
 //   put in order, and the border is exact.
-template <int R>
+template <int R, bool MORE>
 __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
-    typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+    typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));   // rows need no alignment
     __shared__ uint64_t s_hist[k_bins];   // later the lists
     __shared__ uint64_t s_seg[k_list / 2];   // segments' sums; before, the places of order_items
     static_assert(k_seg_max <= k_list / 2, "");
@@ -308,43 +316,50 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
     const float *x = a.logits + r * a.ld;
     static_assert(2 * k_list <= k_bins, "both lists lie in the histogram's place");
 
-    // a segment's sixteen logits of a lane: 256 q + 4 lane + j; NaN as -inf
-    auto load = [&](int seg, float4u *v) {
+    // a segment's sixteen logits of a lane, v[4 q + j] number 256 q + 4 lane + j;
+    // NaN, and what lies past the row, as -inf
+    auto load = [&](int seg, float (&v)[16]) {
         const int i0 = seg * k_seg + lane * 4;
         if ((seg + 1) * k_seg <= n) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) v[q] = *reinterpret_cast<const float4u *>(x + i0 + 256 * q);
+            for (int q = 0; q < 4; q++) {
+                const float4u t = *reinterpret_cast<const float4u *>(x + i0 + 256 * q);
+                v[4 * q] = t[0], v[4 * q + 1] = t[1], v[4 * q + 2] = t[2], v[4 * q + 3] = t[3];
+            }
         } else {
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) v[q][j] = i0 + 256 * q + j < n ? x[i0 + 256 * q + j] : -INFINITY;
-        }
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[q][j] = fmaxf(v[q][j], -INFINITY);
-    };
-    float4u keep[R > 0 ? R : 1][4];
-    // f(segment, its logits) for every segment of the wave
-    auto each = [&](auto f) {
-        if constexpr (R > 0) {
-#pragma unroll
-            for (int i = 0; i < R; i++)
-                if (i * k_draw_waves + wave < segs) f(i * k_draw_waves + wave, keep[i]);
-        } else {
-            for (int seg = wave; seg < segs; seg += k_draw_waves) {
-                float4u v[4];
-                load(seg, v);
-                f(seg, v);
+            for (int e = 0; e < 16; e++) {
+                const int i = i0 + (e >> 2) * 256 + (e & 3);
+                const float t = x[min(i, n - 1)];
+                v[e] = i < n ? t : -INFINITY;
             }
         }
+#pragma unroll
+        for (int e = 0; e < 16; e++) v[e] = fmaxf(v[e], -INFINITY);
     };
-    if constexpr (R > 0) {
+    auto index = [&](int seg, int e) { return seg * k_seg + (e >> 2) * 256 + lane * 4 + (e & 3); };
+    // f(segment, its logits) for every segment of the wave: the first R are kept
+    // in registers, the others loaded for every pass, one ahead
+    float keep[R][16];
+#pragma unroll
+    for (int i = 0; i < R; i++)
+        if (i * k_draw_waves + wave < segs) load(i * k_draw_waves + wave, keep[i]);
+    auto each = [&](auto f) {
+        float next[16];
+        int seg = R * k_draw_waves + wave;
+        if (MORE && seg < segs) load(seg, next);
 #pragma unroll
         for (int i = 0; i < R; i++)
-            if (i * k_draw_waves + wave < segs) load(i * k_draw_waves + wave, keep[i]);
-    }
+            if (i * k_draw_waves + wave < segs) f(i * k_draw_waves + wave, keep[i]);
+        if constexpr (MORE)
+            for (; seg < segs; seg += k_draw_waves) {
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) v[e] = next[e];
+                if (seg + k_draw_waves < segs) load(seg + k_draw_waves, next);
+                f(seg, v);
+            }
+    };
 
     draw_row D;
     auto easy = [&]() -> bool {
@@ -354,19 +369,17 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
         float mx = -INFINITY;
         int at = 0x7fffffff;
         if (!greedy) {
-            each([&](int, const float4u *v) {
-    #pragma unroll
-                for (int q = 0; q < 4; q++) mx = fmaxf(fmaxf(mx, fmaxf(v[q][0], v[q][1])), fmaxf(v[q][2], v[q][3]));
+            each([&](int, const float *v) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) mx = fmaxf(mx, v[e]);
             });
         } else {
-            each([&](int seg, const float4u *v) {
-    #pragma unroll
-                for (int q = 0; q < 4; q++)
-    #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (v[q][j] > mx) {
-                            mx = v[q][j];
-                            at = seg * k_seg + 256 * q + lane * 4 + j;
+            each([&](int seg, const float *v) {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                        if (v[e] > mx) {
+                            mx = v[e];
+                            at = index(seg, e);
                         }
             });
         }
@@ -411,30 +424,26 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
             if (tid == 0) s_n = 0;
             __syncthreads();
             if (by_count) {
-                each([&](int, const float4u *v) {
-    #pragma unroll
-                    for (int q = 0; q < 4; q++)
-    #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int b = bin_of(v[q][j]);
+                each([&](int, const float *v) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                            const int b = bin_of(v[e]);
                             if (b < k_bins - 1) atomicAdd((unsigned int *)&s_hist[b], 1u);
                         }
                 });
             } else {
-                each([&](int, const float4u *v) {
-    #pragma unroll
-                    for (int q = 0; q < 4; q++)
-    #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int b = bin_of(v[q][j]);
-                            if (b < k_bins - 1) atomicAdd((unsigned long long *)&s_hist[b], (unsigned long long)W(v[q][j]));
+                each([&](int, const float *v) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                            const int b = bin_of(v[e]);
+                            if (b < k_bins - 1) atomicAdd((unsigned long long *)&s_hist[b], (unsigned long long)W(v[e]));
                         }
                 });
             }
             __syncthreads();
             // the first bin up to which the counts (the weights) reach what is kept
             uint64_t h[4], sum = 0, all;
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; i++) sum += h[i] = s_hist[tid * 4 + i];
             uint64_t run = block_scan(sum, s_scan[1], all) - sum;
             uint64_t want = (uint64_t)D.top_k;
@@ -446,7 +455,7 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
             __syncthreads();
             if (run < want && run + sum >= want) {
                 int b = tid * 4;
-    #pragma unroll
+#pragma unroll
                 for (int i = 0; i < 3; i++)
                     if (run + h[i] < want) run += h[i], b++;
                     else break;
@@ -458,17 +467,15 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
             if (border < k_bins - 1) {
                 const uint64_t above = s_x[1];
                 const int from = by_count ? 0 : border;   // the bins of the list
-                each([&](int seg, const float4u *v) {
-    #pragma unroll
-                    for (int q = 0; q < 4; q++)
-    #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int b = bin_of(v[q][j]);
+                each([&](int seg, const float *v) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                            const int b = bin_of(v[e]);
                             if (b <= border && b >= from) {
                                 const int i = atomicAdd(&s_n, 1);
                                 if (i < k_list)
-                                    s_list[i] = (uint64_t)order_key(v[q][j]) << 32 |
-                                                (uint32_t)(0x7fffffff - (seg * k_seg + 256 * q + lane * 4 + j));
+                                    s_list[i] = (uint64_t)order_key(v[e]) << 32 |
+                                                (uint32_t)(0x7fffffff - index(seg, e));
                             }
                         }
                 });
@@ -541,12 +548,10 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
             }
             return w;
         };
-        each([&](int seg, const float4u *v) {
+        each([&](int seg, const float *v) {
             uint64_t w = 0;
-    #pragma unroll
-            for (int q = 0; q < 4; q++)
-    #pragma unroll
-                for (int j = 0; j < 4; j++) w += weigh(v[q][j], seg * k_seg + 256 * q + lane * 4 + j);
+#pragma unroll
+            for (int e = 0; e < 16; e++) w += weigh(v[e], index(seg, e));
             w = wave_sum(w);
             if (lane == 0) s_seg[seg] = w;
         });
@@ -603,10 +608,10 @@ int lnship_sample(const lnship_sample_args *a, void *stream) {
     const dim3 grid((unsigned)a->n_rows), block(k_draw_block);
     hipStream_t st = (hipStream_t)stream;
     const int rounds = (int)((a->n_vocab + k_seg * k_draw_waves - 1) / (k_seg * k_draw_waves));
-    if (rounds == 1) hipLaunchKernelGGL(k_draw<1>, grid, block, 0, st, d);
-    else if (rounds == 2) hipLaunchKernelGGL(k_draw<2>, grid, block, 0, st, d);
-    else if (rounds == 3) hipLaunchKernelGGL(k_draw<3>, grid, block, 0, st, d);
-    else hipLaunchKernelGGL(k_draw<0>, grid, block, 0, st, d);
+    if (rounds == 1) hipLaunchKernelGGL((k_draw<1, false>), grid, block, 0, st, d);
+    else if (rounds == 2) hipLaunchKernelGGL((k_draw<2, false>), grid, block, 0, st, d);
+    else if (rounds == 3) hipLaunchKernelGGL((k_draw<3, false>), grid, block, 0, st, d);
+    else hipLaunchKernelGGL((k_draw<LNSHIP_RES, true>), grid, block, 0, st, d);
     LNSHIP_HIP(hipGetLastError());
     return 0;
 }
