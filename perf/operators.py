@@ -21,6 +21,7 @@ own = False
 
 DEV = "cuda"
 THETA = 10000.0
+PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xlns-ggml-backend_amd")
 
 
 def listed():
@@ -172,9 +173,8 @@ def prepare(case, seed):
 # ---- the framework's calls -----------------------------------------------------------------------
 
 def _package():
-    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xlns-ggml-backend_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
+    if PACKAGE not in sys.path:
+        sys.path.insert(0, PACKAGE)
     import lnship
     import lnship.paged
     return lnship
