@@ -233,6 +233,21 @@ struct cvt16_lds {
         return c;
     }
 };
+// a batch of values: one branch for the batch's special values
+template <int B>
+__device__ __forceinline__ void cvt16_batch(const cvt16_lds &C, const float (&f)[B], uint32_t (&c)[B]) {
+    bool special = false;
+#pragma unroll
+    for (int q = 0; q < B; q++) {
+        const uint32_t b = f32_bits(f[q]), ex = __builtin_amdgcn_ubfe(b, 23, 8), m = __builtin_amdgcn_ubfe(b, 15, 8);
+        c[q] = (((uint32_t)C.t[m + (ex < 127u ? 0u : 256u)] + (ex << 7)) & k16_logmask) | ((b >> 16) & k16_sign);
+        special |= ex - 1u >= 254u;
+    }
+    if (__any(special)) {
+#pragma unroll
+        for (int q = 0; q < B; q++) c[q] = x16_from_f32(C.cvt, f[q]);
+    }
+}
 constexpr int k_cvt_lds = 512;
 __device__ __forceinline__ cvt16_lds stage_cvt16(const uint16_t *cvt, uint16_t *t) {
     for (int i = threadIdx.x; i < k_cvt_lds; i += blockDim.x)

@@ -192,21 +192,6 @@ __global__ void k_to_f32_32(const uint32_t *__restrict__ src, float *__restrict_
         dst[i] = x32_to_f32(src[i]);
 }
 
-// a batch of values: one branch for the batch's special values
-template <int B>
-__device__ __forceinline__ void cvt16_batch(const cvt16_lds &C, const float (&f)[B], uint32_t (&c)[B]) {
-    bool special = false;
-#pragma unroll
-    for (int q = 0; q < B; q++) {
-        const uint32_t b = f32_bits(f[q]), ex = __builtin_amdgcn_ubfe(b, 23, 8), m = __builtin_amdgcn_ubfe(b, 15, 8);
-        c[q] = (((uint32_t)C.t[m + (ex < 127u ? 0u : 256u)] + (ex << 7)) & k16_logmask) | ((b >> 16) & k16_sign);
-        special |= ex - 1u >= 254u;
-    }
-    if (__any(special)) {
-#pragma unroll
-        for (int q = 0; q < B; q++) c[q] = x16_from_f32(C.cvt, f[q]);
-    }
-}
 // rows x cols row-major -> k8-interleaved (k = col, m = row), one slice per
 // blockIdx.y; padding columns (cols..Kp) get code 0.  TY: 0 F32, 1 IEEE half,
 // 2 xlns16 codes.  Bound by HBM (xlns32: by its FP64 logarithms): a thread

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "lnship.h"
 #include "lnship_device.h"
@@ -26,8 +27,30 @@ __device__ __forceinline__ int last_at_most(int n, int64_t x, F key) {
     return lo;
 }
 
+// The same by a whole wave, 64 keys a round: a round takes as long as a step
+// above, and up to 64 sequences take one.
+template <class F>
+__device__ __forceinline__ int wave_last_at_most(int n, int x, F key) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, len = n;
+    while (len > 1) {
+        const int step = (len + 63) >> 6, i = lane * step;
+        const uint64_t in = __ballot(i < len && key(lo + min(i, len - 1)) <= x);
+        const int last = max(__popcll(in) - 1, 0) * step;   // (keys rise: the lanes in are the first ones)
+        lo += last;
+        len = min(step, len - last);
+    }
+    return lo;
+}
+
 // ---- rope and stores ------------------------------------------------------------
 
+#ifndef LNSHIP_SROWS
+#define LNSHIP_SROWS 32
+#endif
+#ifndef LNSHIP_SWG
+#define LNSHIP_SWG 16
+#endif
 struct store_args {
     lnship_paged_kv kv;
     lnship_paged_store_args a;
@@ -44,7 +67,7 @@ __global__ __launch_bounds__(k_block) void k_store_paged(store_args s, dev_table
     const int64_t t = blockIdx.x, hd = kv.head_dim;
     const int n_seq = (int)kv.n_seq;
     if (t < kv.q_start[0] || t >= kv.q_start[n_seq]) return;
-    const int sq = last_at_most(n_seq, t, [&](int i) { return kv.q_start[i]; });
+    const int sq = wave_last_at_most(n_seq, (int)t, [&](int i) { return kv.q_start[i]; });
     const int64_t p = (int64_t)kv.kv_len[sq] - kv.q_start[sq + 1] + t;
     const int nd = a.rope_n_dims;
     if (p < 0 || p >> s.page_sh >= kv.table_ld || (nd > 0 && p >= a.n_pos)) {
@@ -82,6 +105,156 @@ __global__ __launch_bounds__(k_block) void k_store_paged(store_args s, dev_table
                                     : kv.v_pages + base + ((c >> 3) * hd + d) * 8 + (c & 7);
             *o = (uint16_t)F.from(__half2float(__float2half_rn(v)));
         }
+    }
+}
+
+// The codes of a rotated key through F32 and half and back, for a code whose
+// value is a normal half: its exponent, and of its fraction one of two tables
+// of 128 (below 1 the conversion's truncation is upward).  Any other code takes
+// the way through the tables in memory.
+struct half_codes {
+    const int16_t *t;   // LDS: [0, 128) below 1, [128, 256) from 1 on; the new fraction (up to 128)
+    const dev_tables &T;
+    __device__ __forceinline__ uint32_t slow(uint32_t c) const {
+        return x16_from_f32(T.cvt16, __half2float(__float2half_rn(T.rev16[c])));
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t c) const {
+        const uint32_t l = c & k16_logmask, e = l >> 7;
+        uint32_t r = (c & (k16_sign | 0x7f80u)) + (uint32_t)(int32_t)t[(l & 127u) + (e < 128u ? 0u : 128u)];
+        if (__builtin_expect(e - 114u >= 29u, 0)) r = slow(c);   // below 2^-14, or 2^15 and more
+        return r;
+    }
+};
+
+// The F32 value of a code: those of 2^-8 to 2^8 from LDS.
+constexpr int k_rev_binades = 16, k_rev_lds = k_rev_binades * 128;
+struct rev16_lds {
+    const float *t;
+    const float *rev;
+    __device__ __forceinline__ float operator()(uint32_t c) const {
+        const uint32_t i = (c & k16_logmask) - (k16_one - k_rev_lds / 2);
+        float v = t[min(i, (uint32_t)k_rev_lds - 1u)];
+        v = __uint_as_float(f32_bits(v) | (c & k16_sign) << 16);
+        if (__builtin_expect(i >= (uint32_t)k_rev_lds, 0)) v = rev[c];
+        return v;
+    }
+};
+
+constexpr int k_store_rows = 64;   // rows of a workgroup at most
+
+// Many rows, in 16-byte loads: a thread rotates four pairs (or converts eight
+// dims behind the rotated ones) of a head, or stores one dim of a value; a
+// workgroup has consecutive rows.  The conversions, the Gaussian logs and the
+// decoded values come from tables in LDS: from memory each is a gather that
+// costs a cache line a lane.  Bound by HBM and the LDS lookups (8 a pair).
+template <bool NEOX>
+__global__ __launch_bounds__(k_block) void k_store_paged_rows(store_args s, int rows_wg, dev_tables T,
+                                                              unsigned long long *err) {
+    __shared__ uint16_t s_cvt[k_cvt_lds];
+    __shared__ alignas(16) int16_t s_g[2 * k16_gauss_n];
+    __shared__ int16_t s_half[256];
+    __shared__ float s_rev[k_rev_lds];
+    __shared__ int s_pos[k_store_rows], s_page[k_store_rows];
+    const lnship_paged_kv &kv = s.kv;
+    const lnship_paged_store_args &a = s.a;
+    const int tid = threadIdx.x, hd = (int)kv.head_dim, nd = a.rope_n_dims, page = (int)kv.page;
+    const int n_head = (int)a.n_head, n_head_kv = (int)kv.n_head_kv, n_seq = (int)kv.n_seq;
+    const int64_t t0 = (int64_t)blockIdx.x * rows_wg;
+    const int rows = (int)min((int64_t)rows_wg, kv.ntok - t0);
+    if (tid < rows) {
+        const int64_t t = t0 + tid;
+        int pos = -1, id = -1;
+        if (t >= kv.q_start[0] && t < kv.q_start[n_seq]) {
+            // single tokens: row t is sequence t's
+            int sq = (int)min(t, (int64_t)n_seq - 1);
+            if (kv.q_start[sq] > t || kv.q_start[sq + 1] <= t)
+                sq = last_at_most(n_seq, t, [&](int i) { return kv.q_start[i]; });
+            const int64_t p = (int64_t)kv.kv_len[sq] - kv.q_start[sq + 1] + t;
+            if (p < 0 || p >> s.page_sh >= kv.table_ld || p >= a.n_pos) {
+                index_fault(err, p);
+            } else {
+                pos = (int)p;
+                id = kv.table[sq * kv.table_ld + (p >> s.page_sh)];
+                if (id < 0 || id >= kv.n_pages) {
+                    index_fault(err, id);
+                    id = -1;
+                }
+            }
+        }
+        s_pos[tid] = pos;
+        s_page[tid] = id;
+    }
+    const cvt16_lds C = stage_cvt16(T.cvt16, s_cvt);
+    for (int i = tid; i < k16_gauss_n; i += k_block)
+        reinterpret_cast<uint32_t *>(s_g)[i] = reinterpret_cast<const uint32_t *>(T.gauss16)[i];
+    for (int i = tid; i < k_rev_lds; i += k_block) s_rev[i] = T.rev16[k16_one - k_rev_lds / 2 + i];
+    const half_codes H{s_half, T};
+    for (int i = tid; i < 256; i += k_block) s_half[i] = (int16_t)(H.slow(k16_one - 128 + i) - (k16_one + (i & 128) - 128));
+    const rev16_lds V{s_rev, T.rev16};
+    __syncthreads();
+
+    const int eighths = hd >> 3, rot_q = n_head * eighths, rot = rot_q + n_head_kv * eighths, per = rot + n_head_kv * hd;
+    const int64_t head_codes = (int64_t)page * hd;
+    int r = 0, e = tid;
+    while (e >= per) e -= per, r++;
+    for (; r < rows;) {
+        const int pos = s_pos[r], id = s_page[r];
+        const int64_t t = t0 + r;
+        if (pos >= 0) {
+            const int c = pos & (page - 1);
+            if (e < rot) {
+                const bool key = e >= rot_q;
+                const int f = key ? e - rot_q : e, h = (int)((uint32_t)f / (uint32_t)eighths), o = f - h * eighths;
+                const float *x = (key ? a.k + t * a.k_ld : a.q + t * a.q_ld) + h * hd;
+                const bool rotate = o * 8 < nd;
+                // the item's dims: d0.. and d1.. (four each)
+                const int d0 = NEOX && rotate ? o * 4 : o * 8, d1 = NEOX && rotate ? nd / 2 + o * 4 : o * 8 + 4;
+                uint32_t y[8];
+                {
+                    const float4 u = *reinterpret_cast<const float4 *>(x + d0), v = *reinterpret_cast<const float4 *>(x + d1);
+                    const float w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+                    cvt16_batch(C, w, y);
+                }
+                if (rotate) {
+                    const float4 *cs = reinterpret_cast<const float4 *>(a.cos_sin + (int64_t)pos * nd) + o * 2;
+                    const float4 u = cs[0], v = cs[1];
+                    const float w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+                    uint32_t z[8];   // cos, sin of four pairs
+                    cvt16_batch(C, w, z);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int i0 = NEOX ? j : 2 * j, i1 = NEOX ? j + 4 : 2 * j + 1;
+                        const uint32_t x0 = y[i0], x1 = y[i1], co = z[2 * j], si = z[2 * j + 1];
+                        y[i0] = x16_add_g(s_g, x16_mul(x0, co), x16_mul(x1, si) ^ k16_sign);
+                        y[i1] = x16_add_g(s_g, x16_mul(x0, si), x16_mul(x1, co));
+                    }
+                }
+                if (!key) {
+                    float *q = a.q_dst + t * a.q_dst_ld + h * hd;
+                    *reinterpret_cast<float4 *>(q + d0) = make_float4(V(y[0]), V(y[1]), V(y[2]), V(y[3]));
+                    *reinterpret_cast<float4 *>(q + d1) = make_float4(V(y[4]), V(y[5]), V(y[6]), V(y[7]));
+                } else if (id >= 0) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) y[j] = H(y[j]);
+                    uint16_t *k = kv.k_pages + ((int64_t)id * n_head_kv + h) * head_codes + c * 8;
+                    const uint2 lo = make_uint2(y[0] | y[1] << 16, y[2] | y[3] << 16);
+                    const uint2 hi = make_uint2(y[4] | y[5] << 16, y[6] | y[7] << 16);
+                    if (!NEOX) {
+                        *reinterpret_cast<uint4 *>(k + (d0 >> 3) * page * 8) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    } else {
+                        *reinterpret_cast<uint2 *>(k + (d0 >> 3) * page * 8 + (d0 & 7)) = lo;
+                        *reinterpret_cast<uint2 *>(k + (d1 >> 3) * page * 8 + (d1 & 7)) = hi;
+                    }
+                }
+            } else if (id >= 0) {
+                const int f = e - rot, h = (int)((uint32_t)f / (uint32_t)hd), d = f - h * hd;
+                const float v = a.v[t * a.v_ld + f];
+                kv.v_pages[((int64_t)id * n_head_kv + h) * head_codes + ((c >> 3) * hd + d) * 8 + (c & 7)] =
+                    (uint16_t)C(__half2float(__float2half_rn(v)));
+            }
+        }
+        e += k_block;
+        while (e >= per) e -= per, r++;
     }
 }
 
@@ -208,7 +381,7 @@ __device__ __forceinline__ row_tile find_tile(const attn_paged_args &a, int tile
     const uint32_t R = (uint32_t)a.tile_rows, rep = (uint32_t)a.rep;
     auto first_tile = [&](int i) { return (int)((uint32_t)min(max(kv.q_start[i], 0), (int)kv.ntok) * rep / R) + i; };
     row_tile t;
-    t.sq = last_at_most((int)kv.n_seq, tile, first_tile);
+    t.sq = wave_last_at_most((int)kv.n_seq, tile, first_tile);
     t.t0 = min(max(kv.q_start[t.sq], 0), (int)kv.ntok);
     const int64_t end = kv.q_start[t.sq + 1];
     t.rows = (int)max(min(end, kv.ntok) - t.t0, (int64_t)0) * a.rep;
@@ -815,8 +988,14 @@ static int64_t attn_work(const lnship_paged_kv *kv, int64_t n_head, int splits) 
 template <int NB, int NW>
 static int launch_chunk(const attn_paged_args &m, const attn_plan &p, hipStream_t s, unsigned long long *err) {
     const int lds = 2 * 4 * 64 * NB * 32 * 2;
-    LNSHIP_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_chunk<NB, NW>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    static std::atomic<uint64_t> done{0};   // devices that know the kernel's LDS
+    int dev = 0;
+    if (int rc = current_device(&dev)) return rc;
+    if (!(done.load() >> dev & 1)) {
+        LNSHIP_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_chunk<NB, NW>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        done.fetch_or((uint64_t)1 << dev);
+    }
     hipLaunchKernelGGL((k_attn_chunk<NB, NW>), dim3((unsigned)(p.tiles * m.kv.n_head_kv), (unsigned)p.splits),
                        dim3(NW * 64), lds, s, m, err);
     LNSHIP_HIP(hipGetLastError());
@@ -856,6 +1035,18 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
         return fail(LNSHIP_EINVAL, "rope_store_kv_paged: null pointer%s");
     device_state *st = state();
     if (!st) return LNSHIP_ENOINIT;
+    // 16-byte loads and stores, and eight dims a thread
+    const bool vec = a->rope_n_dims > 0 && a->rope_n_dims % 8 == 0 &&
+                     (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->cos_sin | (uintptr_t)a->q_dst) & 15) == 0 &&
+                     ((a->q_ld | a->k_ld | s.a.q_dst_ld) & 3) == 0;
+    if (vec && kv->ntok >= LNSHIP_SROWS) {
+        const int rows = (int)std::min<int64_t>(k_store_rows, std::max<int64_t>(1, kv->ntok / (LNSHIP_SWG * st->cus)));
+        const dim3 grid((unsigned)((kv->ntok + rows - 1) / rows));
+        if (a->neox) hipLaunchKernelGGL(k_store_paged_rows<true>, grid, dim3(k_block), 0, (hipStream_t)stream, s, rows, st->T, st->index_err);
+        else hipLaunchKernelGGL(k_store_paged_rows<false>, grid, dim3(k_block), 0, (hipStream_t)stream, s, rows, st->T, st->index_err);
+        LNSHIP_HIP(hipGetLastError());
+        return 0;
+    }
     const int64_t y = std::min<int64_t>((nq + 2 * nk + k_block - 1) / k_block, 65535);
     hipLaunchKernelGGL(k_store_paged, dim3((unsigned)kv->ntok, (unsigned)y), dim3(k_block), 0, (hipStream_t)stream, s,
                        st->T, st->index_err);

@@ -18,6 +18,7 @@ _ready = set()
 
 c_i64 = ctypes.c_int64
 c_p = ctypes.c_void_p
+byref = ctypes.byref
 
 
 class LnshipError(RuntimeError):
@@ -240,6 +241,19 @@ def init(device=None):
 def _stream():
     import torch
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def current_stream(dev):
+    """The current stream, as a pointer, of device dev, which must be the
+    current one; uploads the tables to it at its first use.  For entry points
+    that are called once a token: it costs a tenth of init() and _stream()."""
+    import torch
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise LnshipError("tensors must be on the current device (they are on %s)" %
+                          ("the CPU" if dev < 0 else "cuda:%d" % dev))
+    if dev not in _ready:
+        init()
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _p(t):
@@ -477,10 +491,10 @@ def lfsr_advance(state, draws):
 
 # ---- drawing tokens ----------------------------------------------------------
 
-def _row_values(t, rows, dtype, name, device):
+def _row_values(t, rows, dtype, name, dev):
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != (rows,) or t.device != device or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != (rows,) or t.get_device() != dev or not t.is_contiguous():
         raise LnshipError(f"sample: {name} must be a contiguous {dtype} tensor of {rows} on the logits' device")
     return t.data_ptr()
 
@@ -492,26 +506,22 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=
     numbers u [n_rows].  Returns (tokens int32, probs float32), or fills the
     pair out; a row that holds no number above -inf gets token -1."""
     import torch
-    init()
-    dev = logits.device
-    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1 or not logits.is_cuda:
-        raise LnshipError("sample: logits must be float32 [n_rows, n_vocab] on the GPU, a row's values together")
-    if dev.index != torch.cuda.current_device():
-        raise LnshipError("sample: logits are not on the current device")
+    f32, i32 = torch.float32, torch.int32
+    dev = logits.get_device()
+    stream = current_stream(dev)
+    if logits.dtype != f32 or logits.dim() != 2 or logits.stride(1) != 1:
+        raise LnshipError("sample: logits must be float32 [n_rows, n_vocab], a row's values together")
     rows, vocab = logits.shape
-    tokens, probs = out if out is not None else (torch.empty(rows, dtype=torch.int32, device=dev),
-                                                 torch.empty(rows, dtype=torch.float32, device=dev))
+    tokens, probs = out if out is not None else (torch.empty(rows, dtype=i32, device=logits.device),
+                                                 torch.empty(rows, dtype=f32, device=logits.device))
     need = lib().lnship_sample_work(rows, vocab)
     if need < 0:
         check(need)
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
     a = SampleArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
-                   _row_values(temperature, rows, torch.float32, "temperature", dev),
-                   _row_values(top_k, rows, torch.int32, "top_k", dev),
-                   _row_values(top_p, rows, torch.float32, "top_p", dev),
-                   _row_values(min_p, rows, torch.float32, "min_p", dev),
-                   _row_values(u, rows, torch.float32, "u", dev),
-                   _row_values(tokens, rows, torch.int32, "tokens", dev),
-                   _row_values(probs, rows, torch.float32, "probs", dev), _p(work), need)
-    check(lib().lnship_sample(ctypes.byref(a), _stream()))
+                   _row_values(temperature, rows, f32, "temperature", dev), _row_values(top_k, rows, i32, "top_k", dev),
+                   _row_values(top_p, rows, f32, "top_p", dev), _row_values(min_p, rows, f32, "min_p", dev),
+                   _row_values(u, rows, f32, "u", dev), _row_values(tokens, rows, i32, "tokens", dev),
+                   _row_values(probs, rows, f32, "probs", dev), _p(work), need)
+    check(lib().lnship_sample(byref(a), stream))
     return tokens, probs

@@ -7,51 +7,57 @@ replays with other lengths and pages: q_start [n_seq + 1] (rows q_start[s] to
 q_start[s+1] - 1 are sequence s's new tokens), kv_len [n_seq] (its cells, the
 new tokens' included) and table [n_seq, pages a sequence may have].
 """
-import ctypes
+import torch
 
-from . import LnshipError, PagedAttnArgs, PagedKV, PagedStoreArgs, _stream, check, init, lib
+from . import LnshipError, PagedAttnArgs, PagedKV, PagedStoreArgs, byref, check, current_stream, lib
+
+_I16, _I32, _F32 = torch.int16, torch.int32, torch.float32
 
 
 def alloc_pages(n_pages, page, n_head_kv, head_dim, device="cuda"):
     """Key and value pages of one layer, empty: int16 [n_pages, n_head_kv, page * head_dim] each."""
-    import torch
     shape = (n_pages, n_head_kv, page * head_dim)
     return tuple(torch.zeros(shape, dtype=torch.int16, device=device) for _ in range(2))
 
 
-def _need(ok, what):
-    if not ok:
-        raise LnshipError("paged cache: " + what)
+def _no(what):
+    raise LnshipError("paged cache: " + what)
 
 
 def _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok):
-    import torch
-    dev = k_pages.device
-    _need(k_pages.is_cuda and dev.index == torch.cuda.current_device(), "the pages are not on the current device")
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        _need(t.dtype == torch.int16 and t.dim() == 3 and t.is_contiguous() and t.shape == k_pages.shape and
-              t.device == dev, name + " must be contiguous int16 [n_pages, n_head_kv, page * head_dim]")
-    for t, name in ((table, "table"), (q_start, "q_start"), (kv_len, "kv_len")):
-        _need(t.dtype == torch.int32 and t.device == dev, name + " must be int32 on the pages' device")
-    n_seq = kv_len.shape[0]
-    _need(kv_len.dim() == 1 and kv_len.is_contiguous(), "kv_len must be contiguous [n_seq]")
-    _need(q_start.shape == (n_seq + 1,) and q_start.is_contiguous(), "q_start must be contiguous [n_seq + 1]")
-    _need(table.dim() == 2 and table.shape[0] == n_seq and table.is_contiguous(),
-          "table must be contiguous [n_seq, pages]")
-    n_pages, n_head_kv, codes = k_pages.shape
-    _need(page > 0 and codes % page == 0, "pages of %d codes a head hold no %d cells" % (codes, page))
+    """lnship_paged_kv of the tensors, checked; and the device that all must be on, the current one."""
+    dev = k_pages.get_device()
+    shape = k_pages.shape
+    if k_pages.dtype != _I16 or k_pages.dim() != 3 or not k_pages.is_contiguous():
+        _no("k_pages must be contiguous int16 [n_pages, n_head_kv, page * head_dim]")
+    if v_pages.dtype != _I16 or v_pages.shape != shape or not v_pages.is_contiguous() or v_pages.get_device() != dev:
+        _no("v_pages must be as k_pages")
+    n_seq = kv_len.numel()
+    if kv_len.dtype != _I32 or kv_len.dim() != 1 or not kv_len.is_contiguous() or kv_len.get_device() != dev:
+        _no("kv_len must be contiguous int32 [n_seq] on the pages' device")
+    if q_start.dtype != _I32 or q_start.shape != (n_seq + 1,) or not q_start.is_contiguous() or \
+            q_start.get_device() != dev:
+        _no("q_start must be contiguous int32 [n_seq + 1] on the pages' device")
+    if table.dtype != _I32 or table.dim() != 2 or not table.is_contiguous() or table.get_device() != dev:
+        _no("table must be contiguous int32 [n_seq, pages] on the pages' device")
+    rows, width = table.shape
+    n_pages, n_head_kv, codes = shape
+    if rows != n_seq:
+        _no("table must have a row for every sequence")
+    if page < 1 or codes % page:
+        _no("pages of %d codes a head hold no %d cells" % (codes, page))
     return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, n_head_kv, codes // page, table.data_ptr(),
-                   table.shape[1], ntok, n_seq, q_start.data_ptr(), kv_len.data_ptr())
+                   width, ntok, n_seq, q_start.data_ptr(), kv_len.data_ptr()), dev
 
 
-def _rows(t, name, ntok, heads, dim, dev):
+def _ld(t, name, ntok, heads, dim, dev):
     """The row stride of a [ntok, heads, dim] float32 tensor whose heads lie behind each other."""
-    import torch
-    _need(t.dtype == torch.float32 and t.shape == (ntok, heads, dim) and t.device == dev,
-          "%s must be float32 [%d, %d, %d] on the pages' device" % (name, ntok, heads, dim))
-    s = t.stride()
-    _need(s[2] == 1 and (s[1] == dim or heads == 1), name + ": a row's heads must lie behind each other")
-    return s[0] if ntok > 1 else max(s[0], heads * dim)
+    if t.dtype != _F32 or t.shape != (ntok, heads, dim) or t.get_device() != dev:
+        _no("%s must be float32 [%d, %d, %d] on the pages' device" % (name, ntok, heads, dim))
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (s1 != dim and heads > 1):
+        _no(name + ": a row's heads must lie behind each other")
+    return s0 if ntok > 1 else max(s0, heads * dim)
 
 
 def rope_store_kv(q, k, v, k_pages, v_pages, page, table, q_start, kv_len, cos_sin, n_dims=None, neox=False, out=None):
@@ -60,25 +66,28 @@ def rope_store_kv(q, k, v, k_pages, v_pages, page, table, q_start, kv_len, cos_s
     v [ntok, n_head_kv, head_dim] float32: arrays, or the parts of a fused
     q|k|v product's rows; cos_sin [n_pos, n_dims / 2, 2] float32 (None with
     n_dims 0: nothing is rotated).  Returns the rotated queries."""
-    import torch
-    init()
     ntok = k.shape[0]
-    kv = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
-    dev, hd, nkv = k_pages.device, kv.head_dim, kv.n_head_kv
+    kv, dev = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
+    stream = current_stream(dev)
+    hd, nkv = kv.head_dim, kv.n_head_kv
     if n_dims is None:
         n_dims = hd if cos_sin is not None else 0
-    _need(n_dims == 0 or (cos_sin is not None and cos_sin.dtype == torch.float32 and cos_sin.dim() == 3 and
-                          cos_sin.shape[1:] == (n_dims // 2, 2) and cos_sin.is_contiguous() and
-                          cos_sin.device == dev), "cos_sin must be contiguous float32 [n_pos, n_dims / 2, 2]")
-    nh = q.shape[1] if q is not None else 0
-    if nh and out is None:
-        out = torch.empty((ntok, nh, hd), dtype=torch.float32, device=dev)
-    a = PagedStoreArgs(q.data_ptr() if nh else None, k.data_ptr(), v.data_ptr(),
-                       _rows(q, "q", ntok, nh, hd, dev) if nh else 0, _rows(k, "k", ntok, nkv, hd, dev),
-                       _rows(v, "v", ntok, nkv, hd, dev), nh, n_dims, int(neox),
-                       cos_sin.data_ptr() if n_dims else None, cos_sin.shape[0] if n_dims else 0,
-                       out.data_ptr() if nh else None, _rows(out, "out", ntok, nh, hd, dev) if nh else 0)
-    check(lib().lnship16_rope_store_kv_paged(ctypes.byref(kv), ctypes.byref(a), _stream()))
+    cs = n_pos = 0
+    if n_dims:
+        if cos_sin is None or cos_sin.dtype != _F32 or cos_sin.dim() != 3 or not cos_sin.is_contiguous() or \
+                cos_sin.get_device() != dev or cos_sin.shape[1:] != (n_dims // 2, 2):
+            _no("cos_sin must be contiguous float32 [n_pos, n_dims / 2, 2] on the pages' device")
+        cs, n_pos = cos_sin.data_ptr(), cos_sin.shape[0]
+    nh = q_ld = out_ld = q_at = out_at = 0
+    if q is not None:
+        nh = q.shape[1]
+        if out is None:
+            out = torch.empty((ntok, nh, hd), dtype=_F32, device=k_pages.device)
+        q_ld, out_ld = _ld(q, "q", ntok, nh, hd, dev), _ld(out, "out", ntok, nh, hd, dev)
+        q_at, out_at = q.data_ptr(), out.data_ptr()
+    a = PagedStoreArgs(q_at, k.data_ptr(), v.data_ptr(), q_ld, _ld(k, "k", ntok, nkv, hd, dev),
+                       _ld(v, "v", ntok, nkv, hd, dev), nh, n_dims, neox, cs, n_pos, out_at, out_ld)
+    check(lib().lnship16_rope_store_kv_paged(byref(kv), byref(a), stream))
     return out
 
 
@@ -87,20 +96,19 @@ def attention(q, k_pages, v_pages, page, table, q_start, kv_len, scale, window=0
     their sequences' cells in the pages: those up to each token's own position
     and, with window > 0, no further than window - 1 before it.  Returns out,
     [ntok, n_head, head_dim] float32."""
-    import torch
-    init()
-    ntok, nh = q.shape[0], q.shape[1]
-    kv = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
-    dev, hd = k_pages.device, kv.head_dim
+    ntok, nh = q.shape[:2]
+    kv, dev = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
+    stream = current_stream(dev)
+    hd = kv.head_dim
     if out is None:
-        out = torch.empty((ntok, nh, hd), dtype=torch.float32, device=dev)
-    q_ld, out_ld = _rows(q, "q", ntok, nh, hd, dev), _rows(out, "out", ntok, nh, hd, dev)
-    need = lib().lnship16_attn_paged_work(ctypes.byref(kv), nh)
+        out = torch.empty((ntok, nh, hd), dtype=_F32, device=k_pages.device)
+    q_ld, out_ld = _ld(q, "q", ntok, nh, hd, dev), _ld(out, "out", ntok, nh, hd, dev)
+    L, ref = lib(), byref(kv)
+    need = L.lnship16_attn_paged_work(ref, nh)
     if need < 0:
         check(need)
     # (of torch's allocator: the stream's own, a captured graph's own)
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    a = PagedAttnArgs(q.data_ptr(), out.data_ptr(), q_ld, out_ld, nh, scale, window,
-                      work.data_ptr() if need else None, need)
-    check(lib().lnship16_attn_paged(ctypes.byref(kv), ctypes.byref(a), _stream()))
+    work = torch.empty(need, dtype=torch.uint8, device=k_pages.device) if need else None
+    a = PagedAttnArgs(q.data_ptr(), out.data_ptr(), q_ld, out_ld, nh, scale, window, work.data_ptr() if need else 0, need)
+    check(L.lnship16_attn_paged(ref, byref(a), stream))
     return out
