@@ -419,17 +419,17 @@ __device__ __forceinline__ row_out out_row(const attn_paged_args &a, const row_t
     return {a.sums + part * hd, 1.0f};
 }
 
-// eight queries of a row from dim d on (zeros past head_dim)
+// Eight queries of a row from dim d on.  Past head_dim other ones are loaded
+// (in bounds) and made zeros: what is loaded is not written before it arrives,
+// or every load would be waited for.
 __device__ __forceinline__ void load_q(const float *q, int d, int hd, bool vec, float *x) {
-    if (d >= hd) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = 0.0f;
-    } else if (vec) {
-        const float4 u = *reinterpret_cast<const float4 *>(q + d), v = *reinterpret_cast<const float4 *>(q + d + 4);
+    q += min(d, hd - 8);
+    if (vec) {
+        const float4 u = *reinterpret_cast<const float4 *>(q), v = *reinterpret_cast<const float4 *>(q + 4);
         x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = q[d + j];
+        for (int j = 0; j < 8; j++) x[j] = q[j];
     }
 }
 
@@ -473,7 +473,8 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
     // a page of cell c, or page 0 (hidden cells: whatever it holds is finite)
     auto page_of = [&](int c) { return c < cend ? table[c >> a.page_sh] : 0; };
     auto sound = [&](int id) { return (uint32_t)id < (uint32_t)kv.n_pages; };
-    const uint4 zero = make_uint4(0, 0, 0, 0);
+    // (past head_dim the last dims are loaded again: the queries are zeros there,
+    // and those sums are not written)
     uint4 kc[2][NB], vc[2 * NB];
     auto load_k = [&](int cb, int id) {
         const int c = (cb + kcell) & (page - 1);
@@ -484,7 +485,6 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
             for (int i = 0; i < NB; i++) {
                 const int d8 = FULL ? i * 4 + g : min(i * 4 + g, hd / 8 - 1);
                 kc[t][i] = *reinterpret_cast<const uint4 *>(k + (d8 * page + 4 * t) * 8);
-                if (!FULL && (i * 4 + g) * 8 >= hd) kc[t][i] = zero;
             }
     };
     auto load_v = [&](int cb, int id) {
@@ -493,7 +493,6 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
         for (int i = 0; i < 2 * NB; i++) {
             const int d = FULL ? i * 16 + n : min(i * 16 + n, hd - 1);
             vc[i] = *reinterpret_cast<const uint4 *>(v + d * 8);
-            if (!FULL && i * 16 + n >= hd) vc[i] = zero;
         }
     };
 
@@ -517,7 +516,10 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[b][j]));
+            for (int j = 0; j < 8; j++) {
+                if (!FULL && b * 32 + g * 8 >= hd) x[b][j] = 0.0f;
+                mx = fmaxf(mx, fabsf(x[b][j]));
+            }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const int e = (int)(f32_bits(mx) >> 23) - 127;   // -127 for zeros
@@ -676,7 +678,10 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[kk][j]));
+            for (int j = 0; j < 8; j++) {
+                if (kk * 16 + h * 8 >= hd) x[kk][j] = 0.0f;
+                mx = fmaxf(mx, fabsf(x[kk][j]));
+            }
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const int e = (int)(f32_bits(mx) >> 23) - 127;
 #pragma unroll
@@ -692,6 +697,8 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     const uint16_t *kbase = kv.k_pages + kvh * head_codes, *vbase = kv.v_pages + kvh * head_codes;
     auto page_of = [&](int c) { return c < cend ? table[c >> a.page_sh] : 0; };
     auto sound = [&](int id) { return (uint32_t)id < (uint32_t)kv.n_pages; };
+    // (past head_dim the last dims are loaded again: the queries are zeros there,
+    // and those sums are not written)
     // unit u of the keys: dims u / 64 * 8.., cell u % 64 of the tile (the same
     // for all of a thread's); of the values: cells u / HD * 8.., dim u % HD
     uint4 kc[UT], vc[UT];
@@ -708,14 +715,12 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
         for (int i = 0; i < UT; i++) {
             const int d8 = (tid + i * NT) >> 6;
             kc[i] = *reinterpret_cast<const uint4 *>(k + min(d8, hd / 8 - 1) * page * 8);
-            if (d8 * 8 >= hd) kc[i] = make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < UT; i++) {
             const int c8 = (tid + i * NT) / HD, d = (tid + i * NT) % HD;
             const uint16_t *v = vbase + (sound(vid[i]) ? vid[i] : 0) * page_codes + ((cb + c8 * 8) & (page - 1)) * hd;
             vc[i] = *reinterpret_cast<const uint4 *>(v + min(d, hd - 1) * 8);
-            if (d >= hd) vc[i] = make_uint4(0, 0, 0, 0);
         }
     };
     // the cell's row of its block's key product: a lane's 16 results are then
