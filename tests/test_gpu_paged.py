@@ -386,6 +386,20 @@ def test_pages_past_32_bits(ln):
     assert (np.abs(got - ref) <= tol).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 7, 31, 97, 250, 255, 256])
+def test_a_pool_of_one_page(ln, hd, n):
+    """The only page is the last one of the pool: loads ahead of the last cells stay inside it."""
+    rng = np.random.default_rng(n)
+    for q_len in (1, min(n, 70)):
+        c = R.Cache(1, 256, 2, hd)
+        keys, vals = (R.store_codes(rng.standard_normal((n, 2, hd)).astype(np.float32)) for _ in range(2))
+        c.put([0], np.arange(n), keys, vals)
+        q = rng.standard_normal((q_len, 4, hd)).astype(np.float32)
+        got = run_attn(ln, q, c, np.int32([[0]]), [q_len], [n]).cpu().numpy()
+        check_attn(got, q, [q_len], [n], [keys], [vals])
+
+
 def test_long_cache_of_one_token(ln):
     """Many splits: the parts of a long cache are joined."""
     rng = np.random.default_rng(18)

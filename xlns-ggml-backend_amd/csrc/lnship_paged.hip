@@ -264,6 +264,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));   // rows of any alignment
 
 struct attn_paged_args {
     lnship_paged_kv kv;
@@ -470,8 +471,8 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
     // the lane's cells of a block: as a row of the key products (4 of each of
     // the two), and of its eight scores
     const int kcell = 8 * (n >> 2), vcell = 8 * g;
-    // a page of cell c, or page 0 (hidden cells: whatever it holds is finite)
-    auto page_of = [&](int c) { return c < cend ? table[c >> a.page_sh] : 0; };
+    // the page of cell c (of hidden cells: another's, whatever it holds is finite)
+    auto page_of = [&](int c) { return table[min(c, cend - 1) >> a.page_sh]; };
     auto sound = [&](int id) { return (uint32_t)id < (uint32_t)kv.n_pages; };
     // (past head_dim the last dims are loaded again: the queries are zeros there,
     // and those sums are not written)
@@ -501,10 +502,22 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
     for (int i = 0; i < 2 * NB; i++) o[i] = float4v{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
     int cb = T.c0 + split * T.per * 64 + wave * 32;
-    int vid = page_of(cb + vcell), kid = page_of(cb + kcell);
+    // (a page's number is used before the next one is loaded into its place, so
+    // that no copy of it waits for loads behind it)
+    int vid = 0, kid = 0;
+    bool vok = false;
+    auto sound_v = [&](int cb) {
+        vok = cb + vcell < cend && sound(vid);
+        if (cb + vcell < cend && !vok) index_fault(err, vid);
+    };
     if (cb < cend) {
+        kid = page_of(cb + kcell);
+        vid = page_of(cb + vcell);
         load_k(cb, kid);
+        kid = page_of(cb + 128 + kcell);
+        sound_v(cb);
         load_v(cb, vid);
+        vid = page_of(cb + 128 + vcell);
     }
     // the queries as halves, scaled by the row's largest to at most 2: by the
     // first wave, for all
@@ -536,9 +549,6 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
     __syncthreads();
     const float qs = s_qs[n];
     for (; cb < cend; cb += 128) {
-        const int vid1 = page_of(cb + 128 + vcell), kid1 = page_of(cb + 128 + kcell);
-        const bool vok = cb + vcell < cend && sound(vid);
-        if (cb + vcell < cend && !vok) index_fault(err, vid);
         float4v sh[2], sx[2];
         sh[0] = sh[1] = sx[0] = sx[1] = float4v{0, 0, 0, 0};
 #pragma unroll
@@ -555,7 +565,8 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
                 sx[t] = mma(kh, ql, sx[t]);
             }
         }
-        load_k(min(cb + 128, cend - 1), kid1);
+        load_k(cb + 128, kid);
+        kid = page_of(cb + 256 + kcell);
         float s[8], mb = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -591,9 +602,9 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
             o[i] = mma(vh, pl, o[i]);
             o[i] = mma(vl, pc, o[i]);
         }
-        load_v(min(cb + 128, cend - 1), vid1);
-        kid = kid1;
-        vid = vid1;
+        sound_v(cb + 128);
+        load_v(cb + 128, vid);
+        vid = page_of(cb + 256 + vcell);
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -631,6 +642,9 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
     const row_out out = out_row(a, T, split, tok2, head2, M2, L2, (threadIdx.x & 15) == 0);
     for (int d = threadIdx.x & 15; d < hd; d += 16) out.dst[d] = s_o[rr][d] * out.f;
 }
+
+// A barrier that waits for LDS alone: loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Many rows a sequence (prompts, chunks): NW waves of 32 rows each go over the
 // cells together, 64 at a time.  Every code is decoded once a workgroup, by the
@@ -695,7 +709,7 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     const int32_t *table = kv.table + (int64_t)T.sq * kv.table_ld;
     const int64_t head_codes = (int64_t)page * hd, page_codes = nkv * head_codes;
     const uint16_t *kbase = kv.k_pages + kvh * head_codes, *vbase = kv.v_pages + kvh * head_codes;
-    auto page_of = [&](int c) { return c < cend ? table[c >> a.page_sh] : 0; };
+    auto page_of = [&](int c) { return table[min(c, cend - 1) >> a.page_sh]; };
     auto sound = [&](int id) { return (uint32_t)id < (uint32_t)kv.n_pages; };
     // (past head_dim the last dims are loaded again: the queries are zeros there,
     // and those sums are not written)
@@ -707,7 +721,7 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     auto pages = [&](int cb) {
         kid = page_of(cb + (tid & 63));
 #pragma unroll
-        for (int i = 0; i < UT; i++) vid[i] = has(i) ? page_of(cb + (tid + i * NT) / HD * 8) : 0;
+        for (int i = 0; i < UT; i++) vid[i] = page_of(cb + (tid + i * NT) / HD * 8);
     };
     auto load = [&](int cb) {
         const uint16_t *k = kbase + (sound(kid) ? kid : 0) * page_codes + ((cb + (tid & 63)) & (page - 1)) * 8;
@@ -727,7 +741,7 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     // cells 8 h + 0..7 and 16 + 8 h + 0..7 of the block
     const int kcell = tid & 63, kin = kcell & 31;
     const int krow = 8 * ((kin >> 4) * 2 + ((kin >> 2) & 1)) + 4 * ((kin >> 3) & 1) + (kin & 3);
-    auto store = [&](int buf, int cb, const int *ids) {
+    auto store = [&](int buf, uint32_t ok) {
         uint4 *s = s_tile + buf * 4 * U;
 #pragma unroll
         for (int i = 0; i < UT; i++) {
@@ -748,37 +762,55 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
             const int at = (c8 >> 2) * (U / 2) + (d >> 5) * 128 + ((c8 >> 1) & 1) * 64 + (c8 & 1) * 32 + (d & 31);
             s[2 * U + at] = hi.w;
             s[3 * U + at] = lo.w;
-            if (d == 0) {
-                const int c = cb + c8 * 8;
-                s_ok[buf][c8] = c < cend && sound(ids[i]);
-                if (c < cend && !sound(ids[i])) index_fault(err, ids[i]);
-            }
+            if (d == 0) s_ok[buf][c8] = ok >> i & 1;
         }
+    };
+
+    // Whether the pages of the thread's values, for the tile at cb, are sound.
+    // Taken from the pages' numbers before the next ones are loaded, so that no
+    // copy of a number waits for its load (and with it for all before it).
+    auto sound_pages = [&](int cb) {
+        uint32_t ok = 0;
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            const bool in = has(i) && cb + (tid + i * NT) / HD * 8 < cend;
+            if (in && sound(vid[i])) ok |= 1u << i;
+            else if (in) index_fault(err, vid[i]);
+        }
+        return ok;
     };
 
     float16v o[NB];
 #pragma unroll
     for (int i = 0; i < NB; i++) o[i] = float16v{};
     float m = -INFINITY, l = 0.0f;
-    int ids[UT];
+    // Codes are loaded a tile ahead of their decoding, which goes into the other
+    // buffer.  Half of the waves decode before their products, half behind them:
+    // on a SIMD one wave then forms weights or decodes while the other multiplies
+    // (in step, both would wait for the matrix core and then leave it idle).
+    uint32_t ok_next = 0;
     if (cbeg < cend) {
         pages(cbeg);
         load(cbeg);
-#pragma unroll
-        for (int i = 0; i < UT; i++) ids[i] = vid[i];
+        ok_next = sound_pages(cbeg);
         pages(cbeg + 64);
-        store(0, cbeg, ids);
+        store(0, ok_next);
+        load(cbeg + 64);   // (past the last tile: page 0, not used)
+        ok_next = sound_pages(cbeg + 64);
+        pages(cbeg + 128);
     }
-    __syncthreads();
+    lds_barrier();
+    auto prepare = [&](int cb, int buf) {   // the tile at cb into buf, the loads of the one behind it
+        if (cb >= cend) return;
+        store(buf, ok_next);
+        load(cb + 64);
+        ok_next = sound_pages(cb + 64);
+        pages(cb + 128);
+    };
+    const bool early = NW == 8 && wave >= NW / 2;
     int buf = 0;
     for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
-        const bool more = cb + 64 < cend;
-        if (more) {
-            load(cb + 64);
-#pragma unroll
-            for (int i = 0; i < UT; i++) ids[i] = vid[i];
-            pages(cb + 128);
-        }
+        if (early) prepare(cb + 64, buf ^ 1);
         if (wave_has) {
             const frag *s = reinterpret_cast<const frag *>(s_tile + buf * 4 * U) + lane;
 #pragma unroll 1
@@ -843,8 +875,8 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
                     }
             }
         }
-        if (more) store(buf ^ 1, cb + 64, ids);
-        __syncthreads();
+        if (!early) prepare(cb + 64, buf ^ 1);
+        lds_barrier();
     }
     l += __shfl_xor(l, 32);
     if (!have) return;
@@ -852,9 +884,10 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
 #pragma unroll
     for (int i = 0; i < NB; i++)
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const int d = i * 32 + 8 * (j >> 2) + 4 * h + (j & 3);
-            if (d < hd) out.dst[d] = o[i][j] * out.f;
+        for (int j = 0; j < 16; j += 4) {
+            const int d = i * 32 + 2 * j + 4 * h;
+            const float4v x = {o[i][j] * out.f, o[i][j + 1] * out.f, o[i][j + 2] * out.f, o[i][j + 3] * out.f};
+            if (d < hd) *reinterpret_cast<float4u *>(out.dst + d) = x;
         }
 }
 
