@@ -266,6 +266,21 @@ def test_attention_against_64_bits(ln, q_len, kv_len, page, nh, nkv, hd, window)
     assert np.array_equal(got, run_attn(ln, q, c, table, q_len, kv_len, window).cpu().numpy())   # run to run
 
 
+@pytest.mark.parametrize("q_len,kv_len,page,nh,nkv,hd,window", [
+    ([300], [300], 16, 9, 3, 64, 0), ([70, 5], [70, 333], 32, 5, 1, 96, 0), ([131], [260], 64, 16, 1, 128, 0),
+    ([40, 90], [300, 90], 16, 4, 4, 24, 50), ([520, 1, 90], [800, 50, 90], 32, 8, 2, 64, 0)])
+def test_chunks_behind_a_table_of_many_pages(ln, q_len, kv_len, page, nh, nkv, hd, window):
+    """Tables of more cells than the workspace holds decoded: each workgroup decodes what it sees."""
+    rng = np.random.default_rng(hd)
+    q, c, table, keys, vals = attn_case(rng, q_len, kv_len, page, nh, nkv, hd)
+    narrow = run_attn(ln, q, c, table, q_len, kv_len, window).cpu().numpy()
+    wide = np.full((len(q_len), (1 << 30) // (nkv * 8 * ((hd + 31) // 32 * 32) * page * len(q_len)) + 3), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    got = run_attn(ln, q, c, wide, q_len, kv_len, window).cpu().numpy()
+    check_attn(got, q, q_len, kv_len, keys, vals, window)
+    check_attn(narrow, q, q_len, kv_len, keys, vals, window)
+
+
 @pytest.mark.parametrize("qscale,kstd,vstd", [(1e-6, 1.0, 1.0), (30.0, 1.0, 1.0), (1.0, 1e-3, 1e-3),
                                               (1e4, 1e-4, 500.0), (1.0, 20.0, 8000.0), (1e-30, 1.0, 1e-2)])
 @pytest.mark.parametrize("q_len,kv_len", [([1], [200]), ([100], [180])])

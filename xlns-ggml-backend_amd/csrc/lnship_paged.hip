@@ -280,6 +280,10 @@ struct attn_paged_args {
     float *sums;
     float2 *stats;
     int *used;
+    // k_attn_decode's tiles [n_seq][pre_tiles][n_head_kv], and the flags of their groups of eight cells
+    uint4 *pre;
+    uint8_t *pre_ok;
+    int pre_tiles;
 };
 
 constexpr int k_lo_sh = 11;             // the low halves are scaled by 2^11
@@ -643,26 +647,160 @@ __global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_at
     for (int d = threadIdx.x & 15; d < hd; d += 16) out.dst[d] = s_o[rr][d] * out.f;
 }
 
-// A barrier that waits for LDS alone: loads from memory stay in flight.
+// A barrier that waits for LDS alone: loads from memory stay in flight; and one
+// that waits for them too (copies into LDS among them).
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ void copy_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Copies 16 bytes a lane from memory to LDS, from `to` on in the lanes' order,
+// without a register between.
+__device__ __forceinline__ void copy_to_lds(const uint4 *from, uint4 *to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+// 64 cells of one kv head as split halves, in the order in which k_attn_chunk's
+// products read them (a lane's 16 bytes of an operand behind the lane before's):
+// U units of the keys' high halves, of their low ones, of the values' high and
+// low ones.  Past head_dim the last dims are repeated: the queries are zeros
+// there, and those sums are not written.
+template <int NB>
+struct tile_of {
+    static constexpr int HD = NB * 32;
+    static constexpr int U = 64 * HD / 8;   // 16-byte units of 64 cells' keys, and values
+};
+
+// A workgroup of NT threads that makes such tiles of the cells [.., cend) of one
+// sequence: a thread loads its units' codes ahead, then decodes them.  Unit u of
+// the keys: dims u / 64 * 8.., cell u % 64 of the tile (the same for all of a
+// thread's); of the values: cells u / HD * 8.., dim u % HD.
+template <int NB, int NT>
+struct tile_maker {
+    static constexpr int HD = tile_of<NB>::HD, U = tile_of<NB>::U, UT = (U + NT - 1) / NT;
+    const int32_t *table;
+    const uint16_t *kbase, *vbase;
+    int64_t page_codes;
+    int cend, page_sh, page, hd, n_pages;
+    unsigned long long *err;
+    uint4 kc[UT], vc[UT];
+    int kid, vid[UT];   // the pages of the next units to load
+
+    __device__ __forceinline__ tile_maker(const lnship_paged_kv &kv, int sq, int kvh, int sh, int end, unsigned long long *e)
+        : table(kv.table + (int64_t)sq * kv.table_ld), cend(end), page_sh(sh), page((int)kv.page), hd((int)kv.head_dim),
+          n_pages((int)kv.n_pages), err(e) {
+        const int64_t head_codes = (int64_t)page * hd;
+        page_codes = kv.n_head_kv * head_codes;
+        kbase = kv.k_pages + kvh * head_codes;
+        vbase = kv.v_pages + kvh * head_codes;
+    }
+    __device__ __forceinline__ bool has(int i) const { return (i + 1) * NT <= U || (int)threadIdx.x + i * NT < U; }
+    // the page of cell c (of hidden cells: another's, whatever it holds is finite)
+    __device__ __forceinline__ int page_of(int c) const { return table[min(c, cend - 1) >> page_sh]; }
+    __device__ __forceinline__ bool sound(int id) const { return (uint32_t)id < (uint32_t)n_pages; }
+    __device__ __forceinline__ void pages(int cb) {
+        kid = page_of(cb + (threadIdx.x & 63));
+#pragma unroll
+        for (int i = 0; i < UT; i++) vid[i] = page_of(cb + ((int)threadIdx.x + i * NT) / HD * 8);
+    }
+    __device__ __forceinline__ void load(int cb) {
+        const int tid = threadIdx.x;
+        const uint16_t *k = kbase + (sound(kid) ? kid : 0) * page_codes + ((cb + (tid & 63)) & (page - 1)) * 8;
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            const int d8 = (tid + i * NT) >> 6;
+            kc[i] = *reinterpret_cast<const uint4 *>(k + min(d8, hd / 8 - 1) * page * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            const int c8 = (tid + i * NT) / HD, d = (tid + i * NT) % HD;
+            const uint16_t *v = vbase + (sound(vid[i]) ? vid[i] : 0) * page_codes + ((cb + c8 * 8) & (page - 1)) * hd;
+            vc[i] = *reinterpret_cast<const uint4 *>(v + min(d, hd - 1) * 8);
+        }
+    }
+    // Whether the pages of the thread's values, for the tile at cb, are sound.
+    // Taken from the pages' numbers before the next ones are loaded, so that no
+    // copy of a number waits for its load (and with it for all before it).
+    __device__ __forceinline__ uint32_t sound_pages(int cb) const {
+        uint32_t ok = 0;
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            const bool in = has(i) && cb + ((int)threadIdx.x + i * NT) / HD * 8 < cend;
+            if (in && sound(vid[i])) ok |= 1u << i;
+            else if (in) index_fault(err, vid[i]);
+        }
+        return ok;
+    }
+    // decodes the loaded codes into the tile s; its groups of eight cells' flags into oks
+    __device__ __forceinline__ void store(uint4 *s, uint32_t ok, uint8_t *oks) const {
+        const int tid = threadIdx.x;
+        // the cell's row of its block's key product: a lane's 16 results are
+        // then cells 8 h + 0..7 and 16 + 8 h + 0..7 of the block
+        const int cell = tid & 63, in = cell & 31;
+        const int row = 8 * ((in >> 4) * 2 + ((in >> 2) & 1)) + 4 * ((in >> 3) & 1) + (in & 3);
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            frag hi, lo;
+            decode8(kc[i], hi, lo);
+            if (!has(i)) continue;
+            const int d8 = (tid + i * NT) >> 6;
+            const int at = (cell >> 5) * (U / 2) + (d8 >> 1) * 64 + (d8 & 1) * 32 + row;
+            s[at] = hi.w;
+            s[U + at] = lo.w;
+        }
+#pragma unroll
+        for (int i = 0; i < UT; i++) {
+            frag hi, lo;
+            decode8(vc[i], hi, lo);
+            if (!has(i)) continue;
+            const int c8 = (tid + i * NT) / HD, d = (tid + i * NT) % HD;
+            const int at = (c8 >> 2) * (U / 2) + (d >> 5) * 128 + ((c8 >> 1) & 1) * 64 + (c8 & 1) * 32 + (d & 31);
+            s[2 * U + at] = hi.w;
+            s[3 * U + at] = lo.w;
+            if (oks && d == 0) oks[c8] = ok >> i & 1;
+        }
+    }
+};
+
+// The cells that a chunk sees, decoded into the workspace, for k_attn_chunk to
+// copy: a workgroup takes every gridDim.x-th tile of a sequence and kv head.
+template <int NB>
+__global__ __launch_bounds__(256) void k_attn_decode(attn_paged_args a, unsigned long long *err) {
+    const lnship_paged_kv &kv = a.kv;
+    const int nkv = (int)kv.n_head_kv, kvh = (int)(blockIdx.y % (uint32_t)nkv);
+    for (int sq = (int)(blockIdx.y / (uint32_t)nkv); sq < (int)kv.n_seq; sq += (int)(gridDim.y / (uint32_t)nkv)) {
+        const int64_t start = kv.q_start[sq], end = kv.q_start[sq + 1];
+        const int cend = (int)max(min((int64_t)kv.kv_len[sq], kv.table_ld << a.page_sh), (int64_t)0);
+        if (end <= start) continue;
+        // the first cell that the sequence's first token sees
+        const int64_t first = kv.kv_len[sq] - (end - start) - a.window + 1;
+        const int lo = a.window > 0 ? (int)(min(max(first, (int64_t)0), (int64_t)cend) >> 6) : 0;
+        tile_maker<NB, 256> t(kv, sq, kvh, a.page_sh, cend, err);
+        for (int i = lo + (int)blockIdx.x; i * 64 < cend; i += (int)gridDim.x) {
+            t.pages(i * 64);
+            t.load(i * 64);
+            const uint32_t ok = t.sound_pages(i * 64);
+            const int64_t at = (int64_t)sq * a.pre_tiles + i;
+            t.store(a.pre + (at * nkv + kvh) * 4 * tile_of<NB>::U, ok, kvh == 0 ? a.pre_ok + at * 8 : nullptr);
+        }
+    }
+}
 
 // Many rows a sequence (prompts, chunks): NW waves of 32 rows each go over the
-// cells together, 64 at a time.  Every code is decoded once a workgroup, by the
-// thread that loaded it, into split halves in LDS, in the order in which the
-// products read them: each operand is one 16-byte read a lane of consecutive
-// addresses.  Products are 32 x 32 x 16, transposed as above; a lane has 16
-// scores of one row.  Two LDS buffers: while one is multiplied the next tile's
-// codes are in flight; they are decoded into the other before the barrier.
-template <int NB, int NW>   // 32-wide groups of head_dim; waves
+// cells together, 64 at a time, from tiles of split halves in LDS: each operand
+// is one 16-byte read a lane of consecutive addresses.  Products are 32 x 32 x
+// 16, transposed as above; a lane has 16 scores of one row.  Two LDS buffers:
+// while one is multiplied the other is filled, with PRE by copies of tiles that
+// k_attn_decode has made, else by the workgroup's own decoding of codes that
+// were loaded a tile before.
+template <int NB, int NW, bool PRE>   // 32-wide groups of head_dim; waves
 __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsigned long long *err) {
-    constexpr int HD = NB * 32, NT = NW * 64, KK = HD / 16;
-    constexpr int U = 64 * HD / 8;        // 16-byte units of a tile's keys, and of its values
-    constexpr int UT = (U + NT - 1) / NT; // of a thread
-    extern __shared__ uint4 s_tile[];     // [2][keys high, low, values high, low][U]
-    __shared__ alignas(16) int s_ok[2][8];   // whether a tile's groups of eight cells lie in a page
+    constexpr int NT = NW * 64, KK = NB * 2, U = tile_of<NB>::U;
+    static_assert(4 * U % NT == 0, "whole copies");
+    extern __shared__ uint4 s_tile[];          // [2][4 U]
+    __shared__ alignas(16) uint8_t s_ok[2][8];   // whether a tile's groups of eight cells lie in a page
     const lnship_paged_kv &kv = a.kv;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, h = lane >> 5;
-    const int rep = a.rep, nkv = (int)kv.n_head_kv, hd = (int)kv.head_dim, page = (int)kv.page;
+    const int rep = a.rep, nkv = (int)kv.n_head_kv, hd = (int)kv.head_dim;
     // kv heads side by side (on the XCDs' L2s), the last tiles (most cells) first
     const int kvh = (int)(blockIdx.x % (uint32_t)nkv), split = blockIdx.y;
     const int tile = (int)(gridDim.x / (uint32_t)nkv) - 1 - (int)(blockIdx.x / (uint32_t)nkv);
@@ -681,6 +819,39 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     const int wlast = T.pos0 + (int)((uint32_t)(min(wrow + 32, T.rows) - 1) / (uint32_t)rep);
     const int all_lo = a.window > 0 ? wlast - a.window : -1, any_lo = a.window > 0 ? wfirst - a.window : -1;
     const bool wave_has = wrow < T.rows;
+
+    // how the next tile gets into a buffer: begin(cb) starts it, ahead of
+    // multiplying, finish() ends it before the barrier
+    tile_maker<NB, NT> maker(kv, T.sq, kvh, a.page_sh, cend, err);
+    const int64_t tiles0 = (int64_t)T.sq * a.pre_tiles;
+    uint2 ok_pre = make_uint2(0, 0), ok_now = make_uint2(0, 0);   // (PRE) flags of the tile being copied, of the one in use
+    uint32_t ok_next = 0;
+    auto copy = [&](int cb, int buf) {
+        const int64_t at = tiles0 + (cb >> 6);
+        const uint4 *from = a.pre + (at * nkv + kvh) * 4 * U + tid;
+#pragma unroll
+        for (int i = 0; i < 4 * U / NT; i++)
+            copy_to_lds(from + i * NT, s_tile + buf * 4 * U + i * NT + wave * 64);
+        ok_pre = *reinterpret_cast<const uint2 *>(a.pre_ok + at * 8);
+    };
+    auto prepare = [&](int cb, int buf) {   // the tile at cb into buf, the loads of the one behind it
+        if (cb >= cend) return;
+        maker.store(s_tile + buf * 4 * U, ok_next, s_ok[buf]);
+        maker.load(cb + 64);   // (past the last tile: other cells of a page, not used)
+        ok_next = maker.sound_pages(cb + 64);
+        maker.pages(cb + 128);
+    };
+    if (cbeg < cend) {
+        if constexpr (PRE) {
+            copy(cbeg, 0);
+        } else {
+            maker.pages(cbeg);
+            maker.load(cbeg);
+            ok_next = maker.sound_pages(cbeg);
+            maker.pages(cbeg + 64);
+            prepare(cbeg, 0);
+        }
+    }
 
     frag qh[KK], ql[KK];
     float qs;
@@ -705,111 +876,19 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
                 split2(ldexpf(x[kk][j], -e), ldexpf(x[kk][j + 1], -e), qh[kk].u[j / 2], ql[kk].u[j / 2]);
         qs = ldexpf(a.scale, e);
     }
-
-    const int32_t *table = kv.table + (int64_t)T.sq * kv.table_ld;
-    const int64_t head_codes = (int64_t)page * hd, page_codes = nkv * head_codes;
-    const uint16_t *kbase = kv.k_pages + kvh * head_codes, *vbase = kv.v_pages + kvh * head_codes;
-    auto page_of = [&](int c) { return table[min(c, cend - 1) >> a.page_sh]; };
-    auto sound = [&](int id) { return (uint32_t)id < (uint32_t)kv.n_pages; };
-    // (past head_dim the last dims are loaded again: the queries are zeros there,
-    // and those sums are not written)
-    // unit u of the keys: dims u / 64 * 8.., cell u % 64 of the tile (the same
-    // for all of a thread's); of the values: cells u / HD * 8.., dim u % HD
-    uint4 kc[UT], vc[UT];
-    int kid, vid[UT];
-    auto has = [&](int i) { return (i + 1) * NT <= U || tid + i * NT < U; };   // the thread's last unit may not be one
-    auto pages = [&](int cb) {
-        kid = page_of(cb + (tid & 63));
-#pragma unroll
-        for (int i = 0; i < UT; i++) vid[i] = page_of(cb + (tid + i * NT) / HD * 8);
-    };
-    auto load = [&](int cb) {
-        const uint16_t *k = kbase + (sound(kid) ? kid : 0) * page_codes + ((cb + (tid & 63)) & (page - 1)) * 8;
-#pragma unroll
-        for (int i = 0; i < UT; i++) {
-            const int d8 = (tid + i * NT) >> 6;
-            kc[i] = *reinterpret_cast<const uint4 *>(k + min(d8, hd / 8 - 1) * page * 8);
-        }
-#pragma unroll
-        for (int i = 0; i < UT; i++) {
-            const int c8 = (tid + i * NT) / HD, d = (tid + i * NT) % HD;
-            const uint16_t *v = vbase + (sound(vid[i]) ? vid[i] : 0) * page_codes + ((cb + c8 * 8) & (page - 1)) * hd;
-            vc[i] = *reinterpret_cast<const uint4 *>(v + min(d, hd - 1) * 8);
-        }
-    };
-    // the cell's row of its block's key product: a lane's 16 results are then
-    // cells 8 h + 0..7 and 16 + 8 h + 0..7 of the block
-    const int kcell = tid & 63, kin = kcell & 31;
-    const int krow = 8 * ((kin >> 4) * 2 + ((kin >> 2) & 1)) + 4 * ((kin >> 3) & 1) + (kin & 3);
-    auto store = [&](int buf, uint32_t ok) {
-        uint4 *s = s_tile + buf * 4 * U;
-#pragma unroll
-        for (int i = 0; i < UT; i++) {
-            frag hi, lo;
-            decode8(kc[i], hi, lo);
-            if (!has(i)) continue;
-            const int d8 = (tid + i * NT) >> 6;
-            const int at = (kcell >> 5) * (U / 2) + (d8 >> 1) * 64 + (d8 & 1) * 32 + krow;
-            s[at] = hi.w;
-            s[U + at] = lo.w;
-        }
-#pragma unroll
-        for (int i = 0; i < UT; i++) {
-            frag hi, lo;
-            decode8(vc[i], hi, lo);
-            if (!has(i)) continue;
-            const int c8 = (tid + i * NT) / HD, d = (tid + i * NT) % HD;
-            const int at = (c8 >> 2) * (U / 2) + (d >> 5) * 128 + ((c8 >> 1) & 1) * 64 + (c8 & 1) * 32 + (d & 31);
-            s[2 * U + at] = hi.w;
-            s[3 * U + at] = lo.w;
-            if (d == 0) s_ok[buf][c8] = ok >> i & 1;
-        }
-    };
-
-    // Whether the pages of the thread's values, for the tile at cb, are sound.
-    // Taken from the pages' numbers before the next ones are loaded, so that no
-    // copy of a number waits for its load (and with it for all before it).
-    auto sound_pages = [&](int cb) {
-        uint32_t ok = 0;
-#pragma unroll
-        for (int i = 0; i < UT; i++) {
-            const bool in = has(i) && cb + (tid + i * NT) / HD * 8 < cend;
-            if (in && sound(vid[i])) ok |= 1u << i;
-            else if (in) index_fault(err, vid[i]);
-        }
-        return ok;
-    };
-
     float16v o[NB];
 #pragma unroll
     for (int i = 0; i < NB; i++) o[i] = float16v{};
     float m = -INFINITY, l = 0.0f;
-    // Codes are loaded a tile ahead of their decoding, which goes into the other
-    // buffer.  Half of the waves decode before their products, half behind them:
-    // on a SIMD one wave then forms weights or decodes while the other multiplies
-    // (in step, both would wait for the matrix core and then leave it idle).
-    uint32_t ok_next = 0;
-    if (cbeg < cend) {
-        pages(cbeg);
-        load(cbeg);
-        ok_next = sound_pages(cbeg);
-        pages(cbeg + 64);
-        store(0, ok_next);
-        load(cbeg + 64);   // (past the last tile: page 0, not used)
-        ok_next = sound_pages(cbeg + 64);
-        pages(cbeg + 128);
-    }
-    lds_barrier();
-    auto prepare = [&](int cb, int buf) {   // the tile at cb into buf, the loads of the one behind it
-        if (cb >= cend) return;
-        store(buf, ok_next);
-        load(cb + 64);
-        ok_next = sound_pages(cb + 64);
-        pages(cb + 128);
-    };
-    const bool early = NW == 8 && wave >= NW / 2;
+    if (PRE) copy_barrier();
+    else lds_barrier();
+    // Half of the waves decode before their products, half behind them: on a
+    // SIMD one wave then forms weights or decodes while the other multiplies.
+    const bool early = !PRE && NW == 8 && wave >= NW / 2;
     int buf = 0;
     for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
+        if (PRE) ok_now = ok_pre;
+        if (PRE && cb + 64 < cend) copy(cb + 64, buf ^ 1);
         if (early) prepare(cb + 64, buf ^ 1);
         if (wave_has) {
             const frag *s = reinterpret_cast<const frag *>(s_tile + buf * 4 * U) + lane;
@@ -825,15 +904,16 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
                     sx = mma(kl, qh[kk], sx);
                     sx = mma(kh, ql[kk], sx);
                 }
-                const int4 ok = *reinterpret_cast<const int4 *>(&s_ok[buf][blk * 4]);
+                const uint32_t ok = PRE ? (blk ? ok_now.y : ok_now.x)
+                                        : (uint32_t)__builtin_amdgcn_readfirstlane(
+                                              (int)*reinterpret_cast<const uint32_t *>(&s_ok[buf][blk * 4]));
                 float p[16], mb = -INFINITY;
                 const float sub = (m == -INFINITY ? 0.0f : m) - k_p_sh;
 #pragma unroll
                 for (int j = 0; j < 16; j++) p[j] = fmaf(sx[j], qs * k_lo_inv, fmaf(sh[j], qs, -sub));
-                const int ok_all = __builtin_amdgcn_readfirstlane(ok.x & ok.y & ok.z & ok.w);
-                if (b0 + 31 > wfirst || b0 + 31 >= T.c1 || b0 <= all_lo || !ok_all) {
+                if (b0 + 31 > wfirst || b0 + 31 >= T.c1 || b0 <= all_lo || ok != 0x01010101u) {
                     asm volatile("");   // a branch: few blocks need it
-                    const bool ok0 = h ? ok.y : ok.x, ok1 = h ? ok.w : ok.z;
+                    const bool ok0 = ok >> (8 * h) & 1, ok1 = ok >> (16 + 8 * h) & 1;
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
                         const int cell = b0 + (j >> 3) * 16 + h * 8 + (j & 7);
@@ -875,8 +955,9 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
                     }
             }
         }
-        if (!early) prepare(cb + 64, buf ^ 1);
-        lds_barrier();
+        if (!PRE && !early) prepare(cb + 64, buf ^ 1);
+        if (PRE) copy_barrier();
+        else lds_barrier();
     }
     l += __shfl_xor(l, 32);
     if (!have) return;
@@ -985,7 +1066,10 @@ static int log2_of(int64_t page) {
 // of a tile, tiles, and the parts that a row's cells are split into.
 struct attn_plan {
     int waves, tile_rows, splits, min_per;
+    bool pre;   // cells decoded once, into the workspace
     int64_t tiles;
+    // the workspace: bytes of the splits' parts, of the decoded tiles, of their flags
+    int64_t parts_bytes, pre_bytes, ok_bytes, pre_tiles;
 };
 #ifndef LNSHIP_TGT
 #define LNSHIP_TGT 8
@@ -1005,6 +1089,10 @@ struct attn_plan {
 #ifndef LNSHIP_CHUNK_ROWS8
 #define LNSHIP_CHUNK_ROWS8 384
 #endif
+#ifndef LNSHIP_PRE
+#define LNSHIP_PRE 1
+#endif
+constexpr int64_t k_pre_bytes = (int64_t)1 << 30;   // of the workspace for decoded cells, at most
 static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
     attn_plan p;
     const int64_t rows = kv->ntok * rep, of_seq = kv->n_seq ? rows / kv->n_seq : 0;
@@ -1016,35 +1104,46 @@ static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
     const int64_t most = (kv->table_ld * kv->page / 64 + p.min_per - 1) / p.min_per;
     const int64_t want = p.waves ? LNSHIP_TGT2 : LNSHIP_TGT;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want * cus + wgs - 1) / wgs, most, 256}));
+    const int64_t n_head = rep * kv->n_head_kv, hdp = (kv->head_dim + 31) & ~(int64_t)31;
+    p.parts_bytes = p.splits > 1 ? (kv->ntok * n_head * (p.splits * (kv->head_dim + 2) + 1) * 4 + 255) & ~(int64_t)255 : 0;
+    p.pre_tiles = (kv->table_ld * kv->page + 63) / 64;
+    const int64_t tile_bytes = kv->n_head_kv * 64 * hdp * 8;
+    p.pre = p.waves > 0 && kv->n_seq * p.pre_tiles <= k_pre_bytes / tile_bytes && LNSHIP_PRE;
+    p.pre_bytes = p.pre ? kv->n_seq * p.pre_tiles * tile_bytes : 0;
+    p.ok_bytes = p.pre ? (kv->n_seq * p.pre_tiles * 8 + 255) & ~(int64_t)255 : 0;
     return p;
 }
 
-static int64_t attn_work(const lnship_paged_kv *kv, int64_t n_head, int splits) {
-    return splits > 1 ? kv->ntok * n_head * (splits * (kv->head_dim + 2) + 1) * 4 : 0;
-}
-
-template <int NB, int NW>
+template <int NB, int NW, bool PRE>
 static int launch_chunk(const attn_paged_args &m, const attn_plan &p, hipStream_t s, unsigned long long *err) {
-    const int lds = 2 * 4 * 64 * NB * 32 * 2;
+    const int lds = 2 * 4 * tile_of<NB>::U * 16;
     static std::atomic<uint64_t> done{0};   // devices that know the kernel's LDS
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
     if (!(done.load() >> dev & 1)) {
-        LNSHIP_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_chunk<NB, NW>),
+        LNSHIP_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_chunk<NB, NW, PRE>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         done.fetch_or((uint64_t)1 << dev);
     }
-    hipLaunchKernelGGL((k_attn_chunk<NB, NW>), dim3((unsigned)(p.tiles * m.kv.n_head_kv), (unsigned)p.splits),
+    hipLaunchKernelGGL((k_attn_chunk<NB, NW, PRE>), dim3((unsigned)(p.tiles * m.kv.n_head_kv), (unsigned)p.splits),
                        dim3(NW * 64), lds, s, m, err);
     LNSHIP_HIP(hipGetLastError());
     return 0;
 }
 
 template <int NB>
-static int launch_attn(const attn_paged_args &m, const attn_plan &p, hipStream_t s, unsigned long long *err) {
+static int launch_attn(const attn_paged_args &m, const attn_plan &p, int cus, hipStream_t s, unsigned long long *err) {
     if constexpr (NB <= 4) {
-        if (p.waves == 4) return launch_chunk<NB, 4>(m, p, s, err);
-        if (p.waves == 8) return launch_chunk<NB, 8>(m, p, s, err);
+        if (p.pre) {
+            // (a grid's y and z are counted in 16 bits)
+            const int64_t y = std::min<int64_t>(m.kv.n_seq, 65535 / m.kv.n_head_kv) * m.kv.n_head_kv;
+            const int64_t x = std::max<int64_t>(1, std::min<int64_t>(p.pre_tiles, 8 * cus / y));
+            hipLaunchKernelGGL(k_attn_decode<NB>, dim3((unsigned)x, (unsigned)y), dim3(256), 0, s, m, err);
+            LNSHIP_HIP(hipGetLastError());
+            return p.waves == 4 ? launch_chunk<NB, 4, true>(m, p, s, err) : launch_chunk<NB, 8, true>(m, p, s, err);
+        }
+        if (p.waves == 4) return launch_chunk<NB, 4, false>(m, p, s, err);
+        if (p.waves == 8) return launch_chunk<NB, 8, false>(m, p, s, err);
     }
     const dim3 grid((unsigned)p.tiles, (unsigned)m.kv.n_head_kv, (unsigned)p.splits);
     if (m.kv.head_dim == NB * 32) hipLaunchKernelGGL((k_attn_paged<NB, true>), grid, dim3(256), 0, s, m, err);
@@ -1098,7 +1197,8 @@ int64_t lnship16_attn_paged_work(const lnship_paged_kv *kv, int64_t n_head) {
         return fail(LNSHIP_EINVAL, "attn_paged: n_head not a multiple of n_head_kv%s");
     device_state *st = state();
     if (!st) return LNSHIP_ENOINIT;
-    return attn_work(kv, n_head, plan_attn(kv, n_head / kv->n_head_kv, st->cus).splits);
+    const attn_plan p = plan_attn(kv, n_head / kv->n_head_kv, st->cus);
+    return p.parts_bytes + p.pre_bytes + p.ok_bytes;
 }
 
 int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args *a, void *stream) {
@@ -1114,7 +1214,7 @@ int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args 
     if (!st) return LNSHIP_ENOINIT;
     const int64_t rep = a->n_head / kv->n_head_kv;
     const attn_plan p = plan_attn(kv, rep, st->cus);
-    const int64_t need = attn_work(kv, a->n_head, p.splits);
+    const int64_t need = p.parts_bytes + p.pre_bytes + p.ok_bytes;
     if (need && (!a->work || a->work_bytes < (size_t)need || ((uintptr_t)a->work & 15)))
         return fail(LNSHIP_EINVAL, "attn_paged: work smaller than lnship16_attn_paged_work or not aligned%s");
     // (a grid's threads along x are counted in 32 bits)
@@ -1122,25 +1222,31 @@ int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args 
         return fail(LNSHIP_ERANGE, "attn_paged: grid too large%s");
     attn_paged_args m{*kv, a->q, a->dst, q_ld, dst_ld, a->scale * 1.44269504088896341f,
                       a->window > 0x3fffffff ? 0 : (int)a->window, (int)a->n_head, (int)rep, log2_of(kv->page), p.splits,
-                      p.tile_rows, p.min_per, q_ld % 4 == 0 && ((uintptr_t)a->q & 15) == 0, nullptr, nullptr, nullptr};
+                      p.tile_rows, p.min_per, q_ld % 4 == 0 && ((uintptr_t)a->q & 15) == 0};
     const int64_t all = kv->ntok * a->n_head;
-    if (need) {
-        m.sums = (float *)a->work;
+    char *work = (char *)a->work;
+    if (p.splits > 1) {
+        m.sums = (float *)work;
         m.stats = (float2 *)(m.sums + p.splits * all * kv->head_dim);
         m.used = (int *)(m.stats + p.splits * all);
+    }
+    if (p.pre) {
+        m.pre = (uint4 *)(work + p.parts_bytes);
+        m.pre_ok = (uint8_t *)(work + p.parts_bytes + p.pre_bytes);
+        m.pre_tiles = (int)p.pre_tiles;
     }
     if (kv->n_pages == 0) m.kv.table_ld = 0;   // no page to read: no cells
     hipStream_t s = (hipStream_t)stream;
     int rc;
     switch ((kv->head_dim + 31) / 32) {
-        case 1: rc = launch_attn<1>(m, p, s, st->index_err); break;
-        case 2: rc = launch_attn<2>(m, p, s, st->index_err); break;
-        case 3: rc = launch_attn<3>(m, p, s, st->index_err); break;
-        case 4: rc = launch_attn<4>(m, p, s, st->index_err); break;
-        case 5: rc = launch_attn<5>(m, p, s, st->index_err); break;
-        case 6: rc = launch_attn<6>(m, p, s, st->index_err); break;
-        case 7: rc = launch_attn<7>(m, p, s, st->index_err); break;
-        default: rc = launch_attn<8>(m, p, s, st->index_err);
+        case 1: rc = launch_attn<1>(m, p, st->cus, s, st->index_err); break;
+        case 2: rc = launch_attn<2>(m, p, st->cus, s, st->index_err); break;
+        case 3: rc = launch_attn<3>(m, p, st->cus, s, st->index_err); break;
+        case 4: rc = launch_attn<4>(m, p, st->cus, s, st->index_err); break;
+        case 5: rc = launch_attn<5>(m, p, st->cus, s, st->index_err); break;
+        case 6: rc = launch_attn<6>(m, p, st->cus, s, st->index_err); break;
+        case 7: rc = launch_attn<7>(m, p, st->cus, s, st->index_err); break;
+        default: rc = launch_attn<8>(m, p, st->cus, s, st->index_err);
     }
     if (rc || p.splits == 1) return rc;
     if (p.splits > 8) hipLaunchKernelGGL(k_attn_paged_join<4>, dim3((unsigned)all), dim3(256), 0, s, m);
