@@ -447,6 +447,9 @@ __device__ __forceinline__ void load_q(const float *q, int d, int hd, bool vec, 
 // 16-byte loads, straight from memory.  The next block's keys are loaded while
 // this one's weights are formed, its values once this one's are decoded.
 template <int NB, bool FULL>   // 32-wide groups of head_dim; whether it fills them
+#ifndef LNSHIP_CW
+#define LNSHIP_CW 3
+#endif
 #ifndef LNSHIP_W
 #define LNSHIP_W 3
 #endif
@@ -659,15 +662,16 @@ __device__ __forceinline__ void copy_to_lds(const uint4 *from, uint4 *to) {
                                      (__attribute__((address_space(3))) void *)to, 16, 0, 0);
 }
 
-// 64 cells of one kv head as split halves, in the order in which k_attn_chunk's
-// products read them (a lane's 16 bytes of an operand behind the lane before's):
-// U units of the keys' high halves, of their low ones, of the values' high and
-// low ones.  Past head_dim the last dims are repeated: the queries are zeros
-// there, and those sums are not written.
+// 64 cells of one kv head as split halves, in the order in which the products of
+// chunk_rows read them (a lane's 16 bytes of an operand behind the lane
+// before's): for each block of 32 cells B units of the keys' high halves, of
+// their low ones, of the values' high and low ones.  Past head_dim the last dims
+// are repeated: the queries are zeros there, and those sums are not written.
 template <int NB>
 struct tile_of {
     static constexpr int HD = NB * 32;
-    static constexpr int U = 64 * HD / 8;   // 16-byte units of 64 cells' keys, and values
+    static constexpr int B = 32 * HD / 8;   // 16-byte units of 32 cells' keys, and values
+    static constexpr int U = 2 * B;
 };
 
 // A workgroup of NT threads that makes such tiles of the cells [.., cend) of one
@@ -676,7 +680,7 @@ struct tile_of {
 // thread's); of the values: cells u / HD * 8.., dim u % HD.
 template <int NB, int NT>
 struct tile_maker {
-    static constexpr int HD = tile_of<NB>::HD, U = tile_of<NB>::U, UT = (U + NT - 1) / NT;
+    static constexpr int HD = tile_of<NB>::HD, B = tile_of<NB>::B, U = 2 * B, UT = (U + NT - 1) / NT;
     const int32_t *table;
     const uint16_t *kbase, *vbase;
     int64_t page_codes;
@@ -743,9 +747,9 @@ struct tile_maker {
             decode8(kc[i], hi, lo);
             if (!has(i)) continue;
             const int d8 = (tid + i * NT) >> 6;
-            const int at = (cell >> 5) * (U / 2) + (d8 >> 1) * 64 + (d8 & 1) * 32 + row;
-            s[at] = hi.w;
-            s[U + at] = lo.w;
+            uint4 *to = s + (cell >> 5) * 4 * B + (d8 >> 1) * 64 + (d8 & 1) * 32 + row;
+            to[0] = hi.w;
+            to[B] = lo.w;
         }
 #pragma unroll
         for (int i = 0; i < UT; i++) {
@@ -753,9 +757,9 @@ struct tile_maker {
             decode8(vc[i], hi, lo);
             if (!has(i)) continue;
             const int c8 = (tid + i * NT) / HD, d = (tid + i * NT) % HD;
-            const int at = (c8 >> 2) * (U / 2) + (d >> 5) * 128 + ((c8 >> 1) & 1) * 64 + (c8 & 1) * 32 + (d & 31);
-            s[2 * U + at] = hi.w;
-            s[3 * U + at] = lo.w;
+            uint4 *to = s + (c8 >> 2) * 4 * B + (d >> 5) * 128 + ((c8 >> 1) & 1) * 64 + (c8 & 1) * 32 + (d & 31);
+            to[2 * B] = hi.w;
+            to[3 * B] = lo.w;
             if (oks && d == 0) oks[c8] = ok >> i & 1;
         }
     }
@@ -785,77 +789,38 @@ __global__ __launch_bounds__(256) void k_attn_decode(attn_paged_args a, unsigned
     }
 }
 
-// Many rows a sequence (prompts, chunks): NW waves of 32 rows each go over the
-// cells together, 64 at a time, from tiles of split halves in LDS: each operand
-// is one 16-byte read a lane of consecutive addresses.  Products are 32 x 32 x
-// 16, transposed as above; a lane has 16 scores of one row.  Two LDS buffers:
-// while one is multiplied the other is filled, with PRE by copies of tiles that
-// k_attn_decode has made, else by the workgroup's own decoding of codes that
-// were loaded a tile before.
-template <int NB, int NW, bool PRE>   // 32-wide groups of head_dim; waves
-__global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsigned long long *err) {
-    constexpr int NT = NW * 64, KK = NB * 2, U = tile_of<NB>::U;
-    static_assert(4 * U % NT == 0, "whole copies");
-    extern __shared__ uint4 s_tile[];          // [2][4 U]
-    __shared__ alignas(16) uint8_t s_ok[2][8];   // whether a tile's groups of eight cells lie in a page
-    const lnship_paged_kv &kv = a.kv;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, h = lane >> 5;
-    const int rep = a.rep, nkv = (int)kv.n_head_kv, hd = (int)kv.head_dim;
-    // kv heads side by side (on the XCDs' L2s), the last tiles (most cells) first
-    const int kvh = (int)(blockIdx.x % (uint32_t)nkv), split = blockIdx.y;
-    const int tile = (int)(gridDim.x / (uint32_t)nkv) - 1 - (int)(blockIdx.x / (uint32_t)nkv);
-    const row_tile T = find_tile(a, tile, err);
-    if (T.r0 < 0 || (split > 0 && split * T.per >= T.blocks)) return;
-    const int cbeg = T.c0 + split * T.per * 64, cend = min(T.c1, cbeg + T.per * 64);
-
-    const int wrow = T.r0 + wave * 32;   // the wave's rows
-    const bool have = wrow + n < T.rows;
-    const int row = have ? wrow + n : min(wrow, T.rows - 1), tok = T.t0 + (int)((uint32_t)row / (uint32_t)rep);
-    const int head = kvh * rep + (int)((uint32_t)row % (uint32_t)rep);
-    const int pos = min(T.pos0 + tok - T.t0, T.c1 - 1);
-    const int lo_cell = a.window > 0 ? T.pos0 + tok - T.t0 - a.window : -1;
-    // what all of the wave's rows see, and any does
-    const int wfirst = T.pos0 + (int)((uint32_t)min(wrow, T.rows - 1) / (uint32_t)rep);
-    const int wlast = T.pos0 + (int)((uint32_t)(min(wrow + 32, T.rows) - 1) / (uint32_t)rep);
-    const int all_lo = a.window > 0 ? wlast - a.window : -1, any_lo = a.window > 0 ? wfirst - a.window : -1;
-    const bool wave_has = wrow < T.rows;
-
-    // how the next tile gets into a buffer: begin(cb) starts it, ahead of
-    // multiplying, finish() ends it before the barrier
-    tile_maker<NB, NT> maker(kv, T.sq, kvh, a.page_sh, cend, err);
-    const int64_t tiles0 = (int64_t)T.sq * a.pre_tiles;
-    uint2 ok_pre = make_uint2(0, 0), ok_now = make_uint2(0, 0);   // (PRE) flags of the tile being copied, of the one in use
-    uint32_t ok_next = 0;
-    auto copy = [&](int cb, int buf) {
-        const int64_t at = tiles0 + (cb >> 6);
-        const uint4 *from = a.pre + (at * nkv + kvh) * 4 * U + tid;
-#pragma unroll
-        for (int i = 0; i < 4 * U / NT; i++)
-            copy_to_lds(from + i * NT, s_tile + buf * 4 * U + i * NT + wave * 64);
-        ok_pre = *reinterpret_cast<const uint2 *>(a.pre_ok + at * 8);
-    };
-    auto prepare = [&](int cb, int buf) {   // the tile at cb into buf, the loads of the one behind it
-        if (cb >= cend) return;
-        maker.store(s_tile + buf * 4 * U, ok_next, s_ok[buf]);
-        maker.load(cb + 64);   // (past the last tile: other cells of a page, not used)
-        ok_next = maker.sound_pages(cb + 64);
-        maker.pages(cb + 128);
-    };
-    if (cbeg < cend) {
-        if constexpr (PRE) {
-            copy(cbeg, 0);
-        } else {
-            maker.pages(cbeg);
-            maker.load(cbeg);
-            ok_next = maker.sound_pages(cbeg);
-            maker.pages(cbeg + 64);
-            prepare(cbeg, 0);
-        }
-    }
-
+// A wave's 32 rows of a tile and their running sums.  Products are 32 x 32 x 16,
+// transposed as above; a lane has 16 scores of one row (row n, with the lane 32
+// on, which has the block's other cells).
+template <int NB>
+struct chunk_rows {
+    static constexpr int KK = NB * 2, B = tile_of<NB>::B;
+    int h, tok, head, pos, lo_cell;
+    int wfirst, wlast, all_lo, any_lo;   // what all of the wave's rows see, and any does
+    bool have, any;
     frag qh[KK], ql[KK];
-    float qs;
-    {
+    float qs, m, l;
+    float16v o[NB];
+
+    __device__ __forceinline__ void place(const attn_paged_args &a, const row_tile &T, int kvh, int wrow) {
+        const int lane = threadIdx.x & 63, n = lane & 31;
+        const uint32_t rep = (uint32_t)a.rep;
+        h = lane >> 5;
+        any = wrow < T.rows;
+        have = wrow + n < T.rows;
+        const int row = have ? wrow + n : min(wrow, T.rows - 1);
+        tok = T.t0 + (int)((uint32_t)row / rep);
+        head = kvh * a.rep + (int)((uint32_t)row % rep);
+        pos = min(T.pos0 + tok - T.t0, T.c1 - 1);
+        lo_cell = a.window > 0 ? T.pos0 + tok - T.t0 - a.window : -1;
+        wfirst = T.pos0 + (int)((uint32_t)min(wrow, T.rows - 1) / rep);
+        wlast = T.pos0 + (int)((uint32_t)(min(wrow + 32, T.rows) - 1) / rep);
+        all_lo = a.window > 0 ? wlast - a.window : -1;
+        any_lo = a.window > 0 ? wfirst - a.window : -1;
+    }
+    // the queries as halves, scaled by the row's largest to at most 2
+    __device__ __forceinline__ void load(const attn_paged_args &a) {
+        const int hd = (int)a.kv.head_dim;
         float x[KK][8], mx = 0.0f;
         const float *q = a.q + tok * a.q_ld + (int64_t)head * hd;
 #pragma unroll
@@ -868,108 +833,192 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
                 mx = fmaxf(mx, fabsf(x[kk][j]));
             }
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const int e = (int)(f32_bits(mx) >> 23) - 127;
+        const int e = (int)(f32_bits(mx) >> 23) - 127;   // -127 for zeros
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
 #pragma unroll
             for (int j = 0; j < 8; j += 2)
                 split2(ldexpf(x[kk][j], -e), ldexpf(x[kk][j + 1], -e), qh[kk].u[j / 2], ql[kk].u[j / 2]);
         qs = ldexpf(a.scale, e);
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NB; i++) o[i] = float16v{};
     }
-    float16v o[NB];
+    // the block of 32 cells from b0 on, at s in LDS; ok: a byte for each eight of
+    // them, 1 where they lie in a page; c1: the end of the tile's cells
+    __device__ __forceinline__ void block(const uint4 *tile, int b0, uint32_t ok, int c1) {
+        if (!any || b0 > wlast || b0 + 31 <= any_lo) return;
+        const frag *s = reinterpret_cast<const frag *>(tile) + (threadIdx.x & 63);
+        float16v sh{}, sx{};
 #pragma unroll
-    for (int i = 0; i < NB; i++) o[i] = float16v{};
-    float m = -INFINITY, l = 0.0f;
-    if (PRE) copy_barrier();
-    else lds_barrier();
-    // Half of the waves decode before their products, half behind them: on a
-    // SIMD one wave then forms weights or decodes while the other multiplies.
-    const bool early = !PRE && NW == 8 && wave >= NW / 2;
-    int buf = 0;
-    for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
-        if (PRE) ok_now = ok_pre;
-        if (PRE && cb + 64 < cend) copy(cb + 64, buf ^ 1);
-        if (early) prepare(cb + 64, buf ^ 1);
-        if (wave_has) {
-            const frag *s = reinterpret_cast<const frag *>(s_tile + buf * 4 * U) + lane;
-#pragma unroll 1
-            for (int blk = 0; blk < 2; blk++) {
-                const int b0 = cb + blk * 32;
-                if (b0 > wlast || b0 + 31 <= any_lo) continue;
-                float16v sh{}, sx{};
+        for (int kk = 0; kk < KK; kk++) {
+            const frag kh = s[kk * 64], kl = s[B + kk * 64];
+            sh = mma(kh, qh[kk], sh);
+            sx = mma(kl, qh[kk], sx);
+            sx = mma(kh, ql[kk], sx);
+        }
+        float p[16], mb = -INFINITY;
+        const float sub = (m == -INFINITY ? 0.0f : m) - k_p_sh;
 #pragma unroll
-                for (int kk = 0; kk < KK; kk++) {
-                    const frag kh = s[blk * (U / 2) + kk * 64], kl = s[U + blk * (U / 2) + kk * 64];
-                    sh = mma(kh, qh[kk], sh);
-                    sx = mma(kl, qh[kk], sx);
-                    sx = mma(kh, ql[kk], sx);
-                }
-                const uint32_t ok = PRE ? (blk ? ok_now.y : ok_now.x)
-                                        : (uint32_t)__builtin_amdgcn_readfirstlane(
-                                              (int)*reinterpret_cast<const uint32_t *>(&s_ok[buf][blk * 4]));
-                float p[16], mb = -INFINITY;
-                const float sub = (m == -INFINITY ? 0.0f : m) - k_p_sh;
+        for (int j = 0; j < 16; j++) p[j] = fmaf(sx[j], qs * k_lo_inv, fmaf(sh[j], qs, -sub));
+        if (b0 + 31 > wfirst || b0 + 31 >= c1 || b0 <= all_lo || ok != 0x01010101u) {
+            asm volatile("");   // a branch: few blocks need it
+            const bool ok0 = ok >> (8 * h) & 1, ok1 = ok >> (16 + 8 * h) & 1;
 #pragma unroll
-                for (int j = 0; j < 16; j++) p[j] = fmaf(sx[j], qs * k_lo_inv, fmaf(sh[j], qs, -sub));
-                if (b0 + 31 > wfirst || b0 + 31 >= T.c1 || b0 <= all_lo || ok != 0x01010101u) {
-                    asm volatile("");   // a branch: few blocks need it
-                    const bool ok0 = ok >> (8 * h) & 1, ok1 = ok >> (16 + 8 * h) & 1;
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int cell = b0 + (j >> 3) * 16 + h * 8 + (j & 7);
-                        if (!(j < 8 ? ok0 : ok1) || cell > pos || cell <= lo_cell) p[j] = -INFINITY;
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 16; j++) mb = fmaxf(mb, p[j]);
-                // p holds the scores less sub: the first block, and where the maximum has grown far
-                if (__any(m == -INFINITY ? mb != -INFINITY : mb > (float)(k_p_sh + k_p_lag))) {
-                    mb = fmaxf(mb, __shfl_xor(mb, 32));
-                    const float mn = fmaxf(m, mb + sub);
-                    const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-                    const float more_sub = (mn == -INFINITY ? 0.0f : mn) - k_p_sh - sub;
-#pragma unroll
-                    for (int j = 0; j < 16; j++) p[j] -= more_sub;
-                    m = mn;
-                    l *= alpha;
-#pragma unroll
-                    for (int i = 0; i < NB; i++) o[i] *= alpha;
-                }
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    p[j] = __builtin_amdgcn_exp2f(p[j]);
-                    l += p[j];
-                }
-                frag ph[2], pl[2], pc[2];
-                split_p(p, ph[0], pl[0], pc[0]);
-                split_p(p + 8, ph[1], pl[1], pc[1]);
-#pragma unroll
-                for (int i = 0; i < NB; i++)
-#pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        const int at = blk * (U / 2) + i * 128 + t * 64;
-                        const frag vh = s[2 * U + at], vl = s[3 * U + at];
-                        o[i] = mma(vh, ph[t], o[i]);
-                        o[i] = mma(vh, pl[t], o[i]);
-                        o[i] = mma(vl, pc[t], o[i]);
-                    }
+            for (int j = 0; j < 16; j++) {
+                const int cell = b0 + (j >> 3) * 16 + h * 8 + (j & 7);
+                if (!(j < 8 ? ok0 : ok1) || cell > pos || cell <= lo_cell) p[j] = -INFINITY;
             }
         }
-        if (!PRE && !early) prepare(cb + 64, buf ^ 1);
-        if (PRE) copy_barrier();
-        else lds_barrier();
-    }
-    l += __shfl_xor(l, 32);
-    if (!have) return;
-    const row_out out = out_row(a, T, split, tok, head, m, l, h == 0);
 #pragma unroll
-    for (int i = 0; i < NB; i++)
+        for (int j = 0; j < 16; j++) mb = fmaxf(mb, p[j]);
+        // p holds the scores less sub: the first block, and where the maximum has grown far
+        if (__any(m == -INFINITY ? mb != -INFINITY : mb > (float)(k_p_sh + k_p_lag))) {
+            mb = fmaxf(mb, __shfl_xor(mb, 32));
+            const float mn = fmaxf(m, mb + sub);
+            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float more_sub = (mn == -INFINITY ? 0.0f : mn) - k_p_sh - sub;
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            const int d = i * 32 + 2 * j + 4 * h;
-            const float4v x = {o[i][j] * out.f, o[i][j + 1] * out.f, o[i][j + 2] * out.f, o[i][j + 3] * out.f};
-            if (d < hd) *reinterpret_cast<float4u *>(out.dst + d) = x;
+            for (int j = 0; j < 16; j++) p[j] -= more_sub;
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < NB; i++) o[i] *= alpha;
         }
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            p[j] = __builtin_amdgcn_exp2f(p[j]);
+            l += p[j];
+        }
+        frag ph[2], pl[2], pc[2];
+        split_p(p, ph[0], pl[0], pc[0]);
+        split_p(p + 8, ph[1], pl[1], pc[1]);
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const frag vh = s[2 * B + i * 128 + t * 64], vl = s[3 * B + i * 128 + t * 64];
+                o[i] = mma(vh, ph[t], o[i]);
+                o[i] = mma(vh, pl[t], o[i]);
+                o[i] = mma(vl, pc[t], o[i]);
+            }
+    }
+    __device__ __forceinline__ void write(const attn_paged_args &a, const row_tile &T, int split) {
+        const int hd = (int)a.kv.head_dim;
+        l += __shfl_xor(l, 32);
+        if (!have) return;
+        const row_out out = out_row(a, T, split, tok, head, m, l, h == 0);
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                const int d = i * 32 + 2 * j + 4 * h;
+                const float4v x = {o[i][j] * out.f, o[i][j + 1] * out.f, o[i][j + 2] * out.f, o[i][j + 3] * out.f};
+                if (d < hd) *reinterpret_cast<float4u *>(out.dst + d) = x;
+            }
+    }
+};
+
+// the tile, kv head and split of a workgroup: kv heads side by side (on the
+// XCDs' L2s), the last tiles (most cells) first
+__device__ __forceinline__ int chunk_tile(int nkv, int &kvh) {
+    kvh = (int)(blockIdx.x % (uint32_t)nkv);
+    return (int)(gridDim.x / (uint32_t)nkv) - 1 - (int)(blockIdx.x / (uint32_t)nkv);
+}
+
+// Many rows a sequence (prompts, chunks), over cells that k_attn_decode has
+// decoded: four waves of 32 rows go over them 32 at a time, from two LDS
+// buffers; while one is multiplied the next block is copied into the other.
+// Small workgroups, two or more on a CU: a barrier holds only waves of other
+// SIMDs together, so that on each SIMD one workgroup's wave multiplies while
+// another's forms weights.
+template <int NB>
+__global__ __launch_bounds__(256, NB <= 2 ? LNSHIP_CW : 2) void k_attn_tiles(attn_paged_args a, unsigned long long *err) {
+    constexpr int B = tile_of<NB>::B;
+    static_assert(4 * B % 256 == 0, "whole copies");
+    __shared__ uint4 s_tile[2][4 * B];
+    const int tid = threadIdx.x, wave = tid >> 6, nkv = (int)a.kv.n_head_kv, split = blockIdx.y;
+    int kvh;
+    const int tile = chunk_tile(nkv, kvh);
+    const row_tile T = find_tile(a, tile, err);
+    if (T.r0 < 0 || (split > 0 && split * T.per >= T.blocks)) return;
+    const int cbeg = T.c0 + split * T.per * 64, cend = min(T.c1, cbeg + T.per * 64);
+    const uint4 *from = a.pre + ((int64_t)T.sq * a.pre_tiles * nkv + kvh) * 8 * B + tid;
+    const uint32_t *oks = reinterpret_cast<const uint32_t *>(a.pre_ok) + (int64_t)T.sq * a.pre_tiles * 2;
+    uint32_t ok_next = 0;
+    auto copy = [&](int b0, int buf) {
+        const uint4 *f = from + (int64_t)(b0 >> 6) * nkv * 8 * B + (b0 >> 5 & 1) * 4 * B;
+#pragma unroll
+        for (int i = 0; i < 4 * B / 256; i++) copy_to_lds(f + i * 256, &s_tile[buf][i * 256 + wave * 64]);
+        ok_next = oks[b0 >> 5];
+    };
+    if (cbeg < cend) copy(cbeg, 0);
+    chunk_rows<NB> r;
+    r.place(a, T, kvh, T.r0 + wave * 32);
+    r.load(a);
+    copy_barrier();
+    int buf = 0;
+    for (int b0 = cbeg; b0 < cend; b0 += 32, buf ^= 1) {
+        const uint32_t ok = ok_next;
+        if (b0 + 32 < cend) copy(b0 + 32, buf ^ 1);
+        r.block(s_tile[buf], b0, ok, T.c1);
+        copy_barrier();
+    }
+    r.write(a, T, split);
+}
+
+// The same where the tables' cells are more than the workspace holds decoded:
+// NW waves go over 64 cells at a time and decode the codes themselves, each once
+// a workgroup, by the thread that loaded it a tile before, into the other of
+// two LDS buffers.
+template <int NB, int NW>   // 32-wide groups of head_dim; waves
+__global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsigned long long *err) {
+    constexpr int U = tile_of<NB>::U;
+    extern __shared__ uint4 s_cells[];         // [2][4 U]
+    __shared__ alignas(16) uint8_t s_ok[2][8];   // whether a tile's groups of eight cells lie in a page
+    const int wave = threadIdx.x >> 6, split = blockIdx.y;
+    int kvh;
+    const int tile = chunk_tile((int)a.kv.n_head_kv, kvh);
+    const row_tile T = find_tile(a, tile, err);
+    if (T.r0 < 0 || (split > 0 && split * T.per >= T.blocks)) return;
+    const int cbeg = T.c0 + split * T.per * 64, cend = min(T.c1, cbeg + T.per * 64);
+    tile_maker<NB, NW * 64> maker(a.kv, T.sq, kvh, a.page_sh, cend, err);
+    uint32_t ok_next = 0;
+    auto prepare = [&](int cb, int buf) {   // the tile at cb into buf, the loads of the one behind it
+        if (cb >= cend) return;
+        maker.store(s_cells + buf * 4 * U, ok_next, s_ok[buf]);
+        maker.load(cb + 64);   // (past the last tile: other cells of a page, not used)
+        ok_next = maker.sound_pages(cb + 64);
+        maker.pages(cb + 128);
+    };
+    if (cbeg < cend) {
+        maker.pages(cbeg);
+        maker.load(cbeg);
+        ok_next = maker.sound_pages(cbeg);
+        maker.pages(cbeg + 64);
+        prepare(cbeg, 0);
+    }
+    chunk_rows<NB> r;
+    r.place(a, T, kvh, T.r0 + wave * 32);
+    r.load(a);
+    lds_barrier();
+    // Half of the waves decode before their products, half behind them: on a
+    // SIMD one wave then forms weights or decodes while the other multiplies.
+    const bool early = NW == 8 && wave >= NW / 2;
+    int buf = 0;
+    for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
+        if (early) prepare(cb + 64, buf ^ 1);
+#pragma unroll 1
+        for (int blk = 0; blk < 2; blk++) {
+            const uint32_t ok = (uint32_t)__builtin_amdgcn_readfirstlane(
+                (int)*reinterpret_cast<const uint32_t *>(&s_ok[buf][blk * 4]));
+            r.block(s_cells + buf * 4 * U + blk * 2 * U, cb + blk * 32, ok, T.c1);
+        }
+        if (!early) prepare(cb + 64, buf ^ 1);
+        lds_barrier();
+    }
+    r.write(a, T, split);
 }
 
 // The splits' parts of a row joined, in a fixed order, by one wave (four rows a
@@ -1062,7 +1111,7 @@ static int log2_of(int64_t page) {
     return sh;
 }
 
-// How a call runs: k_attn_chunk with `waves` waves, or (0) k_attn_paged; rows
+// How a call runs: k_attn_tiles (pre) or k_attn_chunk with `waves` waves, or (0) k_attn_paged; rows
 // of a tile, tiles, and the parts that a row's cells are split into.
 struct attn_plan {
     int waves, tile_rows, splits, min_per;
@@ -1096,7 +1145,13 @@ constexpr int64_t k_pre_bytes = (int64_t)1 << 30;   // of the workspace for deco
 static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
     attn_plan p;
     const int64_t rows = kv->ntok * rep, of_seq = kv->n_seq ? rows / kv->n_seq : 0;
-    p.waves = kv->head_dim > 128 || of_seq < LNSHIP_CHUNK_ROWS ? 0 : of_seq < LNSHIP_CHUNK_ROWS8 ? 4 : 8;
+    const int64_t n_head = rep * kv->n_head_kv, tile_bytes = kv->n_head_kv * 64 * ((kv->head_dim + 31) & ~(int64_t)31) * 8;
+    const bool chunks = kv->head_dim <= 128 && of_seq >= LNSHIP_CHUNK_ROWS;
+    p.pre_tiles = (kv->table_ld * kv->page + 63) / 64;
+    p.pre = chunks && LNSHIP_PRE && kv->n_seq * p.pre_tiles <= k_pre_bytes / tile_bytes;
+    p.pre_bytes = p.pre ? kv->n_seq * p.pre_tiles * tile_bytes : 0;
+    p.ok_bytes = p.pre ? (kv->n_seq * p.pre_tiles * 8 + 255) & ~(int64_t)255 : 0;
+    p.waves = !chunks ? 0 : p.pre || of_seq < LNSHIP_CHUNK_ROWS8 ? 4 : 8;
     p.tile_rows = p.waves ? p.waves * 32 : 16;
     p.tiles = rows / p.tile_rows + kv->n_seq;
     const int64_t wgs = std::max<int64_t>(1, p.tiles * kv->n_head_kv);
@@ -1104,29 +1159,27 @@ static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
     const int64_t most = (kv->table_ld * kv->page / 64 + p.min_per - 1) / p.min_per;
     const int64_t want = p.waves ? LNSHIP_TGT2 : LNSHIP_TGT;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want * cus + wgs - 1) / wgs, most, 256}));
-    const int64_t n_head = rep * kv->n_head_kv, hdp = (kv->head_dim + 31) & ~(int64_t)31;
     p.parts_bytes = p.splits > 1 ? (kv->ntok * n_head * (p.splits * (kv->head_dim + 2) + 1) * 4 + 255) & ~(int64_t)255 : 0;
-    p.pre_tiles = (kv->table_ld * kv->page + 63) / 64;
-    const int64_t tile_bytes = kv->n_head_kv * 64 * hdp * 8;
-    p.pre = p.waves > 0 && kv->n_seq * p.pre_tiles <= k_pre_bytes / tile_bytes && LNSHIP_PRE;
-    p.pre_bytes = p.pre ? kv->n_seq * p.pre_tiles * tile_bytes : 0;
-    p.ok_bytes = p.pre ? (kv->n_seq * p.pre_tiles * 8 + 255) & ~(int64_t)255 : 0;
     return p;
 }
 
-template <int NB, int NW, bool PRE>
-static int launch_chunk(const attn_paged_args &m, const attn_plan &p, hipStream_t s, unsigned long long *err) {
-    const int lds = 2 * 4 * tile_of<NB>::U * 16;
-    static std::atomic<uint64_t> done{0};   // devices that know the kernel's LDS
+// a kernel's LDS limit, set once on a device (done: the devices that know it)
+static int allow_lds(const void *kernel, int lds, std::atomic<uint64_t> &done) {
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
     if (!(done.load() >> dev & 1)) {
-        LNSHIP_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_chunk<NB, NW, PRE>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        LNSHIP_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         done.fetch_or((uint64_t)1 << dev);
     }
-    hipLaunchKernelGGL((k_attn_chunk<NB, NW, PRE>), dim3((unsigned)(p.tiles * m.kv.n_head_kv), (unsigned)p.splits),
-                       dim3(NW * 64), lds, s, m, err);
+    return 0;
+}
+
+template <int NB, int NW>
+static int launch_chunk(const attn_paged_args &m, const dim3 &grid, hipStream_t s, unsigned long long *err) {
+    constexpr int lds = 2 * 4 * tile_of<NB>::U * 16;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = allow_lds(reinterpret_cast<const void *>(k_attn_chunk<NB, NW>), lds, done)) return rc;
+    hipLaunchKernelGGL((k_attn_chunk<NB, NW>), grid, dim3(NW * 64), lds, s, m, err);
     LNSHIP_HIP(hipGetLastError());
     return 0;
 }
@@ -1134,16 +1187,19 @@ static int launch_chunk(const attn_paged_args &m, const attn_plan &p, hipStream_
 template <int NB>
 static int launch_attn(const attn_paged_args &m, const attn_plan &p, int cus, hipStream_t s, unsigned long long *err) {
     if constexpr (NB <= 4) {
+        const dim3 chunks((unsigned)(p.tiles * m.kv.n_head_kv), (unsigned)p.splits);
         if (p.pre) {
             // (a grid's y and z are counted in 16 bits)
             const int64_t y = std::min<int64_t>(m.kv.n_seq, 65535 / m.kv.n_head_kv) * m.kv.n_head_kv;
             const int64_t x = std::max<int64_t>(1, std::min<int64_t>(p.pre_tiles, 8 * cus / y));
             hipLaunchKernelGGL(k_attn_decode<NB>, dim3((unsigned)x, (unsigned)y), dim3(256), 0, s, m, err);
             LNSHIP_HIP(hipGetLastError());
-            return p.waves == 4 ? launch_chunk<NB, 4, true>(m, p, s, err) : launch_chunk<NB, 8, true>(m, p, s, err);
+            hipLaunchKernelGGL(k_attn_tiles<NB>, chunks, dim3(256), 0, s, m, err);
+            LNSHIP_HIP(hipGetLastError());
+            return 0;
         }
-        if (p.waves == 4) return launch_chunk<NB, 4, false>(m, p, s, err);
-        if (p.waves == 8) return launch_chunk<NB, 8, false>(m, p, s, err);
+        if (p.waves == 4) return launch_chunk<NB, 4>(m, chunks, s, err);
+        if (p.waves == 8) return launch_chunk<NB, 8>(m, chunks, s, err);
     }
     const dim3 grid((unsigned)p.tiles, (unsigned)m.kv.n_head_kv, (unsigned)p.splits);
     if (m.kv.head_dim == NB * 32) hipLaunchKernelGGL((k_attn_paged<NB, true>), grid, dim3(256), 0, s, m, err);
