@@ -238,7 +238,15 @@ def attn_case(rng, q_len, kv_len, page, nh, nkv, hd, qscale=2.0, kstd=1.0, vstd=
     return q, c, table, keys, vals
 
 
-def run_attn(ln, q, c, table, q_len, kv_len, window=0, scale=None, out=None):
+def widen(table, page, cells):
+    """The same pages in a table of so many cells: what a call costs at most, and by it which kernel runs."""
+    wide = np.full((table.shape[0], max(cells // page, table.shape[1])), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
+def run_attn(ln, q, c, table, q_len, kv_len, window=0, scale=None, out=None, cells=0):
+    table = widen(table, c.page, cells)
     return ln.paged.attention(dev(q), dev(c.k), dev(c.v), c.page, dev(table), dev(starts(q_len)), dev(np.int32(kv_len)),
                               scale if scale is not None else q.shape[2] ** -0.5, window=window, out=out)
 
@@ -281,18 +289,35 @@ def test_chunks_behind_a_table_of_many_pages(ln, q_len, kv_len, page, nh, nkv, h
     check_attn(narrow, q, q_len, kv_len, keys, vals, window)
 
 
+@pytest.mark.parametrize("q_len,kv_len,page,nh,nkv,hd,window", [
+    # 64 to 511 rows a sequence: each workgroup decodes; more: decoded before
+    ([300], [300], 16, 9, 3, 64, 0), ([70, 5], [70, 333], 32, 5, 1, 96, 0), ([131], [260], 16, 16, 1, 128, 0),
+    ([40, 90], [300, 90], 16, 4, 4, 24, 50), ([520, 1, 90], [800, 50, 90], 32, 8, 2, 64, 0), ([65], [65], 256, 2, 2, 8, 0),
+    ([600], [900], 16, 1, 1, 32, 0), ([130, 3], [170, 9], 64, 18, 2, 128, 0), ([257], [300], 16, 28, 4, 80, 0),
+    ([300, 1, 0, 180], [310, 5, 7, 900], 128, 32, 4, 96, 0), ([520], [530], 64, 8, 2, 128, 129), ([333], [999], 32, 3, 1, 64, 31),
+    ([1030], [1050], 16, 4, 2, 72, 0), ([519], [700], 32, 8, 2, 104, 0), ([2050], [2050], 64, 2, 2, 128, 700)])
+def test_chunks_behind_wide_tables(ln, q_len, kv_len, page, nh, nkv, hd, window):
+    print(f"\n[attn] {q_len} {kv_len} page {page} {nh}/{nkv}x{hd} window {window}, wide", flush=True)
+    rng = np.random.default_rng(nh * 1000 + hd)
+    q, c, table, keys, vals = attn_case(rng, q_len, kv_len, page, nh, nkv, hd)
+    cells = (1 << 28) // (sum(q_len) * nh * hd) + 2 * page
+    got = run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells).cpu().numpy()
+    check_attn(got, q, q_len, kv_len, keys, vals, window)
+    assert np.array_equal(got, run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells).cpu().numpy())
+
+
 @pytest.mark.parametrize("qscale,kstd,vstd", [(1e-6, 1.0, 1.0), (30.0, 1.0, 1.0), (1.0, 1e-3, 1e-3),
                                               (1e4, 1e-4, 500.0), (1.0, 20.0, 8000.0), (1e-30, 1.0, 1e-2)])
-@pytest.mark.parametrize("q_len,kv_len", [([1], [200]), ([100], [180])])
-def test_attention_of_small_and_large_values(ln, qscale, kstd, vstd, q_len, kv_len):
+@pytest.mark.parametrize("q_len,kv_len,cells", [([1], [200], 0), ([100], [180], 0), ([100], [180], 1 << 14), ([130], [180], 1 << 14)])
+def test_attention_of_small_and_large_values(ln, qscale, kstd, vstd, q_len, kv_len, cells):
     rng = np.random.default_rng(11)
     q, c, table, keys, vals = attn_case(rng, q_len, kv_len, 32, 8, 2, 64, qscale, kstd, vstd)
-    got = run_attn(ln, q, c, table, q_len, kv_len).cpu().numpy()
+    got = run_attn(ln, q, c, table, q_len, kv_len, cells=cells).cpu().numpy()
     check_attn(got, q, q_len, kv_len, keys, vals)
 
 
-@pytest.mark.parametrize("q_len", [[1], [90]])
-def test_attention_is_exact_where_one_cell_counts(ln, q_len):
+@pytest.mark.parametrize("q_len,cells", [([1], 0), ([90], 0), ([90], 1 << 14), ([260], 1 << 14)])
+def test_attention_is_exact_where_one_cell_counts(ln, q_len, cells):
     """Zero queries weigh all cells alike; equal values come out as they are, to 22 bits; and every
     code of the half range, as the value of the only cell, comes out as its real number."""
     page, nkv, hd = 16, 2, 64
@@ -301,11 +326,11 @@ def test_attention_is_exact_where_one_cell_counts(ln, q_len):
     for i in range(0, len(codes), nkv * hd):
         v = np.resize(codes[i:i + nkv * hd], (1, nkv, hd))
         n = q_len[0]
-        c = R.Cache(8, page, nkv, hd, fill=0)
-        row = np.arange(6)
+        c = R.Cache(20, page, nkv, hd, fill=0)
+        row = np.arange(18)
         c.put(row, np.arange(n), np.zeros((n, nkv, hd), np.uint16), np.repeat(v, n, 0))
         q = np.zeros((n, 4, hd), np.float32)
-        got = run_attn(ln, q, c, row[None].astype(np.int32), q_len, q_len).cpu().numpy()
+        got = run_attn(ln, q, c, row[None].astype(np.int32), q_len, q_len, cells=cells).cpu().numpy()
         want = np.repeat(R.value(v), 2, 1)
         # values: 2^-22 as halves, 2^-23 of the power; below the normal halves 2^-36; the mean of n
         # equal terms: n 2^-23
@@ -313,23 +338,24 @@ def test_attention_is_exact_where_one_cell_counts(ln, q_len):
         assert (np.abs(got - want) <= tol).all()
 
 
-@pytest.mark.parametrize("q_len,kv_len", [([4, 3], [2, 3]), ([40, 1], [10, 0]), ([5, 90], [-3, 30])])
-def test_rows_without_cells_are_zero(ln, q_len, kv_len):
+@pytest.mark.parametrize("q_len,kv_len,cells", [([4, 3], [2, 3], 0), ([40, 1], [10, 0], 0), ([5, 90], [-3, 30], 0),
+                                                ([5, 90], [-3, 30], 1 << 14), ([5, 380], [-3, 300], 1 << 13)])
+def test_rows_without_cells_are_zero(ln, q_len, kv_len, cells):
     rng = np.random.default_rng(12)
     q, c, table, keys, vals = attn_case(rng, q_len, kv_len, 16, 6, 2, 64)
-    got = run_attn(ln, q, c, table, q_len, kv_len).cpu().numpy()
+    got = run_attn(ln, q, c, table, q_len, kv_len, cells=cells).cpu().numpy()
     pos = np.concatenate(positions(q_len, kv_len))
     assert (got[pos < 0] == 0).all() and np.isfinite(got).all()
     check_attn(got, q, q_len, kv_len, keys, vals)
 
 
-@pytest.mark.parametrize("q_len,kv_len", [([1], [900]), ([77], [300])])
-def test_bad_pages_hide_their_cells(ln, q_len, kv_len):
+@pytest.mark.parametrize("q_len,kv_len,cells", [([1], [900], 0), ([77], [300], 0), ([77], [300], 1 << 14), ([140], [300], 1 << 14)])
+def test_bad_pages_hide_their_cells(ln, q_len, kv_len, cells):
     rng = np.random.default_rng(13)
     q, c, table, keys, vals = attn_case(rng, q_len, kv_len, 16, 8, 2, 64)
     index_error(ln)
     table[0, 3], table[0, 5] = -7, c.n_pages
-    got = run_attn(ln, q, c, table, q_len, kv_len).cpu().numpy()
+    got = run_attn(ln, q, c, table, q_len, kv_len, cells=cells).cpu().numpy()
     assert index_error(ln)[0] == 1 and index_error(ln)[0] == 0
     check_attn(got, q, q_len, kv_len, keys, vals, hidden=set(range(48, 64)) | set(range(80, 96)))
 
@@ -343,11 +369,12 @@ def test_cells_past_the_table_are_hidden(ln):
     check_attn(got, q, [2], [64], [keys[0]], [vals[0]], hidden=set(range(48, 64)))
 
 
-@pytest.mark.parametrize("q_len,kv_len", [([1, 2], [700, 40]), ([80, 90], [300, 90])])
-def test_rows_of_no_sequence_strides_and_in_place(ln, q_len, kv_len):
+@pytest.mark.parametrize("q_len,kv_len,cells", [([1, 2], [700, 40], 0), ([80, 90], [300, 90], 0), ([80, 90], [300, 90], 1 << 14),
+                                                ([280, 90], [300, 90], 1 << 14)])
+def test_rows_of_no_sequence_strides_and_in_place(ln, q_len, kv_len, cells):
     rng = np.random.default_rng(15)
     q, c, table, keys, vals = attn_case(rng, q_len, kv_len, 16, 6, 2, 64, width=60)
-    T, first = sum(q_len), 3
+    T, first, table = sum(q_len), 3, widen(table, 16, cells)
     buf = torch.full((T + 8, 6 * 64 + 5), 9.0, device="cuda")
     view = torch.as_strided(buf, (T + 8, 6, 64), (6 * 64 + 5, 64, 1), 2)
     view[first:first + T] = dev(q)
@@ -364,16 +391,16 @@ def test_rows_of_no_sequence_strides_and_in_place(ln, q_len, kv_len):
     assert (rest == 9).all()
 
 
-@pytest.mark.parametrize("q_len,kv_len", [([1], [500]), ([70], [140])])
-def test_infinities_and_nan(ln, q_len, kv_len):
+@pytest.mark.parametrize("q_len,kv_len,cells", [([1], [500], 0), ([70], [140], 0), ([70], [140], 1 << 15), ([270], [340], 1 << 14)])
+def test_infinities_and_nan(ln, q_len, kv_len, cells):
     """A NaN or infinite query gives its own row alone no numbers."""
     rng = np.random.default_rng(16)
     q, c, table, keys, vals = attn_case(rng, q_len, kv_len, 16, 4, 2, 64)
-    want = run_attn(ln, q, c, table, q_len, kv_len).cpu().numpy()
+    want = run_attn(ln, q, c, table, q_len, kv_len, cells=cells).cpu().numpy()
     q2 = q.copy()
     q2[0, 1, 5] = np.nan
     q2[0, 2, 7] = np.inf
-    got = run_attn(ln, q2, c, table, q_len, kv_len).cpu().numpy()
+    got = run_attn(ln, q2, c, table, q_len, kv_len, cells=cells).cpu().numpy()
     assert np.isnan(got[0, 1]).all() and np.isnan(got[0, 2]).all()
     keep = np.ones(got.shape[:2], bool)
     keep[0, 1] = keep[0, 2] = False

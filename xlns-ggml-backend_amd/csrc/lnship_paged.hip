@@ -447,13 +447,7 @@ __device__ __forceinline__ void load_q(const float *q, int d, int hd, bool vec, 
 // 16-byte loads, straight from memory.  The next block's keys are loaded while
 // this one's weights are formed, its values once this one's are decoded.
 template <int NB, bool FULL>   // 32-wide groups of head_dim; whether it fills them
-#ifndef LNSHIP_CW
-#define LNSHIP_CW 3
-#endif
-#ifndef LNSHIP_W
-#define LNSHIP_W 3
-#endif
-__global__ __launch_bounds__(256, NB < 4 ? 3 : NB == 4 ? LNSHIP_W : 1) void k_attn_paged(attn_paged_args a, unsigned long long *err) {
+__global__ __launch_bounds__(256, NB <= 4 ? 3 : 1) void k_attn_paged(attn_paged_args a, unsigned long long *err) {
     const lnship_paged_kv &kv = a.kv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int rep = a.rep, kvh = blockIdx.y, split = blockIdx.z, hd = (int)kv.head_dim, page = (int)kv.page;
@@ -933,10 +927,10 @@ __device__ __forceinline__ int chunk_tile(int nkv, int &kvh) {
 // Small workgroups, two or more on a CU: a barrier holds only waves of other
 // SIMDs together, so that on each SIMD one workgroup's wave multiplies while
 // another's forms weights.
-template <int NB>
-__global__ __launch_bounds__(256, NB <= 2 ? LNSHIP_CW : 2) void k_attn_tiles(attn_paged_args a, unsigned long long *err) {
-    constexpr int B = tile_of<NB>::B;
-    static_assert(4 * B % 256 == 0, "whole copies");
+template <int NB, int NW>
+__global__ __launch_bounds__(NW * 64, NB <= 2 ? 3 : 2) void k_attn_tiles(attn_paged_args a, unsigned long long *err) {
+    constexpr int B = tile_of<NB>::B, NT = NW * 64;
+    static_assert(4 * B % NT == 0, "whole copies");
     __shared__ uint4 s_tile[2][4 * B];
     const int tid = threadIdx.x, wave = tid >> 6, nkv = (int)a.kv.n_head_kv, split = blockIdx.y;
     int kvh;
@@ -950,7 +944,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? LNSHIP_CW : 2) void k_attn_tiles(att
     auto copy = [&](int b0, int buf) {
         const uint4 *f = from + (int64_t)(b0 >> 6) * nkv * 8 * B + (b0 >> 5 & 1) * 4 * B;
 #pragma unroll
-        for (int i = 0; i < 4 * B / 256; i++) copy_to_lds(f + i * 256, &s_tile[buf][i * 256 + wave * 64]);
+        for (int i = 0; i < 4 * B / NT; i++) copy_to_lds(f + i * NT, &s_tile[buf][i * NT + wave * 64]);
         ok_next = oks[b0 >> 5];
     };
     if (cbeg < cend) copy(cbeg, 0);
@@ -1120,44 +1114,51 @@ struct attn_plan {
     // the workspace: bytes of the splits' parts, of the decoded tiles, of their flags
     int64_t parts_bytes, pre_bytes, ok_bytes, pre_tiles;
 };
-#ifndef LNSHIP_TGT
-#define LNSHIP_TGT 8
-#endif
-#ifndef LNSHIP_TGT2
-#define LNSHIP_TGT2 1
-#endif
-#ifndef LNSHIP_MINP
-#define LNSHIP_MINP 8
-#endif
-#ifndef LNSHIP_MINP2
-#define LNSHIP_MINP2 8
-#endif
-#ifndef LNSHIP_CHUNK_ROWS
-#define LNSHIP_CHUNK_ROWS 64
-#endif
-#ifndef LNSHIP_CHUNK_ROWS8
-#define LNSHIP_CHUNK_ROWS8 384
-#endif
-#ifndef LNSHIP_PRE
-#define LNSHIP_PRE 1
-#endif
+// Few rows a sequence, or little work: k_attn_paged, whose tiles are 16 rows and
+// whose loads go straight to registers.  Otherwise the chunks' kernels, which
+// read a cell once for 128 or 256 rows but take longer to start.  Measured with
+// 16-row tiles and chunks (us): 8 sequences of 8 tokens over 500 cells, 32 heads
+// of 128 on 8: 21.8 and 30; of 32 tokens (2^29 below): 46.5 and 34.5; 32 of 16 over
+// 1000: 123 and 92; 9 heads of 64 on 3, 8 of 64 over 500: 19.4 and 24.0, over 2000
+// (2^29): 44.9 and 34.6; below 64 rows 32 of 8 over 1000: 78.8 and 82.6.
+constexpr int k_chunk_rows = 64;                // rows of a sequence on average, at least
+constexpr double k_chunk_work = 268435456.0;    // rows x kv heads x cells of the tables x head_dim, at least
+// From two tiles of a sequence on the cells are decoded once for all tiles,
+// while they fit the workspace.  Measured decoded before and in each workgroup
+// (us): 8 sequences of 512 tokens over 2000 cells 98 and 125 (64 dims), 369 and 376
+// (128); of 64 tokens 37 and 35, 113 and 122; of 32 over 500 25 and 23, 43 and 35.
+constexpr int k_decode_rows = 512;
 constexpr int64_t k_pre_bytes = (int64_t)1 << 30;   // of the workspace for decoded cells, at most
+// Waves of a workgroup.  Up to 64 dims four: three or four workgroups share a CU,
+// and uneven sequences leave smaller last tiles (a batch of 9 conversations of
+// 20 to 160 tokens 37 us, with eight waves 45).  Above, eight, which copy or decode a
+// cell once for 256 rows (one sequence of 4096 tokens, 32 heads of 128: 1043 us, with four
+// 1141) but where decoded cells meet less than 2048 rows a sequence (8 sequences of
+// 128 tokens over 2000 cells: 178, with four 157).
+constexpr int k_wide_rows = 2048;
+// Parts of a row's cells: as many workgroups as a CU runs at a time, a part at
+// least so many blocks of 64 cells (single tokens: 64 sequences of up to 8192 cells
+// 302 us with 16 a CU, 340 with 4; conversations 37 us with parts of 4 blocks, 40 with 8
+// and 55 with 2, of which the join reads more).
+constexpr int k_few_wgs = 16, k_few_part = 8, k_many_wgs = 2, k_many_part = 4;
 static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
     attn_plan p;
     const int64_t rows = kv->ntok * rep, of_seq = kv->n_seq ? rows / kv->n_seq : 0;
     const int64_t n_head = rep * kv->n_head_kv, tile_bytes = kv->n_head_kv * 64 * ((kv->head_dim + 31) & ~(int64_t)31) * 8;
-    const bool chunks = kv->head_dim <= 128 && of_seq >= LNSHIP_CHUNK_ROWS;
-    p.pre_tiles = (kv->table_ld * kv->page + 63) / 64;
-    p.pre = chunks && LNSHIP_PRE && kv->n_seq * p.pre_tiles <= k_pre_bytes / tile_bytes;
+    const int64_t cells = kv->table_ld * kv->page;
+    const double work = (double)(rows * kv->n_head_kv) * (double)(cells * kv->head_dim);
+    const bool chunks = kv->head_dim <= 128 && of_seq >= k_chunk_rows && work >= k_chunk_work;
+    p.pre_tiles = (cells + 63) / 64;
+    p.pre = chunks && of_seq >= k_decode_rows && kv->n_seq * p.pre_tiles <= k_pre_bytes / tile_bytes;
     p.pre_bytes = p.pre ? kv->n_seq * p.pre_tiles * tile_bytes : 0;
     p.ok_bytes = p.pre ? (kv->n_seq * p.pre_tiles * 8 + 255) & ~(int64_t)255 : 0;
-    p.waves = !chunks ? 0 : p.pre || of_seq < LNSHIP_CHUNK_ROWS8 ? 4 : 8;
+    p.waves = !chunks ? 0 : kv->head_dim <= 64 || (p.pre && of_seq < k_wide_rows) ? 4 : 8;
     p.tile_rows = p.waves ? p.waves * 32 : 16;
     p.tiles = rows / p.tile_rows + kv->n_seq;
     const int64_t wgs = std::max<int64_t>(1, p.tiles * kv->n_head_kv);
-    p.min_per = p.waves ? LNSHIP_MINP2 : LNSHIP_MINP;
-    const int64_t most = (kv->table_ld * kv->page / 64 + p.min_per - 1) / p.min_per;
-    const int64_t want = p.waves ? LNSHIP_TGT2 : LNSHIP_TGT;
+    p.min_per = p.waves ? k_many_part : k_few_part;
+    const int64_t most = (cells / 64 + p.min_per - 1) / p.min_per;
+    const int64_t want = p.waves ? k_many_wgs : k_few_wgs;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want * cus + wgs - 1) / wgs, most, 256}));
     p.parts_bytes = p.splits > 1 ? (kv->ntok * n_head * (p.splits * (kv->head_dim + 2) + 1) * 4 + 255) & ~(int64_t)255 : 0;
     return p;
@@ -1194,12 +1195,13 @@ static int launch_attn(const attn_paged_args &m, const attn_plan &p, int cus, hi
             const int64_t x = std::max<int64_t>(1, std::min<int64_t>(p.pre_tiles, 8 * cus / y));
             hipLaunchKernelGGL(k_attn_decode<NB>, dim3((unsigned)x, (unsigned)y), dim3(256), 0, s, m, err);
             LNSHIP_HIP(hipGetLastError());
-            hipLaunchKernelGGL(k_attn_tiles<NB>, chunks, dim3(256), 0, s, m, err);
+            constexpr int most = NB <= 2 ? 4 : 8;
+            if (p.waves == 4) hipLaunchKernelGGL((k_attn_tiles<NB, 4>), chunks, dim3(256), 0, s, m, err);
+            else hipLaunchKernelGGL((k_attn_tiles<NB, most>), chunks, dim3(most * 64), 0, s, m, err);
             LNSHIP_HIP(hipGetLastError());
             return 0;
         }
-        if (p.waves == 4) return launch_chunk<NB, 4>(m, chunks, s, err);
-        if (p.waves == 8) return launch_chunk<NB, 8>(m, chunks, s, err);
+        if (p.waves) return launch_chunk<NB, NB <= 2 ? 4 : 8>(m, chunks, s, err);
     }
     const dim3 grid((unsigned)p.tiles, (unsigned)m.kv.n_head_kv, (unsigned)p.splits);
     if (m.kv.head_dim == NB * 32) hipLaunchKernelGGL((k_attn_paged<NB, true>), grid, dim3(256), 0, s, m, err);
