@@ -77,6 +77,32 @@ def test_ties_at_every_border(ln, vocab):
     check(run(ln, x, u, T, k, p, m), x, u, T, k, p, m)
 
 
+@pytest.mark.parametrize("vocab", [5001, 131075])
+@pytest.mark.parametrize("kind", ["smooth", "16 bits", "flat", "tail", "two levels"])
+def test_top_p_alone(ln, vocab, kind):
+    """Borders anywhere in the sum: among crowded tokens, between far levels, in the tail."""
+    rng = np.random.default_rng(vocab)
+    rows = 24
+    x = rng.standard_normal((rows, vocab))
+    x = {"smooth": x * 2.5, "16 bits": x * 8, "flat": x * 0.01, "tail": -4 * np.log(np.abs(x) + 1e-3),
+         "two levels": np.where(x > 2, 6.0, 0.0) + x * 1e-4}[kind].astype(np.float32)
+    if kind == "16 bits":
+        x = (x.view(np.uint32) & np.uint32(0xffff0000)).view(np.float32)
+    p = np.concatenate([[1e-7, 0.01, 0.9999, 0.99999, 0.9999999], rng.random(rows - 5)])
+    m = np.where(np.arange(rows) % 3 == 0, 0.02, 0.0)
+    u = rng.random(rows)
+    u[::4] = 0.9999999
+    check(run(ln, x, u, None, None, p, m), x, u, None, None, p, m)
+
+
+def test_top_k_of_more_than_weigh_anything(ln):
+    """Fewer tokens within reach of the largest than top_k: top_p still cuts them."""
+    x = np.full((6, 3000), -1e4, np.float32)
+    x[:, 70:75] = [3.0, 2.0, 2.5, 1.0, 0.0]
+    u, k, p = np.array([0.1, 0.5, 0.7, 0.9, 0.99, 0.999]), np.full(6, 50), np.array([0.5, 0.7, 0.8, 0.9, 0.3, 0.97])
+    check(run(ln, x, u, None, k, p), x, u, None, k, p, None)
+
+
 @pytest.mark.parametrize("vocab", [33, 50000])
 def test_limits_at_their_ends(ln, vocab):
     rng = np.random.default_rng(1)

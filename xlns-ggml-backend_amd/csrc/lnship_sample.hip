@@ -10,9 +10,6 @@
 
 namespace lnship {
 
-#ifndef LNSHIP_RES
-#define LNSHIP_RES 3
-#endif
 constexpr int k_draw_block = 1024;
 constexpr int k_draw_waves = k_draw_block / 64;
 constexpr int k_w_sh = 40;              // weights are integers in units of 2^-40
@@ -20,6 +17,7 @@ constexpr int k_seg = 1024;             // logits of a segment, which a wave goe
 constexpr int k_seg_max = 512;
 constexpr int64_t k_draw_vocab = (int64_t)k_seg * k_seg_max;
 constexpr int k_bins = 4096, k_bins_binade = 64;   // of the distance from the largest logit, 64 a binade of weight
+constexpr int k_head = 22 * k_bins_binade;   // bins above those of 42 binades, for logits above the first ones
 constexpr int k_list = 2048;            // tokens that are put in order at once
 constexpr int k_small_k = 1024;         // a top_k whose tokens are
 
@@ -34,12 +32,23 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 constexpr uint32_t k_key_ninf = 0x007fffffu;   // order_key(-inf)
 
-// The weight e^((x - x_max) / T) in units of 2^-40, rounded.  The exponent is
-// formed in 64 bits (32 would lose what tells two sums apart), its fraction's
-// power in 32: 24 bits of every weight.  Integers come out of the low bits of
-// a sum with a power of two, which costs less than a conversion: 17 issue slots
-// a weight, four of them the power.
-struct weigher {
+// a value that is the same in all lanes, in scalar registers
+template <class V>
+__device__ __forceinline__ V uniform(V v) {
+    union {
+        V v;
+        int w[sizeof(V) / 4];
+    } u;
+    u.v = v;
+    for (size_t i = 0; i < sizeof(V) / 4; i++) u.w[i] = __builtin_amdgcn_readfirstlane(u.w[i]);
+    return u.v;
+}
+
+// The weight e^((x - x_max) / T) in units of 2^-40, rounded, of any x_max and T.
+// The exponent is formed in 64 bits (32 would lose what tells two sums apart),
+// its fraction's power in 32: 24 bits of every weight.  Integers come out of the
+// low bits of a sum with a power of two.
+struct any_weigher {
     double xmax, f;   // f = log2 e / T
     __device__ __forceinline__ uint64_t operator()(float x) const {
         constexpr double whole = 6755399441055744.0;   // 1.5 2^52: a sum's low word is the integer
@@ -53,10 +62,63 @@ struct weigher {
     }
 };
 
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+// The same where |x_max f| <= 2^20, in three operations of 64 bits: of x f + c,
+// c = 1.5 2^20 - x_max f, the high word holds the exponent's whole part and the
+// low word its fraction, to 2^-32.  The power of the fraction is in [1, 2]; its
+// F32 bits become those of the double with the whole part in its exponent.
+struct weigher {
+    double f, c;
+    float lo;   // x where the weight is 2^-63: what lies below weighs nothing either
+    static __device__ __forceinline__ bool fits(float xmax, double f) {
+        return fabs((double)xmax * f) <= 1048576.0 && f >= 1e-30;
+    }
+    __device__ __forceinline__ weigher(float xmax, double f_)
+        : f(f_), c(uniform(1572864.0 - (double)xmax * f_)), lo(uniform((float)fmax((double)xmax - 63.0 / f_, -3.4028234e38))) {}
+    __device__ __forceinline__ uint64_t operator()(float x) const {
+        constexpr double unit = 4096.0;   // a sum's last place is 2^-40
+        const uint64_t t = (uint64_t)__double_as_longlong(fma((double)fmaxf(x, lo), f, c));
+        const uint32_t p = f32_bits(__builtin_amdgcn_exp2f((float)(uint32_t)t * 0x1p-32f));
+        const uint32_t hi = ((uint32_t)(t >> 32) << 20) + (p >> 3) + ((1023u << 20) - (127u << 20));
+        const double w = __longlong_as_double((int64_t)((uint64_t)hi << 32 | p << 29));
+        return (uint64_t)__double_as_longlong(w + unit) - (uint64_t)__double_as_longlong(unit);
+    }
+};
+
+// v of the lane that DPP control C names, in the rows of M; zero where there is none
+template <int C, int M = 0xf>
+__device__ __forceinline__ uint64_t lane_of(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, C, M, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), C, M, 0xf, false);
+    return (uint64_t)hi << 32 | lo;
 }
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+// Inclusive scans over a row's 16 lanes, and the wave's 64: shifts by 1, 2, 4, 8
+// within rows, then the last lanes of rows 0 and 2, then of the lower half, added
+// to what lies behind.  From register to register: through LDS's permutation a
+// step takes as long as five of these.
+template <class F>
+__device__ __forceinline__ uint64_t row_scan(uint64_t v, F f) {
+    v = f(v, lane_of<0x111>(v));
+    v = f(v, lane_of<0x112>(v));
+    v = f(v, lane_of<0x114>(v));
+    return f(v, lane_of<0x118>(v));
+}
+template <class F>
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v, F f) {
+    v = row_scan(v, f);
+    v = f(v, lane_of<0x142, 0xa>(v));
+    return f(v, lane_of<0x143, 0xc>(v));
+}
+struct add_u64 {
+    __device__ __forceinline__ uint64_t operator()(uint64_t x, uint64_t y) const { return x + y; }
+};
+struct max_u64 {
+    __device__ __forceinline__ uint64_t operator()(uint64_t x, uint64_t y) const { return max(x, y); }
+};
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return read_lane(wave_scan(v, add_u64()), 63); }
 
 struct draw_args {
     const float *logits;
@@ -71,11 +133,15 @@ struct draw_args {
 
 struct draw_row {   // what a row asks for
     float xmax;
-    weigher W;
+    double f;       // log2 e / T
     int top_k;      // 0: no limit
-    float top_p;
-    double wmin;    // least weight that min_p keeps, in units
+    float top_p, min_p;
 };
+
+// the least weight that min_p keeps
+__device__ __forceinline__ uint64_t least_weight(float min_p, uint64_t largest) {
+    return min_p > 0.0f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * (double)largest) : 0;
+}
 
 // the unit of the total that u names
 __device__ __forceinline__ uint64_t draw_target(float u, uint64_t total) {
@@ -86,21 +152,13 @@ __device__ __forceinline__ uint64_t draw_target(float u, uint64_t total) {
 // inclusive sums over the workgroup's threads; the same memory may be used
 // again after the next barrier
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *s, uint64_t &all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    v = wave_scan(v, add_u64());
     if (lane == 63) s[wave] = v;
     __syncthreads();
-    uint64_t t = lane < k_draw_waves ? s[lane] : 0;
-    for (int d = 1; d < k_draw_waves; d <<= 1) {
-        const uint64_t o = __shfl_up(t, d);
-        if (lane >= d) t += o;
-    }
-    all = __shfl(t, k_draw_waves - 1);
-    const uint64_t before = __shfl(t, max(wave - 1, 0));
-    return wave ? v + before : v;
+    const uint64_t t = row_scan(s[lane & (k_draw_waves - 1)], add_u64());
+    all = read_lane(t, k_draw_waves - 1);
+    return wave ? v + read_lane(t, wave - 1) : v;
 }
 
 // The items of list (all different) put in descending order: each item's place
@@ -138,11 +196,12 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n;
     const float *x = a.logits + r * a.ld;
     // (an infinite largest logit, or 1 / T: only its equals weigh anything)
-    const bool sharp = !(fabsf(d0.xmax) < INFINITY) || !(d0.W.f < 1e300);
-    auto W = [&](float v) { return sharp ? (uint64_t)(v == d0.xmax) << k_w_sh : d0.W(v); };
+    const bool sharp = !(fabsf(d0.xmax) < INFINITY) || !(d0.f < 1e300);
+    const any_weigher any{(double)d0.xmax, d0.f};
+    auto W = [&](float v) { return sharp ? (uint64_t)(v == d0.xmax) << k_w_sh : any(v); };
     const int top_k = d0.top_k;
     const float top_p = d0.top_p;
-    const double wmin = d0.wmin;
+    const uint64_t wmin = least_weight(d0.min_p, (uint64_t)1 << k_w_sh);   // (the largest logit weighs 2^40 units)
     __syncthreads();   // (what lay in s_w and s_u64 is read)
     // the border key and how many of its ties are kept
     uint32_t bkey = k_key_ninf + 1, bties = 0xffffffffu;
@@ -258,17 +317,13 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
             }
             if (keep) {
                 w = W(v);
-                if ((double)w < wmin) w = 0;
+                if (w < wmin) w = 0;
             }
             if (!draw) {
                 run += w;
                 continue;
             }
-            uint64_t inc = w;
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint64_t o = __shfl_up(inc, d);
-                if (lane >= d) inc += o;
-            }
+            const uint64_t inc = wave_scan(w, add_u64());
             if (lane == 63) s_u64[wave] = inc;
             __syncthreads();
             uint64_t all = 0, before = run;
@@ -293,28 +348,36 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
 
 // One workgroup a row; a wave goes through segments of 1024 logits.  R segments
 // a wave are held in registers; the rest of a longer row (MORE) is read again
-// for every pass.
-// After its largest logit is known:
-// - without top_k and top_p the weights are summed by segment, the segment that
-//   holds u's share found, and that segment gone through again;
-// - with them one histogram over the distance from the largest logit (of counts
-//   for top_k, of weights for top_p) names the bin of the border; with a top_k
-//   the tokens down to that bin, with top_p alone those of that bin, are
-//   put in order, and the border is exact.
+// for every pass, from L2 or the memory-side cache.
+// - The largest logit; with top_k or top_p also one histogram over the distance
+//   from it, of counts for top_k, of 14-bit weights for top_p, which names the
+//   bins that the border lies in.  In a long row both come from one pass: the
+//   bins are counted from the largest of the first segments, with 22 binades
+//   above it (a row that reaches beyond is counted again).
+// - With a top_k the tokens down to that bin are put in order, which gives
+//   top_p's and min_p's borders too, and the draw.
+// - Otherwise the weights are summed by segment.  With a top_p the tokens of the
+//   border's bins are collected meanwhile and their weights, from the exact sum
+//   above them on, name the border exactly; if it is not among them (or
+//   too many tokens are) the row takes draw_by_digits.
+// - The segment that holds u's share is gone through again.
+// Bound by a row's passes on one CU: one of loads, and one of weights at 98 cycles
+// a wave's 64.  256 rows of 131075: 22 us greedy, 45 with a top_k, 49 with neither
+// and 68 with a top_p (a row's exact histogram of 64-bit weights instead: 106).
 template <int R, bool MORE>
 __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
     typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));   // rows need no alignment
-    __shared__ uint64_t s_hist[k_bins];   // later the lists
-    __shared__ uint64_t s_seg[k_list / 2];   // segments' sums; before, the places of order_items
-    static_assert(k_seg_max <= k_list / 2, "");
-    __shared__ uint64_t s_scan[2][k_draw_waves];
-    __shared__ uint64_t s_x[2];
-    __shared__ int s_n;
-    uint64_t *const s_list = s_hist, *const s_sorted = s_hist + k_list;
+    __shared__ uint64_t s_list[k_list], s_sorted[k_list], s_order[k_list];
+    __shared__ uint32_t s_place[k_list];
+    __shared__ uint64_t s_seg[k_seg_max], s_scan[2][k_draw_waves];
+    __shared__ uint64_t s_x;
+    __shared__ int s_n, s_bin[4];
+    __shared__ uint32_t s_cnt[4];
+    uint32_t *const s_hist = reinterpret_cast<uint32_t *>(s_sorted);   // of counts
+    static_assert(k_bins <= 2 * k_list, "");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n, segs = (n + k_seg - 1) / k_seg;
     const int64_t r = blockIdx.x;
     const float *x = a.logits + r * a.ld;
-    static_assert(2 * k_list <= k_bins, "both lists lie in the histogram's place");
 
     // a segment's sixteen logits of a lane, v[4 q + j] number 256 q + 4 lane + j;
     // NaN, and what lies past the row, as -inf
@@ -344,13 +407,16 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
 #pragma unroll
     for (int i = 0; i < R; i++)
         if (i * k_draw_waves + wave < segs) load(i * k_draw_waves + wave, keep[i]);
+    auto kept = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (i * k_draw_waves + wave < segs) f(i * k_draw_waves + wave, keep[i]);
+    };
     auto each = [&](auto f) {
         float next[16];
         int seg = R * k_draw_waves + wave;
         if (MORE && seg < segs) load(seg, next);
-#pragma unroll
-        for (int i = 0; i < R; i++)
-            if (i * k_draw_waves + wave < segs) f(i * k_draw_waves + wave, keep[i]);
+        kept(f);
         if constexpr (MORE)
             for (; seg < segs; seg += k_draw_waves) {
                 float v[16];
@@ -361,34 +427,92 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
             }
     };
 
+    const float T = uniform(a.temperature ? a.temperature[r] : 1.0f);
+    const bool greedy = !(T > 0.0f);
     draw_row D;
+    D.f = uniform(1.4426950408889634 / (double)T);
+    D.top_k = uniform(a.top_k ? a.top_k[r] : 0);
+    if (D.top_k < 0 || D.top_k >= n) D.top_k = 0;
+    D.top_p = uniform(a.top_p ? a.top_p[r] : 1.0f);
+    if (!(D.top_p < 1.0f)) D.top_p = 1.0f;
+    D.min_p = uniform(a.min_p ? a.min_p[r] : 0.0f);
+
     auto easy = [&]() -> bool {
-        // the largest logit, and the first index that has it
-        const float T = a.temperature ? a.temperature[r] : 1.0f;
-        const bool greedy = !(T > 0.0f);
+        // Bins of a logit's distance from ref, which lies no more than k_head bins
+        // below the largest logit; they never rise with the logit, and the last
+        // holds all whose weight rounds to 0.
+        const bool by_count = D.top_k > 0;
+        const float scale = uniform((float)(k_bins_binade * D.f));
+        const bool bins = !greedy && D.top_k <= k_small_k && (by_count || D.top_p < 1.0f) && scale < INFINITY;
+        float ref = -INFINITY;
+        auto place_of = [&](float v) {
+            return __builtin_amdgcn_fmed3f((ref - v) * scale + (float)k_head, 0.0f, (float)(k_bins - 1));
+        };
+        auto bin_of = [&](float v) { return (int)place_of(v); };
+        // By weight a token counts 2^shift at its bin's start and by the fraction of
+        // its bin that it lies behind it less, as its weight does: a sum fits 32 bits,
+        // and a bin's weight is known to 2^-14 (half a unit of 2^-13, and 2^-16 for
+        // the third power's term).
+        const int shift = by_count ? 0 : min(16, __clz(n));
+        auto count_all = [&](const float *v) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int b = bin_of(v[e]);
+                if (b < k_bins - 1) atomicAdd(&s_hist[b], 1u);
+            }
+        };
+        auto weigh_all = [&](const float *v) {
+            constexpr float step = 0.6931472f / k_bins_binade;
+            const float unit = (float)(1 << shift);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float z = place_of(v[e]);
+                const int b = (int)z;
+                const float behind = z - (float)b;
+                const float q = fmaf(fmaf(behind, 0.5f * step * step, -step) * behind, unit, unit);
+                if (b < k_bins - 1) atomicAdd(&s_hist[b], (uint32_t)(q + 0.5f));
+            }
+        };
+        auto block_max = [&](uint64_t v, uint64_t *s) {
+            v = wave_scan(v, max_u64());
+            if (lane == 63) s[wave] = v;
+            __syncthreads();
+            return read_lane(row_scan(s[lane & (k_draw_waves - 1)], max_u64()), k_draw_waves - 1);
+        };
+
+        // the largest logit, the first index that has it for greedy, and the bins
         float mx = -INFINITY;
         int at = 0x7fffffff;
-        if (!greedy) {
+        if (greedy) {
+            each([&](int seg, const float *v) {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (v[e] > mx) {
+                        mx = v[e];
+                        at = index(seg, e);
+                    }
+            });
+        } else if (bins && MORE) {
+            // the bins in the same pass, from the largest of the segments in registers
+            for (int i = tid; i < k_bins; i += k_draw_block) s_hist[i] = 0;
+            kept([&](int, const float *v) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) mx = fmaxf(mx, v[e]);
+            });
+            ref = key_value((uint32_t)block_max(order_key(mx), s_scan[1]));
+            each([&](int, const float *v) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) mx = fmaxf(mx, v[e]);
+                if (by_count) count_all(v);
+                else weigh_all(v);
+            });
+        } else {
             each([&](int, const float *v) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) mx = fmaxf(mx, v[e]);
             });
-        } else {
-            each([&](int seg, const float *v) {
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                        if (v[e] > mx) {
-                            mx = v[e];
-                            at = index(seg, e);
-                        }
-            });
         }
-        uint64_t best = (uint64_t)order_key(mx) << 32 | (uint32_t)(0x7fffffff - at);
-        for (int d = 32; d; d >>= 1) best = max(best, (uint64_t)__shfl_xor(best, d));
-        if (lane == 0) s_scan[0][wave] = best;
-        __syncthreads();
-        best = s_scan[0][lane & (k_draw_waves - 1)];
-        for (int d = k_draw_waves / 2; d; d >>= 1) best = max(best, (uint64_t)__shfl_xor(best, d));
+        const uint64_t best = block_max((uint64_t)order_key(mx) << 32 | (uint32_t)(0x7fffffff - at), s_scan[0]);
         const uint32_t kmax = (uint32_t)(best >> 32);
         if (kmax <= k_key_ninf || greedy) {
             if (tid == 0) {
@@ -398,175 +522,237 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
             return true;
         }
         D.xmax = key_value(kmax);
-        D.W = {(double)D.xmax, 1.4426950408889634 / (double)T};
-        D.top_k = a.top_k ? a.top_k[r] : 0;
-        if (D.top_k < 0 || D.top_k >= n) D.top_k = 0;
-        D.top_p = a.top_p ? a.top_p[r] : 1.0f;
-        if (!(D.top_p < 1.0f)) D.top_p = 1.0f;
-        // (the largest logit weighs 2^40 units)
-        const float min_p = a.min_p ? a.min_p[r] : 0.0f;
-        D.wmin = min_p > 0.0f ? fmin((double)min_p, 1.0) * (double)((uint64_t)1 << k_w_sh) : 0.0;
-        const weigher &W = D.W;
-        const bool by_count = D.top_k > 0;
-        const float scale = (float)(k_bins_binade * D.W.f);
-        if (D.top_k > k_small_k || !(fabsf(D.xmax) < INFINITY) || !(scale < INFINITY)) {
+        if (D.top_k > k_small_k || !(fabsf(D.xmax) < INFINITY) || !(scale < INFINITY) || !weigher::fits(D.xmax, D.f))
             return false;
-        }
+        const weigher W(D.xmax, D.f);
+        const uint64_t wmin = uniform(least_weight(D.min_p, W(D.xmax)));
 
         // a token is kept if (key, index) does not come behind (bkey, bidx)
         uint32_t bkey = 0;
-        int bidx = 0x7fffffff, above_bin = k_bins;
-        if (by_count || D.top_p < 1.0f) {
-            // bin of a logit: it never rises with the logit; the last holds all
-            // whose weight rounds to 0
-            auto bin_of = [&](float v) { return (int)fminf((D.xmax - v) * scale, (float)(k_bins - 1)); };
-            for (int i = tid; i < k_bins; i += k_draw_block) s_hist[i] = 0;
+        int bidx = 0x7fffffff;
+        bool bordered = false;
+        if (bins) {
+            if (!MORE || !((D.xmax - ref) * scale <= (float)k_head)) {   // (no bins yet, or not down to the largest)
+                __syncthreads();
+                for (int i = tid; i < k_bins; i += k_draw_block) s_hist[i] = 0;
+                ref = D.xmax;
+                __syncthreads();
+                each([&](int, const float *v) {
+                    if (by_count) count_all(v);
+                    else weigh_all(v);
+                });
+            }
             if (tid == 0) s_n = 0;
             __syncthreads();
-            if (by_count) {
-                each([&](int, const float *v) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                            const int b = bin_of(v[e]);
-                            if (b < k_bins - 1) atomicAdd((unsigned int *)&s_hist[b], 1u);
-                        }
-                });
-            } else {
-                each([&](int, const float *v) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                            const int b = bin_of(v[e]);
-                            if (b < k_bins - 1) atomicAdd((unsigned long long *)&s_hist[b], (unsigned long long)W(v[e]));
-                        }
-                });
-            }
-            __syncthreads();
-            // the first bin up to which the counts (the weights) reach what is kept
-            uint64_t h[4], sum = 0, all;
+            uint32_t h[4];
+            uint64_t sum = 0, counts;
 #pragma unroll
             for (int i = 0; i < 4; i++) sum += h[i] = s_hist[tid * 4 + i];
-            uint64_t run = block_scan(sum, s_scan[1], all) - sum;
-            uint64_t want = (uint64_t)D.top_k;
-            if (!by_count) {
-                const double p = ceil((double)D.top_p * (double)all);
-                want = p >= 1.0 ? min((uint64_t)p, all) : 1;
-            }
-            if (tid == 0) s_x[0] = k_bins - 1;   // (top_k: fewer weigh anything)
+            const uint32_t before_bin = (uint32_t)(block_scan(sum, s_scan[0], counts) - sum);
+            if (tid < 4) s_bin[tid] = k_bins - 2, s_cnt[tid] = (uint32_t)counts;
             __syncthreads();
-            if (run < want && run + sum >= want) {
-                int b = tid * 4;
+            // the first bin up to which v's sum (run: before the thread's) reaches
+            // what is wanted, and the tokens before it (or, through, up to it)
+            auto first_bin = [&](const uint64_t (&v)[4], uint64_t run, uint64_t want, int slot, bool through) {
+                uint64_t next = run + v[0] + v[1] + v[2] + v[3];
+                if (run >= want || next < want) return;
+                uint32_t c = before_bin, at_b = 0;
+                int b = 0;
 #pragma unroll
                 for (int i = 0; i < 3; i++)
-                    if (run + h[i] < want) run += h[i], b++;
-                    else break;
-                s_x[0] = (uint64_t)b;
-                s_x[1] = run;
+                    if (b == i && run + v[i] < want) run += v[i], c += h[i], b++;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (b == i) at_b = h[i];
+                s_bin[slot] = tid * 4 + b;
+                s_cnt[slot] = through ? c + at_b : c;
+            };
+            int lo = 0, hi;   // the bins of the list
+            if (by_count) {
+                // (fewer weigh anything: all bins but the last)
+                const uint64_t v[4] = {h[0], h[1], h[2], h[3]};
+                first_bin(v, before_bin, (uint64_t)D.top_k, 0, true);
+                __syncthreads();
+                hi = s_bin[0];
+            } else {
+                // the list: the bins in which the border lies, with 2^-13 of the sum to
+                // either side (the estimate's error twice), or 2^-16 where those are many
+                uint64_t v[4], est = 0, all;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    est += v[i] = (uint64_t)((double)h[i] * (double)__builtin_amdgcn_exp2f(
+                                      (float)(k_w_sh - shift) + (place_of(D.xmax) - (float)(tid * 4 + i)) * (1.0f / k_bins_binade)));
+                const uint64_t run = block_scan(est, s_scan[1], all) - est;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const double p = (double)D.top_p * (double)all, off = i == 0 ? 1.0 / 8192 : 1.0 / 65536;
+                    first_bin(v, run, (uint64_t)fmax(p * (1 - off), 1.0), 2 * i, false);
+                    first_bin(v, run, min((uint64_t)fmax(p * (1 + off), 0.0) + 1, all), 2 * i + 1, true);
+                }
+                __syncthreads();
+                const int of = s_cnt[1] - s_cnt[0] <= (uint32_t)(k_list - 64) << shift ? 0 : 2;
+                lo = s_bin[of], hi = s_bin[of + 1];
             }
-            __syncthreads();   // (the histogram is read; its place is the lists')
-            const int border = (int)s_x[0];
-            if (border < k_bins - 1) {
-                const uint64_t above = s_x[1];
-                const int from = by_count ? 0 : border;   // the bins of the list
+            auto push = [&](float v, int i) {
+                const int at = atomicAdd(&s_n, 1);
+                if (at < k_list) s_list[at] = (uint64_t)order_key(v) << 32 | (uint32_t)(0x7fffffff - i);
+            };
+            uint64_t all = 0, above = 0;
+            asm volatile("" : "+v"(ref));   // bins are formed again, not kept in registers
+            ref = uniform(ref);
+            if (by_count) {
                 each([&](int seg, const float *v) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                            const int b = bin_of(v[e]);
-                            if (b <= border && b >= from) {
-                                const int i = atomicAdd(&s_n, 1);
-                                if (i < k_list)
-                                    s_list[i] = (uint64_t)order_key(v[e]) << 32 |
-                                                (uint32_t)(0x7fffffff - index(seg, e));
-                            }
-                        }
+                    for (int e = 0; e < 16; e++)
+                        if (bin_of(v[e]) <= hi) push(v[e], index(seg, e));
                 });
-                __syncthreads();
-                const int m = s_n;
-                if (m > k_list) {
-                    return false;
-                }
-                uint32_t *const place = (uint32_t *)s_seg;
-                order_items(s_list, s_sorted, place, m);
-                if (by_count) {
-                    // the first top_k, of those top_p's, of those min_p's; then by index
-                    const int k = min(D.top_k, m);
-                    uint64_t w = tid < k ? W(key_value((uint32_t)(s_sorted[tid] >> 32))) : 0, total;
-                    uint64_t c = block_scan(w, s_scan[0], total);
-                    int kept = k;
-                    if (D.top_p < 1.0f) {
-                        const double p = ceil((double)D.top_p * (double)total);
-                        const uint64_t need = p >= 1.0 ? min((uint64_t)p, total) : 1;
-                        if (tid == 0) s_n = 1;
-                        __syncthreads();
-                        if (tid < k && c - w < need && c >= need) s_n = tid + 1;
-                        __syncthreads();
-                        kept = s_n;
+            } else {
+                // the weights of all tokens and of those above the list; by
+                // segment, of those above that min_p keeps
+                each([&](int seg, const float *v) {
+                    uint64_t sum = 0;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const uint64_t w = W(v[e]);
+                        const int b = bin_of(v[e]);
+                        all += w;
+                        if (b < lo) {
+                            above += w;
+                            sum += w >= wmin ? w : 0;
+                        } else if (b <= hi) {
+                            push(v[e], index(seg, e));
+                        }
                     }
-                    const bool in = tid < kept && w > 0 && (double)w >= D.wmin;
-                    if (tid < k_list / 2) s_list[tid] = 0;   // (what is not kept comes last)
-                    __syncthreads();
-                    // order by index: its complement above, its place in the ranking below
-                    if (tid < kept) s_list[tid] = (uint64_t)(uint32_t)s_sorted[tid] << 32 | (in ? (uint32_t)tid + 1u : 0u);
-                    __syncthreads();
-                    uint64_t *const by_index = s_sorted + k_list / 2;   // (top_k <= k_list / 2)
-                    order_items(s_list, by_index, place, kept);
-                    const uint32_t rank = tid < kept ? (uint32_t)by_index[tid] : 0u;
-                    const uint64_t item = rank ? s_sorted[rank - 1] : 0;
-                    w = rank ? W(key_value((uint32_t)(item >> 32))) : 0;
-                    c = block_scan(w, s_scan[1], total);
-                    const uint64_t target = draw_target(a.u[r], total);
-                    if (w && c > target && c - w <= target) {
-                        a.tokens[r] = 0x7fffffff - (int32_t)(uint32_t)item;
-                        if (a.probs) a.probs[r] = (float)((double)w / (double)total);
-                    }
-                    return true;
-                }
-                // top_p: the border bin's first, as many as the weight still needs
-                if (tid == 0) s_n = m;
-                __syncthreads();
-                uint64_t before = above;
-                for (int i0 = 0; i0 < m; i0 += k_draw_block) {
-                    uint64_t part;
-                    const uint64_t w = i0 + tid < m ? W(key_value((uint32_t)(s_sorted[i0 + tid] >> 32))) : 0;
-                    const uint64_t c = before + block_scan(w, s_scan[(i0 / k_draw_block) & 1], part);
-                    if (c - w < want && c >= want) s_n = i0 + tid + 1;
-                    before += part;
-                }
-                __syncthreads();
-                const uint64_t item = s_sorted[s_n - 1];
-                bkey = (uint32_t)(item >> 32);
-                bidx = 0x7fffffff - (int)(uint32_t)item;
-                above_bin = border;
-                __syncthreads();
+                    sum = wave_sum(sum);
+                    if (lane == 0) s_seg[seg] = sum;
+                });
+                all = wave_sum(all), above = wave_sum(above);
+                if (lane == 0) s_scan[0][wave] = all, s_scan[1][wave] = above;
             }
+            __syncthreads();
+            const int m = s_n;
+            if (m > k_list) return false;
+            if (!by_count) {
+                all = above = 0;
+                for (int w = 0; w < k_draw_waves; w++) all += s_scan[0][w], above += s_scan[1][w];
+            }
+            if (by_count) {
+                order_items(s_list, s_sorted, s_place, m);
+                // the first top_k, of those top_p's, of those min_p's; then by index
+                const int k = min(D.top_k, m);
+                uint64_t w = tid < k ? W(key_value((uint32_t)(s_sorted[tid] >> 32))) : 0, total;
+                uint64_t c = block_scan(w, s_scan[0], total);
+                int kept = k;
+                if (D.top_p < 1.0f) {
+                    const double p = ceil((double)D.top_p * (double)total);
+                    const uint64_t need = p >= 1.0 ? min((uint64_t)p, total) : 1;
+                    if (tid == 0) s_n = 1;
+                    __syncthreads();
+                    if (tid < k && c - w < need && c >= need) s_n = tid + 1;
+                    __syncthreads();
+                    kept = s_n;
+                }
+                const bool in = tid < kept && w > 0 && w >= wmin;
+                if (tid < k_list / 2) s_list[tid] = 0;   // (what is not kept comes last)
+                __syncthreads();
+                // order by index: its complement above, its place in the ranking below
+                if (tid < kept) s_list[tid] = (uint64_t)(uint32_t)s_sorted[tid] << 32 | (in ? (uint32_t)tid + 1u : 0u);
+                __syncthreads();
+                uint64_t *const by_index = s_sorted + k_list / 2;   // (top_k <= k_list / 2)
+                order_items(s_list, by_index, s_place, kept);
+                const uint32_t rank = tid < kept ? (uint32_t)by_index[tid] : 0u;
+                const uint64_t item = rank ? s_sorted[rank - 1] : 0;
+                w = rank ? W(key_value((uint32_t)(item >> 32))) : 0;
+                c = block_scan(w, s_scan[1], total);
+                const uint64_t target = draw_target(a.u[r], total);
+                if (w && c > target && c - w <= target) {
+                    a.tokens[r] = 0x7fffffff - (int32_t)(uint32_t)item;
+                    if (a.probs) a.probs[r] = (float)((double)w / (double)total);
+                }
+                return true;
+            }
+            // top_p: the first of the list, as many as the weight still needs.  The
+            // list's weights are summed over finer bins; the tokens of that in which
+            // the border lies are put in order.
+            const double p = ceil((double)D.top_p * (double)all);
+            const uint64_t want = p >= 1.0 ? min((uint64_t)p, all) : 1;
+            auto value = [&](uint64_t item) { return key_value((uint32_t)(item >> 32)); };
+            const float fine = (float)k_draw_block / (float)(hi - lo + 1);
+            auto fine_bin = [&](uint64_t item) {
+                return (int)fminf((place_of(value(item)) - (float)lo) * fine, (float)(k_draw_block - 1));
+            };
+            s_sorted[tid] = 0;
+            if (tid == 0) s_n = -1, s_cnt[0] = 0;
+            __syncthreads();
+            for (int i = tid; i < m; i += k_draw_block)
+                atomicAdd((unsigned long long *)&s_sorted[fine_bin(s_list[i])], (unsigned long long)W(value(s_list[i])));
+            __syncthreads();
+            uint64_t part;
+            const uint64_t wf = s_sorted[tid], cf = above + block_scan(wf, s_scan[0], part);
+            if (cf - wf < want && cf >= want) {
+                s_n = tid;
+                s_x = cf - wf;
+            }
+            __syncthreads();
+            const int at = s_n;
+            if (at < 0) return false;   // (the border is not in the list)
+            uint64_t before = s_x;
+            for (int i = tid; i < m; i += k_draw_block)
+                if (fine_bin(s_list[i]) == at) s_sorted[atomicAdd(&s_cnt[0], 1u)] = s_list[i];
+            __syncthreads();
+            const int few = (int)s_cnt[0];
+            order_items(s_sorted, s_order, s_place, few);
+            for (int i0 = 0; i0 < few; i0 += k_draw_block) {
+                const uint64_t w = i0 + tid < few ? W(value(s_order[i0 + tid])) : 0;
+                const uint64_t c = before + block_scan(w, s_scan[1 - (i0 / k_draw_block & 1)], part);
+                if (c - w < want && c >= want) s_n = i0 + tid;
+                before += part;
+            }
+            __syncthreads();
+            const uint64_t item = s_order[s_n];
+            for (int i = tid; i < m; i += k_draw_block) {
+                const uint64_t w = W(value(s_list[i]));
+                if (s_list[i] >= item && w >= wmin)
+                    atomicAdd((unsigned long long *)&s_seg[(0x7fffffff - (int)(uint32_t)s_list[i]) / k_seg], (unsigned long long)w);
+            }
+            bkey = (uint32_t)(item >> 32);
+            bidx = 0x7fffffff - (int)(uint32_t)item;
+            bordered = true;
+            __syncthreads();
         }
         auto weigh = [&](float v, int i) {
             uint64_t w = W(v);
-            if ((double)w < D.wmin) w = 0;
-            if (above_bin < k_bins) {
+            if (w < wmin) w = 0;
+            if (bordered) {
                 const uint32_t k = order_key(v);
                 if (k < bkey || (k == bkey && i > bidx)) w = 0;
             }
             return w;
         };
-        each([&](int seg, const float *v) {
-            uint64_t w = 0;
+        if (!bordered) {
+            each([&](int seg, const float *v) {
+                uint64_t sum = 0;
 #pragma unroll
-            for (int e = 0; e < 16; e++) w += weigh(v[e], index(seg, e));
-            w = wave_sum(w);
-            if (lane == 0) s_seg[seg] = w;
-        });
-        __syncthreads();
+                for (int e = 0; e < 16; e++) {
+                    const uint64_t w = W(v[e]);
+                    sum += w >= wmin ? w : 0;
+                }
+                sum = wave_sum(sum);
+                if (lane == 0) s_seg[seg] = sum;
+            });
+            __syncthreads();
+        }
         uint64_t total;
         const uint64_t w = tid < segs ? s_seg[tid] : 0, c = block_scan(w, s_scan[0], total);
         const uint64_t target = draw_target(a.u[r], total);
         if (c > target && c - w <= target) {
             s_n = tid;
-            s_x[0] = target - (c - w);
+            s_x = target - (c - w);
         }
         __syncthreads();
         // the segment's tokens, one a thread
         const int i = s_n * k_seg + tid;
-        const uint64_t left = s_x[0];
+        const uint64_t left = s_x;
         const float v = i < n ? x[i] : -INFINITY;
         const uint64_t wi = i < n && v == v ? weigh(v, i) : 0;
         uint64_t of_seg;
@@ -577,7 +763,7 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
         }
         return true;
     };
-    if (!easy()) draw_by_digits(a, D, r, s_hist, s_scan[0]);
+    if (!easy()) draw_by_digits(a, D, r, s_list, s_scan[0]);
 }
 
 }  // namespace lnship
@@ -608,10 +794,13 @@ int lnship_sample(const lnship_sample_args *a, void *stream) {
     const dim3 grid((unsigned)a->n_rows), block(k_draw_block);
     hipStream_t st = (hipStream_t)stream;
     const int rounds = (int)((a->n_vocab + k_seg * k_draw_waves - 1) / (k_seg * k_draw_waves));
+    // Up to two segments a wave stay in registers; of longer rows one, and the
+    // others are read for each pass, which costs less than the registers' spills
+    // (32000 logits 23.4 us in registers, 24.7 so; 49152: 22.1 so, 27.3 with three
+    // in registers; 131075: 75 so, 78 with two).
     if (rounds == 1) hipLaunchKernelGGL((k_draw<1, false>), grid, block, 0, st, d);
     else if (rounds == 2) hipLaunchKernelGGL((k_draw<2, false>), grid, block, 0, st, d);
-    else if (rounds == 3) hipLaunchKernelGGL((k_draw<3, false>), grid, block, 0, st, d);
-    else hipLaunchKernelGGL((k_draw<LNSHIP_RES, true>), grid, block, 0, st, d);
+    else hipLaunchKernelGGL((k_draw<1, true>), grid, block, 0, st, d);
     LNSHIP_HIP(hipGetLastError());
     return 0;
 }
