@@ -53,6 +53,13 @@ STORES = [
     ([9, 12], [25, 12], 16, 2, 2, 72, 18, False),
     ([5], [261], 256, 6, 6, 256, 64, True),
     ([21], [23], 16, 5, 5, 24, 0, False),
+    # 2^19 values and more: tables in LDS, a row or eight to a workgroup
+    ([300, 1, 40], [310, 9, 47], 16, 24, 8, 64, 64, False),
+    ([1] * 90, list(range(1, 91)), 64, 32, 8, 128, 128, True),
+    ([700, 350], [700, 401], 32, 4, 2, 80, 80, True),
+    ([1100], [1117], 16, 2, 2, 96, 48, False),
+    ([1030, 0, 3], [1030, 5, 3], 256, 3, 1, 128, 64, True),
+    ([8200], [8200], 64, 3, 2, 8, 8, False),
 ]
 
 
@@ -147,6 +154,46 @@ def test_store_strides_and_rows_of_no_sequence(ln, ld_extra, shift):
     o = out.cpu().numpy()
     assert np.array_equal(o[2:15], rot_q)
     assert (o[:2] == 7.0).all() and (o[15:] == 7.0).all()
+    assert np.array_equal(k.cpu().numpy().view(np.uint16), c.k) and np.array_equal(v.cpu().numpy().view(np.uint16), c.v)
+
+
+@pytest.mark.parametrize("T,nh,nkv,hd", [(150, 24, 16, 64), (1200, 4, 2, 64)])
+def test_stores_of_many_rows_strided_with_bad_pages(ln, T, nh, nkv, hd):
+    """Rows before the first and behind the last sequence, a bad page, positions past the rope table."""
+    rng = np.random.default_rng(T)
+    page, first = 16, 5
+    q_len = [T - 60, 40]
+    kv_len = [T - 60 + 3, 40]
+    n_pos = T - 62                    # the last five of the first sequence lie behind it
+    table, n_pages = R.tables(rng, kv_len, page)
+    start = starts(q_len, first)
+    cs = rope_table(ln, T, hd)
+    ld = nh * hd + 4
+    q = torch.as_strided(dev(rng.standard_normal(T * ld).astype(np.float32)), (T, nh, hd), (ld, hd, 1), 0)
+    kv = dev((rng.standard_normal((T, 2, nkv, hd)) * 2).astype(np.float32))
+    k, v = ln.paged.alloc_pages(n_pages, page, nkv, hd)
+    bad = table.copy()
+    bad[1, 1] = n_pages + 7           # cells 16 .. 31 of the second sequence
+    index_error(ln)
+    out = torch.full((T, nh, hd), 7.0, device="cuda")
+    ln.paged.rope_store_kv(q, kv[:, 0], kv[:, 1], k, v, page, dev(bad), dev(start), dev(np.int32(kv_len)), dev(cs[:n_pos]),
+                           out=out)
+    assert index_error(ln)[0] == 1
+    pos = positions(q_len, kv_len)
+    rows = np.arange(first, first + T - 20)
+    p, s = np.concatenate(pos), np.repeat([0, 1], q_len)
+    ok = p < n_pos
+    x, kvn = q.cpu().numpy(), kv.cpu().numpy()
+    rot = R.rope(np.concatenate([x[rows], kvn[rows, 0]], 1), cs[p], False, hd)
+    o = out.cpu().numpy()
+    assert np.array_equal(o[rows[ok]], rot[ok][:, :nh])
+    rest = np.setdiff1d(np.arange(T), rows[ok])
+    assert len(rest) == 25 and (o[rest] == 7.0).all()
+    kc, vc = R.store_codes(rot[:, nh:]), R.store_codes(kvn[rows, 1])
+    c = R.Cache(n_pages, page, nkv, hd, fill=0)
+    for i in (0, 1):
+        m = ok & (s == i) & ~((s == 1) & (p // page == 1))
+        c.put(table[i], p[m], kc[m], vc[m])
     assert np.array_equal(k.cpu().numpy().view(np.uint16), c.k) and np.array_equal(v.cpu().numpy().view(np.uint16), c.v)
 
 

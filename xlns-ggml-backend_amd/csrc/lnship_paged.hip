@@ -45,12 +45,6 @@ __device__ __forceinline__ int wave_last_at_most(int n, int x, F key) {
 
 // ---- rope and stores ------------------------------------------------------------
 
-#ifndef LNSHIP_SROWS
-#define LNSHIP_SROWS 32
-#endif
-#ifndef LNSHIP_SWG
-#define LNSHIP_SWG 16
-#endif
 struct store_args {
     lnship_paged_kv kv;
     lnship_paged_store_args a;
@@ -108,6 +102,25 @@ __global__ __launch_bounds__(k_block) void k_store_paged(store_args s, dev_table
     }
 }
 
+// The rotation of a pair of codes by cs, the cosine's code and above it the sine's:
+// y0 = x0 cos - x1 sin, y1 = x0 sin + x1 cos, as x16_mul and x16_add_g form them.
+// Of the two sums exactly one is of two addends alike in sign.
+__device__ __forceinline__ void rotate_pair(const int16_t *g, uint32_t x0, uint32_t x1, uint32_t cs, uint32_t &y0, uint32_t &y1) {
+    const int l0 = x0 & k16_logmask, l1 = x1 & k16_logmask, lc = cs & k16_logmask, ls = cs >> 16 & k16_logmask;
+    auto in_range = [](int l) { return min(max(l, 0), (int)k16_logmask); };
+    auto sum = [&](int p, int q, uint32_t sp, uint32_t sq, bool differ) {
+        const int most = max(p, q), d = most - min(p, q);
+        const int l = in_range(most + g[min(d, k16_esszer + 1) + (differ ? k16_gauss_n : 0)]);
+        const uint32_t r = ((p > q ? sp : sq) & k16_sign) | (uint32_t)l;
+        return (d == 0 && differ) ? 0u : r;
+    };
+    constexpr int one = (int)k16_one;
+    const uint32_t s0 = x0 ^ cs, s1 = x1 ^ cs >> 16;   // (bit 15)
+    const bool alike = (s0 ^ s1) & k16_sign;           // of x0 cos and -x1 sin
+    y0 = sum(in_range(l0 + lc - one), in_range(l1 + ls - one), s0, ~s1, !alike);
+    y1 = sum(in_range(l0 + ls - one), in_range(l1 + lc - one), x0 ^ cs >> 16, x1 ^ cs, alike);
+}
+
 // The codes of a rotated key through F32 and half and back, for a code whose
 // value is a normal half: its exponent, and of its fraction one of two tables
 // of 128 (below 1 the conversion's truncation is upward).  Any other code takes
@@ -140,27 +153,36 @@ struct rev16_lds {
     }
 };
 
-constexpr int k_store_rows = 64;   // rows of a workgroup at most
+constexpr int k_store_rows = 8;   // rows of a workgroup at most
 
 // Many rows, in 16-byte loads: a thread rotates four pairs (or converts eight
-// dims behind the rotated ones) of a head, or stores one dim of a value; a
-// workgroup has consecutive rows.  The conversions, the Gaussian logs and the
-// decoded values come from tables in LDS: from memory each is a gather that
-// costs a cache line a lane.  Bound by HBM and the LDS lookups (8 a pair).
+// dims behind the rotated ones) of a head, or stores four dims of a value; a
+// workgroup has one row or eight, threads beside each other taking the rows of
+// one item, whose cells then fill cache lines in one store.  The conversions, the
+// Gaussian logs and the decoded values come from tables in LDS: from memory each
+// is a gather that costs a cache line a lane.  A row's cosines and sines are
+// converted once for all heads.  Bound by the arithmetic of the codes, some 40
+// instructions a pair and 60 for its conversions, and by the scattered stores:
+// 11414 rows of 32 heads of 64 on 8 in 77 us, 3.4 TB/s of what is read and written
+// (with rows spread over all XCDs 94: the caches' lines are then written in parts).
 template <bool NEOX>
-__global__ __launch_bounds__(k_block) void k_store_paged_rows(store_args s, int rows_wg, dev_tables T,
+__global__ __launch_bounds__(k_block, 8) void k_store_paged_rows(store_args s, int row_sh, dev_tables T,
                                                               unsigned long long *err) {
     __shared__ uint16_t s_cvt[k_cvt_lds];
     __shared__ alignas(16) int16_t s_g[2 * k16_gauss_n];
     __shared__ int16_t s_half[256];
     __shared__ float s_rev[k_rev_lds];
     __shared__ int s_pos[k_store_rows], s_page[k_store_rows];
+    __shared__ alignas(16) uint16_t s_cs[k_store_rows * 256];
     const lnship_paged_kv &kv = s.kv;
     const lnship_paged_store_args &a = s.a;
     const int tid = threadIdx.x, hd = (int)kv.head_dim, nd = a.rope_n_dims, page = (int)kv.page;
     const int n_head = (int)a.n_head, n_head_kv = (int)kv.n_head_kv, n_seq = (int)kv.n_seq;
-    const int64_t t0 = (int64_t)blockIdx.x * rows_wg;
-    const int rows = (int)min((int64_t)rows_wg, kv.ntok - t0);
+    // rows side by side on one XCD: their cells share cache lines
+    const uint32_t of_xcd = (gridDim.x + 7) / 8, wg = blockIdx.x % 8 * of_xcd + blockIdx.x / 8;
+    const int64_t t0 = (int64_t)wg << row_sh;
+    const int rows = (int)min((int64_t)1 << row_sh, kv.ntok - t0);
+    if (rows <= 0) return;
     if (tid < rows) {
         const int64_t t = t0 + tid;
         int pos = -1, id = -1;
@@ -192,12 +214,24 @@ __global__ __launch_bounds__(k_block) void k_store_paged_rows(store_args s, int 
     for (int i = tid; i < 256; i += k_block) s_half[i] = (int16_t)(H.slow(k16_one - 128 + i) - (k16_one + (i & 128) - 128));
     const rev16_lds V{s_rev, T.rev16};
     __syncthreads();
+    // a row's cosines and sines, once for all heads
+    for (int i = tid * 4; i < rows * nd; i += k_block * 4) {
+        const int r = (int)((uint32_t)i / (uint32_t)nd);
+        const float4 u = *reinterpret_cast<const float4 *>(a.cos_sin + (int64_t)max(s_pos[r], 0) * nd + (i - r * nd));
+        const float w[4] = {u.x, u.y, u.z, u.w};
+        uint32_t z[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) z[j] = C(w[j]);
+        *reinterpret_cast<uint2 *>(&s_cs[i]) = make_uint2(z[0] | z[1] << 16, z[2] | z[3] << 16);
+    }
+    __syncthreads();
 
-    const int eighths = hd >> 3, rot_q = n_head * eighths, rot = rot_q + n_head_kv * eighths, per = rot + n_head_kv * hd;
+    const int eighths = hd >> 3, rot_q = n_head * eighths, rot = rot_q + n_head_kv * eighths;
+    const int nk = n_head_kv * hd, span = 64 >> row_sh, per = rot + (nk + 4 * span - 1) / (4 * span) * span;
     const int64_t head_codes = (int64_t)page * hd;
-    int r = 0, e = tid;
-    while (e >= per) e -= per, r++;
-    for (; r < rows;) {
+    for (int i = (int)(blockIdx.y * k_block) + tid; i < per << row_sh; i += (int)(gridDim.y * k_block)) {
+        const int r = i & ((1 << row_sh) - 1), e = i >> row_sh;
+        if (r >= rows) continue;
         const int pos = s_pos[r], id = s_page[r];
         const int64_t t = t0 + r;
         if (pos >= 0) {
@@ -216,17 +250,12 @@ __global__ __launch_bounds__(k_block) void k_store_paged_rows(store_args s, int 
                     cvt16_batch(C, w, y);
                 }
                 if (rotate) {
-                    const float4 *cs = reinterpret_cast<const float4 *>(a.cos_sin + (int64_t)pos * nd) + o * 2;
-                    const float4 u = cs[0], v = cs[1];
-                    const float w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-                    uint32_t z[8];   // cos, sin of four pairs
-                    cvt16_batch(C, w, z);
+                    const uint4 cs = *reinterpret_cast<const uint4 *>(&s_cs[r * nd + o * 8]);   // of four pairs
+                    const uint32_t z[4] = {cs.x, cs.y, cs.z, cs.w};
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const int i0 = NEOX ? j : 2 * j, i1 = NEOX ? j + 4 : 2 * j + 1;
-                        const uint32_t x0 = y[i0], x1 = y[i1], co = z[2 * j], si = z[2 * j + 1];
-                        y[i0] = x16_add_g(s_g, x16_mul(x0, co), x16_mul(x1, si) ^ k16_sign);
-                        y[i1] = x16_add_g(s_g, x16_mul(x0, si), x16_mul(x1, co));
+                        rotate_pair(s_g, y[i0], y[i1], z[j], y[i0], y[i1]);
                     }
                 }
                 if (!key) {
@@ -247,14 +276,22 @@ __global__ __launch_bounds__(k_block) void k_store_paged_rows(store_args s, int 
                     }
                 }
             } else if (id >= 0) {
-                const int f = e - rot, h = (int)((uint32_t)f / (uint32_t)hd), d = f - h * hd;
-                const float v = a.v[t * a.v_ld + f];
-                kv.v_pages[((int64_t)id * n_head_kv + h) * head_codes + ((c >> 3) * hd + d) * 8 + (c & 7)] =
-                    (uint16_t)C(__half2float(__float2half_rn(v)));
+                // four dims of the values, 64 / rows apart
+                const int g = e - rot, f = (g & ~(span - 1)) * 4 + (g & (span - 1));
+                const float *x = a.v + t * a.v_ld;
+                float w[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = x[min(f + span * j, nk - 1)];
+                int h = (int)((uint32_t)f / (uint32_t)hd), d = f - h * hd;
+                uint16_t *v = kv.v_pages + (int64_t)id * n_head_kv * head_codes + (c >> 3) * hd * 8 + (c & 7);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (f + span * j < nk) v[h * head_codes + d * 8] = (uint16_t)C(__half2float(__float2half_rn(w[j])));
+                    d += span;
+                    while (d >= hd) d -= hd, h++;
+                }
             }
         }
-        e += k_block;
-        while (e >= per) e -= per, r++;
     }
 }
 
@@ -1234,11 +1271,21 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
     const bool vec = a->rope_n_dims > 0 && a->rope_n_dims % 8 == 0 &&
                      (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->cos_sin | (uintptr_t)a->q_dst) & 15) == 0 &&
                      ((a->q_ld | a->k_ld | s.a.q_dst_ld) & 3) == 0;
-    if (vec && kv->ntok >= LNSHIP_SROWS) {
-        const int rows = (int)std::min<int64_t>(k_store_rows, std::max<int64_t>(1, kv->ntok / (LNSHIP_SWG * st->cus)));
-        const dim3 grid((unsigned)((kv->ntok + rows - 1) / rows));
-        if (a->neox) hipLaunchKernelGGL(k_store_paged_rows<true>, grid, dim3(k_block), 0, (hipStream_t)stream, s, rows, st->T, st->index_err);
-        else hipLaunchKernelGGL(k_store_paged_rows<false>, grid, dim3(k_block), 0, (hipStream_t)stream, s, rows, st->T, st->index_err);
+    // (its tables take 4 us to lay out: 64 rows of 32 heads of 128 on 8 6.7 us without,
+    // 8.4 so, 128 rows 9.6 and 8.6; 128 of 9 heads of 64 on 3 4.9 and 8.3)
+    if (vec && kv->ntok * (nq + 2 * nk) >= 1 << 19) {
+        // Eight rows of a prompt together, as their cells share cache lines (8 prompts
+        // of 511 to 2047 tokens, 32 heads of 64 on 8: 77 us, by single rows 85); single
+        // tokens' rows, and few, by themselves (4096 sequences' tokens, heads of 128: 75,
+        // by eight 83).  Workgroups: 16 a CU, if there is an item for each thread (256
+        // tokens 10.3 us, a workgroup a row 13).
+        const int sh = kv->ntok >= 1024 && kv->ntok >= 8 * kv->n_seq ? 3 : 0;
+        const int64_t x = (((kv->ntok + (1 << sh) - 1) >> sh) + 7) / 8 * 8;   // (all of every XCD's share)
+        const int64_t items = (nq / 8 + nk / 8 + nk / 4) << sh;
+        const int64_t y = std::max<int64_t>(1, std::min(16 * st->cus / x, items / k_block));
+        const dim3 grid((unsigned)x, (unsigned)y);
+        if (a->neox) hipLaunchKernelGGL(k_store_paged_rows<true>, grid, dim3(k_block), 0, (hipStream_t)stream, s, sh, st->T, st->index_err);
+        else hipLaunchKernelGGL(k_store_paged_rows<false>, grid, dim3(k_block), 0, (hipStream_t)stream, s, sh, st->T, st->index_err);
         LNSHIP_HIP(hipGetLastError());
         return 0;
     }
