@@ -44,28 +44,44 @@ __device__ __forceinline__ V uniform(V v) {
     return u.v;
 }
 
-// The weight e^((x - x_max) / T) in units of 2^-40, rounded, of any x_max and T.
-// The exponent is formed in 64 bits (32 would lose what tells two sums apart),
-// its fraction's power in 32: 24 bits of every weight.  Integers come out of the
-// low bits of a sum with a power of two.
+// 2^r for r in [-1/2, 1/2], to 2^-34: the polynomial of degree 7 through it at the
+// Chebyshev nodes of that range.
+__device__ __forceinline__ double power(double r) {
+    double p = 1.5303700711425663e-05;
+    p = fma(p, r, 0.00015469729214122798);
+    p = fma(p, r, 0.0013333478473685175);
+    p = fma(p, r, 0.009618025613318018);
+    p = fma(p, r, 0.055504109063258665);
+    p = fma(p, r, 0.24022651213498092);
+    p = fma(p, r, 0.6931471805568324);
+    return fma(p, r, 0.9999999999595618);
+}
+
+// 2^y, y in [-64, 0], in units of 2^-40, rounded.  A sum with a power of two
+// splits y and makes the result an integer, which costs less than conversions;
+// the whole part goes into the power's exponent.  All in 64 bits: in 32 the
+// weights of a few likely tokens are off by more than the share of a token of a
+// large vocabulary's tail, and another than it would be drawn now and then.
+__device__ __forceinline__ uint64_t in_units(double y) {
+    constexpr double whole = 6755399441055744.0;   // 1.5 2^52: a sum's low word is the integer
+    constexpr double unit = 4096.0;                // a sum's last place is 2^-40
+    const double t = y + whole;
+    const uint64_t p = (uint64_t)__double_as_longlong(power(y - (t - whole)));
+    const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)(uint64_t)__double_as_longlong(t) << 20);
+    const double w = __longlong_as_double((int64_t)((uint64_t)hi << 32 | (uint32_t)p));
+    return (uint64_t)__double_as_longlong(w + unit) - (uint64_t)__double_as_longlong(unit);
+}
+
+// The weight e^((x - x_max) / T) in units of 2^-40, of any x_max and T.
 struct any_weigher {
     double xmax, f;   // f = log2 e / T
     __device__ __forceinline__ uint64_t operator()(float x) const {
-        constexpr double whole = 6755399441055744.0;   // 1.5 2^52: a sum's low word is the integer
-        constexpr double unit = 4096.0;                // a sum's last place is 2^-40
-        const double y = fmax(((double)x - xmax) * f, -63.0);   // (-inf times an f of 0: -63)
-        const double t = y + whole;
-        // 2^r in [2^-1/2, 2^1/2]
-        const float p = __builtin_amdgcn_exp2f((float)(y - (t - whole)));
-        const double w = ldexp((double)p, (int)(uint32_t)__double_as_longlong(t));
-        return (uint64_t)__double_as_longlong(w + unit) - (uint64_t)__double_as_longlong(unit);
+        return in_units(fmax(((double)x - xmax) * f, -63.0));   // (-inf times an f of 0: -63)
     }
 };
 
-// The same where |x_max f| <= 2^20, in three operations of 64 bits: of x f + c,
-// c = 1.5 2^20 - x_max f, the high word holds the exponent's whole part and the
-// low word its fraction, to 2^-32.  The power of the fraction is in [1, 2]; its
-// F32 bits become those of the double with the whole part in its exponent.
+// The same where |x_max f| <= 2^20: the exponent in one product, to 2^-33.  Some 105
+// cycles of a wave, most of them the 13 operations of 64 bits.
 struct weigher {
     double f, c;
     float lo;   // x where the weight is 2^-63: what lies below weighs nothing either
@@ -73,15 +89,8 @@ struct weigher {
         return fabs((double)xmax * f) <= 1048576.0 && f >= 1e-30;
     }
     __device__ __forceinline__ weigher(float xmax, double f_)
-        : f(f_), c(uniform(1572864.0 - (double)xmax * f_)), lo(uniform((float)fmax((double)xmax - 63.0 / f_, -3.4028234e38))) {}
-    __device__ __forceinline__ uint64_t operator()(float x) const {
-        constexpr double unit = 4096.0;   // a sum's last place is 2^-40
-        const uint64_t t = (uint64_t)__double_as_longlong(fma((double)fmaxf(x, lo), f, c));
-        const uint32_t p = f32_bits(__builtin_amdgcn_exp2f((float)(uint32_t)t * 0x1p-32f));
-        const uint32_t hi = ((uint32_t)(t >> 32) << 20) + (p >> 3) + ((1023u << 20) - (127u << 20));
-        const double w = __longlong_as_double((int64_t)((uint64_t)hi << 32 | p << 29));
-        return (uint64_t)__double_as_longlong(w + unit) - (uint64_t)__double_as_longlong(unit);
-    }
+        : f(f_), c(uniform(-(double)xmax * f_)), lo(uniform((float)fmax((double)xmax - 63.0 / f_, -3.4028234e38))) {}
+    __device__ __forceinline__ uint64_t operator()(float x) const { return in_units(fma((double)fmaxf(x, lo), f, c)); }
 };
 
 // v of the lane that DPP control C names, in the rows of M; zero where there is none
@@ -361,9 +370,9 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
 //   above them on, name the border exactly; if it is not among them (or
 //   too many tokens are) the row takes draw_by_digits.
 // - The segment that holds u's share is gone through again.
-// Bound by a row's passes on one CU: one of loads, and one of weights at 98 cycles
-// a wave's 64.  256 rows of 131075: 22 us greedy, 45 with a top_k, 49 with neither
-// and 68 with a top_p (a row's exact histogram of 64-bit weights instead: 106).
+// Bound by a row's passes on one CU: one of loads, and one of weights (above).
+// 256 rows of 131075: 22 us greedy (6 TB/s), 45 with a top_k, 53 with neither and
+// 74 with a top_p (with an exact histogram of 64-bit weights for its border 106).
 template <int R, bool MORE>
 __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
     typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));   // rows need no alignment
@@ -568,6 +577,7 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
                 s_cnt[slot] = through ? c + at_b : c;
             };
             int lo = 0, hi;   // the bins of the list
+            bool cut = true;
             if (by_count) {
                 // (fewer weigh anything: all bins but the last)
                 const uint64_t v[4] = {h[0], h[1], h[2], h[3]};
@@ -592,133 +602,138 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
                 __syncthreads();
                 const int of = s_cnt[1] - s_cnt[0] <= (uint32_t)(k_list - 64) << shift ? 0 : 2;
                 lo = s_bin[of], hi = s_bin[of + 1];
+                if (wmin) {
+                    // min_p's border above top_p's: that one alone counts; at or below the
+                    // list's first bin: what lies above the list is above it too
+                    const int at = (int)(place_of(D.xmax) - log2f(fminf(D.min_p, 1.0f)) * k_bins_binade);
+                    cut = at + 1 >= s_bin[0];
+                    lo = max(min(lo, at - 1), 0);
+                }
             }
-            auto push = [&](float v, int i) {
-                const int at = atomicAdd(&s_n, 1);
-                if (at < k_list) s_list[at] = (uint64_t)order_key(v) << 32 | (uint32_t)(0x7fffffff - i);
-            };
-            uint64_t all = 0, above = 0;
-            asm volatile("" : "+v"(ref));   // bins are formed again, not kept in registers
-            ref = uniform(ref);
-            if (by_count) {
-                each([&](int seg, const float *v) {
+            if (cut) {
+                auto push = [&](float v, int i) {
+                    const int at = atomicAdd(&s_n, 1);
+                    if (at < k_list) s_list[at] = (uint64_t)order_key(v) << 32 | (uint32_t)(0x7fffffff - i);
+                };
+                uint64_t all = 0, above = 0;
+                asm volatile("" : "+v"(ref));   // bins are formed again, not kept in registers
+                ref = uniform(ref);
+                if (by_count) {
+                    each([&](int seg, const float *v) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (bin_of(v[e]) <= hi) push(v[e], index(seg, e));
-                });
-            } else {
-                // the weights of all tokens and of those above the list; by
-                // segment, of those above that min_p keeps
-                each([&](int seg, const float *v) {
-                    uint64_t sum = 0;
+                        for (int e = 0; e < 16; e++)
+                            if (bin_of(v[e]) <= hi) push(v[e], index(seg, e));
+                    });
+                } else {
+                    // the weights of all tokens, and by segment of those above the list
+                    each([&](int seg, const float *v) {
+                        uint64_t sum = 0;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const uint64_t w = W(v[e]);
-                        const int b = bin_of(v[e]);
-                        all += w;
-                        if (b < lo) {
-                            above += w;
-                            sum += w >= wmin ? w : 0;
-                        } else if (b <= hi) {
-                            push(v[e], index(seg, e));
+                        for (int e = 0; e < 16; e++) {
+                            const uint64_t w = W(v[e]);
+                            const int b = bin_of(v[e]);
+                            all += w;
+                            sum += b < lo ? w : 0;
+                            if (b >= lo && b <= hi) push(v[e], index(seg, e));
                         }
+                        sum = wave_sum(sum);
+                        above += sum;
+                        if (lane == 0) s_seg[seg] = sum;
+                    });
+                    all = wave_sum(all);
+                    if (lane == 0) s_scan[0][wave] = all, s_scan[1][wave] = above;
+                }
+                __syncthreads();
+                const int m = s_n;
+                if (m > k_list) return false;
+                if (!by_count) {
+                    all = above = 0;
+                    for (int w = 0; w < k_draw_waves; w++) all += s_scan[0][w], above += s_scan[1][w];
+                }
+                if (by_count) {
+                    order_items(s_list, s_sorted, s_place, m);
+                    // the first top_k, of those top_p's, of those min_p's; then by index
+                    const int k = min(D.top_k, m);
+                    uint64_t w = tid < k ? W(key_value((uint32_t)(s_sorted[tid] >> 32))) : 0, total;
+                    uint64_t c = block_scan(w, s_scan[0], total);
+                    int kept = k;
+                    if (D.top_p < 1.0f) {
+                        const double p = ceil((double)D.top_p * (double)total);
+                        const uint64_t need = p >= 1.0 ? min((uint64_t)p, total) : 1;
+                        if (tid == 0) s_n = 1;
+                        __syncthreads();
+                        if (tid < k && c - w < need && c >= need) s_n = tid + 1;
+                        __syncthreads();
+                        kept = s_n;
                     }
-                    sum = wave_sum(sum);
-                    if (lane == 0) s_seg[seg] = sum;
-                });
-                all = wave_sum(all), above = wave_sum(above);
-                if (lane == 0) s_scan[0][wave] = all, s_scan[1][wave] = above;
-            }
-            __syncthreads();
-            const int m = s_n;
-            if (m > k_list) return false;
-            if (!by_count) {
-                all = above = 0;
-                for (int w = 0; w < k_draw_waves; w++) all += s_scan[0][w], above += s_scan[1][w];
-            }
-            if (by_count) {
-                order_items(s_list, s_sorted, s_place, m);
-                // the first top_k, of those top_p's, of those min_p's; then by index
-                const int k = min(D.top_k, m);
-                uint64_t w = tid < k ? W(key_value((uint32_t)(s_sorted[tid] >> 32))) : 0, total;
-                uint64_t c = block_scan(w, s_scan[0], total);
-                int kept = k;
-                if (D.top_p < 1.0f) {
-                    const double p = ceil((double)D.top_p * (double)total);
-                    const uint64_t need = p >= 1.0 ? min((uint64_t)p, total) : 1;
-                    if (tid == 0) s_n = 1;
+                    const bool in = tid < kept && w > 0 && w >= wmin;
+                    if (tid < k_list / 2) s_list[tid] = 0;   // (what is not kept comes last)
                     __syncthreads();
-                    if (tid < k && c - w < need && c >= need) s_n = tid + 1;
+                    // order by index: its complement above, its place in the ranking below
+                    if (tid < kept) s_list[tid] = (uint64_t)(uint32_t)s_sorted[tid] << 32 | (in ? (uint32_t)tid + 1u : 0u);
                     __syncthreads();
-                    kept = s_n;
+                    uint64_t *const by_index = s_sorted + k_list / 2;   // (top_k <= k_list / 2)
+                    order_items(s_list, by_index, s_place, kept);
+                    const uint32_t rank = tid < kept ? (uint32_t)by_index[tid] : 0u;
+                    const uint64_t item = rank ? s_sorted[rank - 1] : 0;
+                    w = rank ? W(key_value((uint32_t)(item >> 32))) : 0;
+                    c = block_scan(w, s_scan[1], total);
+                    const uint64_t target = draw_target(a.u[r], total);
+                    if (w && c > target && c - w <= target) {
+                        a.tokens[r] = 0x7fffffff - (int32_t)(uint32_t)item;
+                        if (a.probs) a.probs[r] = (float)((double)w / (double)total);
+                    }
+                    return true;
                 }
-                const bool in = tid < kept && w > 0 && w >= wmin;
-                if (tid < k_list / 2) s_list[tid] = 0;   // (what is not kept comes last)
+                // top_p: the first of the list, as many as the weight still needs.  The
+                // list's weights are summed over finer bins; the tokens of that in which
+                // the border lies are put in order.
+                const double p = ceil((double)D.top_p * (double)all);
+                const uint64_t want = p >= 1.0 ? min((uint64_t)p, all) : 1;
+                auto value = [&](uint64_t item) { return key_value((uint32_t)(item >> 32)); };
+                const float fine = (float)k_draw_block / (float)(hi - lo + 1);
+                auto fine_bin = [&](uint64_t item) {
+                    return (int)fminf((place_of(value(item)) - (float)lo) * fine, (float)(k_draw_block - 1));
+                };
+                s_sorted[tid] = 0;
+                if (tid == 0) s_n = -1, s_cnt[0] = 0;
                 __syncthreads();
-                // order by index: its complement above, its place in the ranking below
-                if (tid < kept) s_list[tid] = (uint64_t)(uint32_t)s_sorted[tid] << 32 | (in ? (uint32_t)tid + 1u : 0u);
+                for (int i = tid; i < m; i += k_draw_block)
+                    atomicAdd((unsigned long long *)&s_sorted[fine_bin(s_list[i])], (unsigned long long)W(value(s_list[i])));
                 __syncthreads();
-                uint64_t *const by_index = s_sorted + k_list / 2;   // (top_k <= k_list / 2)
-                order_items(s_list, by_index, s_place, kept);
-                const uint32_t rank = tid < kept ? (uint32_t)by_index[tid] : 0u;
-                const uint64_t item = rank ? s_sorted[rank - 1] : 0;
-                w = rank ? W(key_value((uint32_t)(item >> 32))) : 0;
-                c = block_scan(w, s_scan[1], total);
-                const uint64_t target = draw_target(a.u[r], total);
-                if (w && c > target && c - w <= target) {
-                    a.tokens[r] = 0x7fffffff - (int32_t)(uint32_t)item;
-                    if (a.probs) a.probs[r] = (float)((double)w / (double)total);
+                uint64_t part;
+                const uint64_t wf = s_sorted[tid], cf = above + block_scan(wf, s_scan[0], part);
+                if (cf - wf < want && cf >= want) {
+                    s_n = tid;
+                    s_x = cf - wf;
                 }
-                return true;
+                __syncthreads();
+                const int at = s_n;
+                if (at < 0) return false;   // (the border is not in the list)
+                uint64_t before = s_x;
+                for (int i = tid; i < m; i += k_draw_block)
+                    if (fine_bin(s_list[i]) == at) s_sorted[atomicAdd(&s_cnt[0], 1u)] = s_list[i];
+                __syncthreads();
+                const int few = (int)s_cnt[0];
+                order_items(s_sorted, s_order, s_place, few);
+                for (int i0 = 0; i0 < few; i0 += k_draw_block) {
+                    const uint64_t w = i0 + tid < few ? W(value(s_order[i0 + tid])) : 0;
+                    const uint64_t c = before + block_scan(w, s_scan[1 - (i0 / k_draw_block & 1)], part);
+                    if (c - w < want && c >= want) s_n = i0 + tid;
+                    before += part;
+                }
+                __syncthreads();
+                const uint64_t item = s_order[s_n];
+                for (int i = tid; i < m; i += k_draw_block) {
+                    const uint64_t w = W(value(s_list[i]));
+                    if (s_list[i] >= item && w >= wmin)
+                        atomicAdd((unsigned long long *)&s_seg[(0x7fffffff - (int)(uint32_t)s_list[i]) / k_seg], (unsigned long long)w);
+                }
+                bkey = (uint32_t)(item >> 32);
+                bidx = 0x7fffffff - (int)(uint32_t)item;
+                bordered = true;
+                __syncthreads();
             }
-            // top_p: the first of the list, as many as the weight still needs.  The
-            // list's weights are summed over finer bins; the tokens of that in which
-            // the border lies are put in order.
-            const double p = ceil((double)D.top_p * (double)all);
-            const uint64_t want = p >= 1.0 ? min((uint64_t)p, all) : 1;
-            auto value = [&](uint64_t item) { return key_value((uint32_t)(item >> 32)); };
-            const float fine = (float)k_draw_block / (float)(hi - lo + 1);
-            auto fine_bin = [&](uint64_t item) {
-                return (int)fminf((place_of(value(item)) - (float)lo) * fine, (float)(k_draw_block - 1));
-            };
-            s_sorted[tid] = 0;
-            if (tid == 0) s_n = -1, s_cnt[0] = 0;
-            __syncthreads();
-            for (int i = tid; i < m; i += k_draw_block)
-                atomicAdd((unsigned long long *)&s_sorted[fine_bin(s_list[i])], (unsigned long long)W(value(s_list[i])));
-            __syncthreads();
-            uint64_t part;
-            const uint64_t wf = s_sorted[tid], cf = above + block_scan(wf, s_scan[0], part);
-            if (cf - wf < want && cf >= want) {
-                s_n = tid;
-                s_x = cf - wf;
-            }
-            __syncthreads();
-            const int at = s_n;
-            if (at < 0) return false;   // (the border is not in the list)
-            uint64_t before = s_x;
-            for (int i = tid; i < m; i += k_draw_block)
-                if (fine_bin(s_list[i]) == at) s_sorted[atomicAdd(&s_cnt[0], 1u)] = s_list[i];
-            __syncthreads();
-            const int few = (int)s_cnt[0];
-            order_items(s_sorted, s_order, s_place, few);
-            for (int i0 = 0; i0 < few; i0 += k_draw_block) {
-                const uint64_t w = i0 + tid < few ? W(value(s_order[i0 + tid])) : 0;
-                const uint64_t c = before + block_scan(w, s_scan[1 - (i0 / k_draw_block & 1)], part);
-                if (c - w < want && c >= want) s_n = i0 + tid;
-                before += part;
-            }
-            __syncthreads();
-            const uint64_t item = s_order[s_n];
-            for (int i = tid; i < m; i += k_draw_block) {
-                const uint64_t w = W(value(s_list[i]));
-                if (s_list[i] >= item && w >= wmin)
-                    atomicAdd((unsigned long long *)&s_seg[(0x7fffffff - (int)(uint32_t)s_list[i]) / k_seg], (unsigned long long)w);
-            }
-            bkey = (uint32_t)(item >> 32);
-            bidx = 0x7fffffff - (int)(uint32_t)item;
-            bordered = true;
-            __syncthreads();
         }
         auto weigh = [&](float v, int i) {
             uint64_t w = W(v);
@@ -730,16 +745,20 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
             return w;
         };
         if (!bordered) {
-            each([&](int seg, const float *v) {
-                uint64_t sum = 0;
+            auto sums = [&](auto keeps) {
+                each([&](int seg, const float *v) {
+                    uint64_t sum = 0;
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const uint64_t w = W(v[e]);
-                    sum += w >= wmin ? w : 0;
-                }
-                sum = wave_sum(sum);
-                if (lane == 0) s_seg[seg] = sum;
-            });
+                    for (int e = 0; e < 16; e++) {
+                        const uint64_t w = W(v[e]);
+                        sum += keeps(w) ? w : 0;
+                    }
+                    sum = wave_sum(sum);
+                    if (lane == 0) s_seg[seg] = sum;
+                });
+            };
+            if (wmin) sums([&](uint64_t w) { return w >= wmin; });
+            else sums([](uint64_t) { return true; });
             __syncthreads();
         }
         uint64_t total;
