@@ -436,7 +436,13 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
  * work: lnship16_attn_paged_work bytes of device memory, 16-byte aligned,
  * that nothing else uses until the call has run (calls on two streams, or
  * graphs that may replay side by side, need one each); it may be null where
- * that is 0. */
+ * that is 0.  It holds the parts that a row's cells are split into and, where
+ * many rows meet a sequence's cells, those cells decoded once for all of them
+ * (8 bytes a value, up to 1 GiB; where the tables' cells are more, each
+ * workgroup decodes what it reads).  Which way a call takes goes by its sizes
+ * (ntok, n_seq and the tables' cells), not by what q_start and kv_len hold, so
+ * a captured graph replays the same kernels.
+ * Up to 2^30 cells a row of the table, 2^24 (token, head) rows. */
 typedef struct lnship_paged_attn_args {
     const float *q;
     float *dst;
@@ -468,7 +474,9 @@ int64_t lnship16_attn_paged_work(const lnship_paged_kv *kv, int64_t n_head);
  * drawn; with an infinite largest logit only its equals weigh anything; a row
  * without any logit above -inf gets token -1 and probability 0.  Weights are
  * summed as integers (units of 2^-40), so the draw does not depend on an order
- * of additions.  n_vocab up to 2^19.  No LNS arithmetic, and no counterpart in
+ * of additions; a weight is exact to 2^-32.  n_vocab up to 2^19.  A row whose
+ * top_k is above 1024, or with thousands of equal logits at a limit, takes
+ * several times as long as another.  No LNS arithmetic, and no counterpart in
  * the reference, which samples on the host.
  * work: lnship_sample_work bytes, as in lnship_paged_attn_args. */
 typedef struct lnship_sample_args {

@@ -483,6 +483,10 @@ __device__ __forceinline__ void load_q(const float *q, int d, int hd, bool vec, 
 // O^T = V^T P^T, and both caches' layouts give a lane's share of K and V in
 // 16-byte loads, straight from memory.  The next block's keys are loaded while
 // this one's weights are formed, its values once this one's are decoded.
+// Bound by HBM where the cache is long: 64 sequences of 100 to 8000 cells, 32 heads of
+// 128 on 8, in 300 us, 3.7 TB/s of keys and values (a sum over memory reads 4.0); one of
+// 131072 cells in 125 us, 4.2 TB/s.  300 cells of 9 heads of 64 on 3 take 10.7 us: the
+// loads of lengths, pages, keys and values wait for each other.
 template <int NB, bool FULL>   // 32-wide groups of head_dim; whether it fills them
 __global__ __launch_bounds__(256, NB <= 4 ? 3 : 1) void k_attn_paged(attn_paged_args a, unsigned long long *err) {
     const lnship_paged_kv &kv = a.kv;
@@ -796,8 +800,9 @@ struct tile_maker {
     }
 };
 
-// The cells that a chunk sees, decoded into the workspace, for k_attn_chunk to
+// The cells that chunks see, decoded into the workspace, for k_attn_tiles to
 // copy: a workgroup takes every gridDim.x-th tile of a sequence and kv head.
+// Eight bytes are written for two: 8192 cells of 8 heads of 128 take 18 us.
 template <int NB>
 __global__ __launch_bounds__(256) void k_attn_decode(attn_paged_args a, unsigned long long *err) {
     const lnship_paged_kv &kv = a.kv;
@@ -959,11 +964,15 @@ __device__ __forceinline__ int chunk_tile(int nkv, int &kvh) {
 }
 
 // Many rows a sequence (prompts, chunks), over cells that k_attn_decode has
-// decoded: four waves of 32 rows go over them 32 at a time, from two LDS
-// buffers; while one is multiplied the next block is copied into the other.
-// Small workgroups, two or more on a CU: a barrier holds only waves of other
-// SIMDs together, so that on each SIMD one workgroup's wave multiplies while
-// another's forms weights.
+// decoded: NW waves of 32 rows go over them 32 at a time, from two LDS buffers;
+// while one is multiplied the next block is copied into the other, without
+// registers.  Two or more workgroups to a CU, where registers leave room: a
+// barrier holds one of them up, and the other's waves multiply meanwhile.
+// Bound by the matrix cores: 4096 tokens behind 4096 cells, 32 heads of 128 on 8, in
+// 1043 to 1090 us (box to box), of which k_attn_decode takes 18: 1140 TFLOP/s in
+// f16, three products for one, where a library's large product reaches 1163; the
+// clock falls from 2.15 to 1.76 GHz under this load.  Two prompts of 1900 to 2500
+// tokens, 32 heads of 64 on 8, in a window of 1000: 134 us.
 template <int NB, int NW>
 __global__ __launch_bounds__(NW * 64, NB <= 2 ? 3 : 2) void k_attn_tiles(attn_paged_args a, unsigned long long *err) {
     constexpr int B = tile_of<NB>::B, NT = NW * 64;
@@ -999,10 +1008,12 @@ __global__ __launch_bounds__(NW * 64, NB <= 2 ? 3 : 2) void k_attn_tiles(attn_pa
     r.write(a, T, split);
 }
 
-// The same where the tables' cells are more than the workspace holds decoded:
-// NW waves go over 64 cells at a time and decode the codes themselves, each once
-// a workgroup, by the thread that loaded it a tile before, into the other of
-// two LDS buffers.
+// The same where a cell meets one tile or two of a sequence, or the tables' cells
+// are more than the workspace holds decoded: NW waves go over 64 cells at a time
+// and decode the codes themselves, each once a workgroup, by the thread that loaded
+// it a tile before, into the other of two LDS buffers.  Bound by the decoding and
+// the products in turn, and with few workgroups by the slowest: 9 conversations of 5
+// to 301 tokens behind up to 1777, 9 heads of 64 on 3, in 36 us with the join.
 template <int NB, int NW>   // 32-wide groups of head_dim; waves
 __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsigned long long *err) {
     constexpr int U = tile_of<NB>::U;
@@ -1034,19 +1045,15 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     r.place(a, T, kvh, T.r0 + wave * 32);
     r.load(a);
     lds_barrier();
-    // Half of the waves decode before their products, half behind them: on a
-    // SIMD one wave then forms weights or decodes while the other multiplies.
-    const bool early = NW == 8 && wave >= NW / 2;
     int buf = 0;
     for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
-        if (early) prepare(cb + 64, buf ^ 1);
 #pragma unroll 1
         for (int blk = 0; blk < 2; blk++) {
             const uint32_t ok = (uint32_t)__builtin_amdgcn_readfirstlane(
                 (int)*reinterpret_cast<const uint32_t *>(&s_ok[buf][blk * 4]));
             r.block(s_cells + buf * 4 * U + blk * 2 * U, cb + blk * 32, ok, T.c1);
         }
-        if (!early) prepare(cb + 64, buf ^ 1);
+        prepare(cb + 64, buf ^ 1);
         lds_barrier();
     }
     r.write(a, T, split);
@@ -1054,7 +1061,8 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
 
 // The splits' parts of a row joined, in a fixed order, by one wave (four rows a
 // workgroup) or, many parts, by the workgroup's four: head_dim / 4 lanes read a
-// part, the others other parts beside it.
+// part, the others other parts beside it.  Bound by the launch and one read of the
+// parts: 7.5 us for the rows of 9 conversations, 9 heads of 64.
 template <int W>   // waves of a row
 __global__ __launch_bounds__(256) void k_attn_paged_join(attn_paged_args a) {
     constexpr int S = W == 4 ? 256 : 64;   // parts at most
