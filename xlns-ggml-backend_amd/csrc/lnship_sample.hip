@@ -359,7 +359,7 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
 // a wave are held in registers; the rest of a longer row (MORE) is read again
 // for every pass, from L2 or the memory-side cache.
 // - The largest logit; with top_k or top_p also one histogram over the distance
-//   from it, of counts for top_k, of 14-bit weights for top_p, which names the
+//   from it, of counts for top_k, of weights in 12 to 16 bits for top_p, which names the
 //   bins that the border lies in.  In a long row both come from one pass: the
 //   bins are counted from the largest of the first segments, with 22 binades
 //   above it (a row that reaches beyond is counted again).
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
     __shared__ uint32_t s_place[k_list];
     __shared__ uint64_t s_seg[k_seg_max], s_scan[2][k_draw_waves];
     __shared__ uint64_t s_x;
-    __shared__ int s_n, s_bin[4];
+    __shared__ int s_n, s_at, s_bin[4];
     __shared__ uint32_t s_cnt[4];
     uint32_t *const s_hist = reinterpret_cast<uint32_t *>(s_sorted);   // of counts
     static_assert(k_bins <= 2 * k_list, "");
@@ -455,13 +455,13 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
         const bool bins = !greedy && D.top_k <= k_small_k && (by_count || D.top_p < 1.0f) && scale < INFINITY;
         float ref = -INFINITY;
         auto place_of = [&](float v) {
-            return __builtin_amdgcn_fmed3f((ref - v) * scale + (float)k_head, 0.0f, (float)(k_bins - 1));
+            return __builtin_amdgcn_fmed3f(fmaf(ref - v, scale, (float)k_head), 0.0f, (float)(k_bins - 1));
         };
         auto bin_of = [&](float v) { return (int)place_of(v); };
         // By weight a token counts 2^shift at its bin's start and by the fraction of
         // its bin that it lies behind it less, as its weight does: a sum fits 32 bits,
-        // and a bin's weight is known to 2^-14 (half a unit of 2^-13, and 2^-16 for
-        // the third power's term).
+        // and a bin's weight is known to half a unit, and 2^-18 for the third power's
+        // term and the place's rounding.
         const int shift = by_count ? 0 : min(16, __clz(n));
         auto count_all = [&](const float *v) {
 #pragma unroll
@@ -585,8 +585,9 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
                 __syncthreads();
                 hi = s_bin[0];
             } else {
-                // the list: the bins in which the border lies, with 2^-13 of the sum to
-                // either side (the estimate's error twice), or 2^-16 where those are many
+                // the list: the bins in which the border may lie, by the estimates' errors
+                // (of the sum up to it and of all, half a unit and 2^-18 each), or, where
+                // those are many, those in which it does if errors mostly cancel
                 uint64_t v[4], est = 0, all;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
                 const uint64_t run = block_scan(est, s_scan[1], all) - est;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const double p = (double)D.top_p * (double)all, off = i == 0 ? 1.0 / 8192 : 1.0 / 65536;
+                    const double p = (double)D.top_p * (double)all, off = (1.0 / (1 << shift) + 1.0 / 131072) / (i == 0 ? 1 : 16);
                     first_bin(v, run, (uint64_t)fmax(p * (1 - off), 1.0), 2 * i, false);
                     first_bin(v, run, min((uint64_t)fmax(p * (1 + off), 0.0) + 1, all), 2 * i + 1, true);
                 }
@@ -696,7 +697,7 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
                     return (int)fminf((place_of(value(item)) - (float)lo) * fine, (float)(k_draw_block - 1));
                 };
                 s_sorted[tid] = 0;
-                if (tid == 0) s_n = -1, s_cnt[0] = 0;
+                if (tid == 0) s_at = -1, s_cnt[0] = 0;   // (s_n may still be read)
                 __syncthreads();
                 for (int i = tid; i < m; i += k_draw_block)
                     atomicAdd((unsigned long long *)&s_sorted[fine_bin(s_list[i])], (unsigned long long)W(value(s_list[i])));
@@ -704,11 +705,11 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
                 uint64_t part;
                 const uint64_t wf = s_sorted[tid], cf = above + block_scan(wf, s_scan[0], part);
                 if (cf - wf < want && cf >= want) {
-                    s_n = tid;
+                    s_at = tid;
                     s_x = cf - wf;
                 }
                 __syncthreads();
-                const int at = s_n;
+                const int at = s_at;
                 if (at < 0) return false;   // (the border is not in the list)
                 uint64_t before = s_x;
                 for (int i = tid; i < m; i += k_draw_block)
@@ -719,11 +720,11 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
                 for (int i0 = 0; i0 < few; i0 += k_draw_block) {
                     const uint64_t w = i0 + tid < few ? W(value(s_order[i0 + tid])) : 0;
                     const uint64_t c = before + block_scan(w, s_scan[1 - (i0 / k_draw_block & 1)], part);
-                    if (c - w < want && c >= want) s_n = i0 + tid;
+                    if (c - w < want && c >= want) s_at = i0 + tid;
                     before += part;
                 }
                 __syncthreads();
-                const uint64_t item = s_order[s_n];
+                const uint64_t item = s_order[s_at];
                 for (int i = tid; i < m; i += k_draw_block) {
                     const uint64_t w = W(value(s_list[i]));
                     if (s_list[i] >= item && w >= wmin)
