@@ -246,6 +246,33 @@ def test_bad_positions_and_pages_are_recorded(ln, what):
         assert (o[[r for r in range(7) if r not in good]] == 7.0).all()
 
 
+@pytest.mark.parametrize("T,nh,nkv,hd", [(5, 2, 1, 64), (150, 24, 16, 64)])
+def test_a_rope_table_without_positions(ln, T, nh, nkv, hd):
+    """Every row is recorded and skipped."""
+    k, v = ln.paged.alloc_pages(20, 16, nkv, hd)
+    x = torch.ones((T, nh + 2 * nkv, hd), device="cuda")
+    cs = torch.ones((1, hd // 2, 2), device="cuda")
+    table = dev(np.arange(20, dtype=np.int32)[None])
+    out = torch.full((T, nh, hd), 7.0, device="cuda")
+    index_error(ln)
+    ln.paged.rope_store_kv(x[:, :nh], x[:, nh:nh + nkv], x[:, nh + nkv:], k, v, 16, table, dev(np.int32([0, T])),
+                           dev(np.int32([T])), cs[:0], out=out)
+    assert index_error(ln)[0] == 1
+    assert (out == 7.0).all() and not k.any() and not v.any()
+
+
+def test_overlapping_rows_are_refused(ln):
+    k, v = ln.paged.alloc_pages(2, 16, 1, 32)
+    batch = (dev(np.int32([[0, 1]])), dev(np.int32([0, 3])), dev(np.int32([3])))
+    one = torch.zeros((1, 2, 32), device="cuda")
+    x = torch.zeros((3, 2, 32), device="cuda")
+    for q, out in ((one.expand(3, 2, 32), x), (x, torch.zeros((1, 2, 32), device="cuda").expand(3, 2, 32))):
+        with pytest.raises(ln.LnshipError, match="overlap"):
+            ln.paged.attention(q, k, v, 16, *batch, 1.0, out=out)
+        with pytest.raises(ln.LnshipError, match="overlap"):
+            ln.paged.rope_store_kv(q, x[:, :1], x[:, 1:], k, v, 16, *batch, None, n_dims=0, out=out)
+
+
 # ---- attention ------------------------------------------------------------------------
 
 ATTN = [
@@ -578,6 +605,37 @@ def test_captured_steps_replay_with_their_lengths(ln):
         want = step()
         for a, b in zip(have, want):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("hd,q_len,cells", [(64, 100, 16384), (64, 150, 8192), (128, 100, 8192), (128, 600, 4096)])
+def test_captured_chunks_replay_with_their_lengths(ln, hd, q_len, cells):
+    """Chunks' kernels (decoding in each workgroup, and before them all) in a captured graph."""
+    rng = np.random.default_rng(22)
+    k, v = ln.paged.alloc_pages(cells // 16, 16, 2, hd)
+    k.random_(0x3c00, 0x4200)
+    v.random_(0x3c00, 0x4200)
+    q = torch.randn((q_len, 8, hd), device="cuda")
+    table = torch.zeros((1, cells // 16), dtype=torch.int32, device="cuda")
+    start, kvl = dev(np.int32([0, q_len])), dev(np.int32([q_len]))
+
+    def inputs(n):
+        table.copy_(dev(rng.permutation(cells // 16).astype(np.int32)[None]))
+        kvl.fill_(n)
+        q.copy_(torch.randn((q_len, 8, hd), device="cuda"))
+
+    inputs(q_len)
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        with torch.cuda.graph(g, stream=s):
+            got = ln.paged.attention(q, k, v, 16, table, start, kvl, 0.1)
+    for n in (q_len + 50, 3000, q_len, q_len - 30):
+        inputs(n)
+        g.replay()
+        have = got.clone()
+        if n % 100:
+            torch.cuda.synchronize()
+        assert torch.equal(have, ln.paged.attention(q, k, v, 16, table, start, kvl, 0.1)), n
 
 
 def test_two_streams_at_once(ln):

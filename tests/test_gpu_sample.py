@@ -95,6 +95,15 @@ def test_top_p_alone(ln, vocab, kind):
     check(run(ln, x, u, None, None, p, m), x, u, None, None, p, m)
 
 
+def test_overlapping_rows_are_refused(ln):
+    x = torch.zeros((1, 50), device="cuda")
+    u = torch.zeros(3, device="cuda")
+    with pytest.raises(ln.LnshipError, match="overlap"):
+        ln.sample(x.expand(3, 50), u)
+    with pytest.raises(ln.LnshipError, match="overlap"):
+        ln.sample(torch.zeros(60, device="cuda").unfold(0, 50, 5), u)
+
+
 def test_top_k_of_more_than_weigh_anything(ln):
     """Fewer tokens within reach of the largest than top_k: top_p still cuts them."""
     x = np.full((6, 3000), -1e4, np.float32)

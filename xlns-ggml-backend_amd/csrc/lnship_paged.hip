@@ -217,7 +217,8 @@ __global__ __launch_bounds__(k_block, 8) void k_store_paged_rows(store_args s, i
     // a row's cosines and sines, once for all heads
     for (int i = tid * 4; i < rows * nd; i += k_block * 4) {
         const int r = (int)((uint32_t)i / (uint32_t)nd);
-        const float4 u = *reinterpret_cast<const float4 *>(a.cos_sin + (int64_t)max(s_pos[r], 0) * nd + (i - r * nd));
+        if (s_pos[r] < 0) continue;
+        const float4 u = *reinterpret_cast<const float4 *>(a.cos_sin + (int64_t)s_pos[r] * nd + (i - r * nd));
         const float w[4] = {u.x, u.y, u.z, u.w};
         uint32_t z[4];
 #pragma unroll
@@ -1132,7 +1133,7 @@ static int check_paged(const lnship_paged_kv *kv, bool ptrs) {
     if (kv->head_dim < 8 || kv->head_dim > 256 || kv->head_dim % 8)
         return fail(LNSHIP_EINVAL, "paged cache: head_dim not a multiple of 8 up to 256%s");
     // (a grid's threads along x are counted in 32 bits)
-    if (kv->ntok > 0xffffff || kv->n_seq > 0x7fffff || kv->n_head_kv > 65535 || kv->n_pages > 0x7fffffff ||
+    if (kv->ntok > 0xfffff0 || kv->n_seq > 0x7fffff || kv->n_head_kv > 65535 || kv->n_pages > 0x7fffffff ||
         kv->table_ld > 0x3fffffff / kv->page)
         return fail(LNSHIP_ERANGE, "paged cache: too large%s");
     if (ptrs && kv->ntok && kv->n_seq) {
@@ -1271,7 +1272,7 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
     if (nq > 0x7fffffff || a->q_ld < (a->n_head ? nq : 0) || a->k_ld < nk || a->v_ld < nk || s.a.q_dst_ld < nq || a->n_pos < 0)
         return fail(LNSHIP_EINVAL, "rope_store_kv_paged: bad shape%s");
     if (kv->ntok == 0 || kv->n_seq == 0) return 0;
-    if (!a->k || !a->v || (a->n_head && (!a->q || !a->q_dst)) || (a->rope_n_dims && !a->cos_sin))
+    if (!a->k || !a->v || (a->n_head && (!a->q || !a->q_dst)) || (a->rope_n_dims && a->n_pos && !a->cos_sin))
         return fail(LNSHIP_EINVAL, "rope_store_kv_paged: null pointer%s");
     device_state *st = state();
     if (!st) return LNSHIP_ENOINIT;
@@ -1281,7 +1282,7 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
                      ((a->q_ld | a->k_ld | s.a.q_dst_ld) & 3) == 0;
     // (its tables take 4 us to lay out: 64 rows of 32 heads of 128 on 8 6.7 us without,
     // 8.4 so, 128 rows 9.6 and 8.6; 128 of 9 heads of 64 on 3 4.9 and 8.3)
-    if (vec && kv->ntok * (nq + 2 * nk) >= 1 << 19) {
+    if (vec && nq <= 1 << 26 && kv->ntok * (nq + 2 * nk) >= 1 << 19) {
         // Eight rows of a prompt together, as their cells share cache lines (8 prompts
         // of 511 to 2047 tokens, 32 heads of 64 on 8: 77 us, by single rows 85); single
         // tokens' rows, and few, by themselves (4096 sequences' tokens, heads of 128: 75,

@@ -512,6 +512,8 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=
     if logits.dtype != f32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise LnshipError("sample: logits must be float32 [n_rows, n_vocab], a row's values together")
     rows, vocab = logits.shape
+    if rows > 1 and logits.stride(0) < vocab:
+        raise LnshipError("sample: rows of logits must not overlap")
     tokens, probs = out if out is not None else (torch.empty(rows, dtype=i32, device=logits.device),
                                                  torch.empty(rows, dtype=f32, device=logits.device))
     need = lib().lnship_sample_work(rows, vocab)

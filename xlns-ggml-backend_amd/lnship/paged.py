@@ -57,6 +57,8 @@ def _ld(t, name, ntok, heads, dim, dev):
     s0, s1, s2 = t.stride()
     if s2 != 1 or (s1 != dim and heads > 1):
         _no(name + ": a row's heads must lie behind each other")
+    if ntok > 1 and s0 < heads * dim:
+        _no(name + ": rows must not overlap")
     return s0 if ntok > 1 else max(s0, heads * dim)
 
 
