@@ -720,30 +720,30 @@ struct tile_maker {
     const int32_t *table;
     const uint16_t *kbase, *vbase;
     int64_t page_codes;
-    int cend, page_sh, page, hd, n_pages;
+    int cend, page_sh, page, hd, n_pages, tid;
     unsigned long long *err;
     uint4 kc[UT], vc[UT];
     int kid, vid[UT];   // the pages of the next units to load
 
-    __device__ __forceinline__ tile_maker(const lnship_paged_kv &kv, int sq, int kvh, int sh, int end, unsigned long long *e)
+    __device__ __forceinline__ tile_maker(const lnship_paged_kv &kv, int sq, int kvh, int sh, int end, int thread,
+                                          unsigned long long *e)
         : table(kv.table + (int64_t)sq * kv.table_ld), cend(end), page_sh(sh), page((int)kv.page), hd((int)kv.head_dim),
-          n_pages((int)kv.n_pages), err(e) {
+          n_pages((int)kv.n_pages), tid(thread), err(e) {
         const int64_t head_codes = (int64_t)page * hd;
         page_codes = kv.n_head_kv * head_codes;
         kbase = kv.k_pages + kvh * head_codes;
         vbase = kv.v_pages + kvh * head_codes;
     }
-    __device__ __forceinline__ bool has(int i) const { return (i + 1) * NT <= U || (int)threadIdx.x + i * NT < U; }
+    __device__ __forceinline__ bool has(int i) const { return (i + 1) * NT <= U || tid + i * NT < U; }
     // the page of cell c (of hidden cells: another's, whatever it holds is finite)
     __device__ __forceinline__ int page_of(int c) const { return table[min(c, cend - 1) >> page_sh]; }
     __device__ __forceinline__ bool sound(int id) const { return (uint32_t)id < (uint32_t)n_pages; }
     __device__ __forceinline__ void pages(int cb) {
-        kid = page_of(cb + (threadIdx.x & 63));
+        kid = page_of(cb + (tid & 63));
 #pragma unroll
-        for (int i = 0; i < UT; i++) vid[i] = page_of(cb + ((int)threadIdx.x + i * NT) / HD * 8);
+        for (int i = 0; i < UT; i++) vid[i] = page_of(cb + (tid + i * NT) / HD * 8);
     }
     __device__ __forceinline__ void load(int cb) {
-        const int tid = threadIdx.x;
         const uint16_t *k = kbase + (sound(kid) ? kid : 0) * page_codes + ((cb + (tid & 63)) & (page - 1)) * 8;
 #pragma unroll
         for (int i = 0; i < UT; i++) {
@@ -764,7 +764,7 @@ struct tile_maker {
         uint32_t ok = 0;
 #pragma unroll
         for (int i = 0; i < UT; i++) {
-            const bool in = has(i) && cb + ((int)threadIdx.x + i * NT) / HD * 8 < cend;
+            const bool in = has(i) && cb + (tid + i * NT) / HD * 8 < cend;
             if (in && sound(vid[i])) ok |= 1u << i;
             else if (in) index_fault(err, vid[i]);
         }
@@ -772,7 +772,6 @@ struct tile_maker {
     }
     // decodes the loaded codes into the tile s; its groups of eight cells' flags into oks
     __device__ __forceinline__ void store(uint4 *s, uint32_t ok, uint8_t *oks) const {
-        const int tid = threadIdx.x;
         // the cell's row of its block's key product: a lane's 16 results are
         // then cells 8 h + 0..7 and 16 + 8 h + 0..7 of the block
         const int cell = tid & 63, in = cell & 31;
@@ -799,6 +798,24 @@ struct tile_maker {
             if (oks && d == 0) oks[c8] = ok >> i & 1;
         }
     }
+    // The same for the tiles [cb, cend), one behind the other: loads the first and
+    // decodes it, then each next one, its loads ahead of the one before's decoding.
+    uint32_t ok_next;
+    __device__ __forceinline__ void first(int cb, uint4 *s, uint8_t *oks) {
+        if (cb >= cend) return;
+        pages(cb);
+        load(cb);
+        ok_next = sound_pages(cb);
+        pages(cb + 64);
+        next(cb, s, oks);
+    }
+    __device__ __forceinline__ void next(int cb, uint4 *s, uint8_t *oks) {
+        if (cb >= cend) return;
+        store(s, ok_next, oks);
+        load(cb + 64);   // (past the last tile: other cells of a page, not used)
+        ok_next = sound_pages(cb + 64);
+        pages(cb + 128);
+    }
 };
 
 // The cells that chunks see, decoded into the workspace, for k_attn_tiles to
@@ -815,7 +832,7 @@ __global__ __launch_bounds__(256) void k_attn_decode(attn_paged_args a, unsigned
         // the first cell that the sequence's first token sees
         const int64_t first = kv.kv_len[sq] - (end - start) - a.window + 1;
         const int lo = a.window > 0 ? (int)(min(max(first, (int64_t)0), (int64_t)cend) >> 6) : 0;
-        tile_maker<NB, 256> t(kv, sq, kvh, a.page_sh, cend, err);
+        tile_maker<NB, 256> t(kv, sq, kvh, a.page_sh, cend, threadIdx.x, err);
         for (int i = lo + (int)blockIdx.x; i * 64 < cend; i += (int)gridDim.x) {
             t.pages(i * 64);
             t.load(i * 64);
@@ -1026,35 +1043,52 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     const row_tile T = find_tile(a, tile, err);
     if (T.r0 < 0 || (split > 0 && split * T.per >= T.blocks)) return;
     const int cbeg = T.c0 + split * T.per * 64, cend = min(T.c1, cbeg + T.per * 64);
-    tile_maker<NB, NW * 64> maker(a.kv, T.sq, kvh, a.page_sh, cend, err);
-    uint32_t ok_next = 0;
-    auto prepare = [&](int cb, int buf) {   // the tile at cb into buf, the loads of the one behind it
-        if (cb >= cend) return;
-        maker.store(s_cells + buf * 4 * U, ok_next, s_ok[buf]);
-        maker.load(cb + 64);   // (past the last tile: other cells of a page, not used)
-        ok_next = maker.sound_pages(cb + 64);
-        maker.pages(cb + 128);
-    };
-    if (cbeg < cend) {
-        maker.pages(cbeg);
-        maker.load(cbeg);
-        ok_next = maker.sound_pages(cbeg);
-        maker.pages(cbeg + 64);
-        prepare(cbeg, 0);
-    }
+    const int tid = threadIdx.x;
+    auto cells = [&](int buf) { return s_cells + buf * 4 * U; };
     chunk_rows<NB> r;
+    auto blocks = [&](int cb, int buf) {
+#pragma unroll 1
+        for (int blk = 0; blk < 2; blk++) {
+            const uint32_t ok = (uint32_t)__builtin_amdgcn_readfirstlane(
+                (int)*reinterpret_cast<const uint32_t *>(&s_ok[buf][blk * 4]));
+            r.block(cells(buf) + blk * 2 * U, cb + blk * 32, ok, T.c1);
+        }
+    };
+    if (NW == 8 && T.rows - T.r0 <= NW * 16) {
+        // Rows for half of the waves: the others decode meanwhile.  (33 sequences of 6
+        // to 27 tokens behind 640 to 5125 cells, 32 heads of 128 on 8: 249 us, all waves
+        // decoding 284.)
+        if (wave >= NW / 2) {
+            tile_maker<NB, NW * 32> maker(a.kv, T.sq, kvh, a.page_sh, cend, tid - NW * 32, err);
+            maker.first(cbeg, cells(0), s_ok[0]);
+            lds_barrier();
+            int buf = 0;
+            for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
+                maker.next(cb + 64, cells(buf ^ 1), s_ok[buf ^ 1]);
+                lds_barrier();
+            }
+            return;
+        }
+        r.place(a, T, kvh, T.r0 + wave * 32);
+        r.load(a);
+        lds_barrier();
+        int buf = 0;
+        for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
+            blocks(cb, buf);
+            lds_barrier();
+        }
+        r.write(a, T, split);
+        return;
+    }
+    tile_maker<NB, NW * 64> maker(a.kv, T.sq, kvh, a.page_sh, cend, tid, err);
+    maker.first(cbeg, cells(0), s_ok[0]);
     r.place(a, T, kvh, T.r0 + wave * 32);
     r.load(a);
     lds_barrier();
     int buf = 0;
     for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
-#pragma unroll 1
-        for (int blk = 0; blk < 2; blk++) {
-            const uint32_t ok = (uint32_t)__builtin_amdgcn_readfirstlane(
-                (int)*reinterpret_cast<const uint32_t *>(&s_ok[buf][blk * 4]));
-            r.block(s_cells + buf * 4 * U + blk * 2 * U, cb + blk * 32, ok, T.c1);
-        }
-        prepare(cb + 64, buf ^ 1);
+        blocks(cb, buf);
+        maker.next(cb + 64, cells(buf ^ 1), s_ok[buf ^ 1]);
         lds_barrier();
     }
     r.write(a, T, split);
