@@ -425,13 +425,14 @@ __device__ __forceinline__ row_tile find_tile(const attn_paged_args &a, int tile
     auto first_tile = [&](int i) { return (int)((uint32_t)min(max(kv.q_start[i], 0), (int)kv.ntok) * rep / R) + i; };
     row_tile t;
     t.sq = wave_last_at_most((int)kv.n_seq, tile, first_tile);
-    t.t0 = min(max(kv.q_start[t.sq], 0), (int)kv.ntok);
+    const int start = kv.q_start[t.sq], len = kv.kv_len[t.sq];   // (all loads before the first wait)
     const int64_t end = kv.q_start[t.sq + 1];
+    t.t0 = min(max(start, 0), (int)kv.ntok);
     t.rows = (int)max(min(end, kv.ntok) - t.t0, (int64_t)0) * a.rep;
     t.r0 = (tile - first_tile(t.sq)) * a.tile_rows;
     if (t.r0 >= t.rows) t.r0 = -1;
     if (t.r0 < 0) return t;
-    const int64_t pos0 = max((int64_t)kv.kv_len[t.sq] - end + t.t0, -((int64_t)1 << 30));
+    const int64_t pos0 = max((int64_t)len - end + t.t0, -((int64_t)1 << 30));
     const int last = (int)((uint32_t)(min(t.r0 + a.tile_rows, t.rows) - 1) / rep), first = (int)((uint32_t)t.r0 / rep);
     const int64_t cells = kv.table_ld << a.page_sh;
     if (err && pos0 + last >= cells && threadIdx.x == 0) index_fault(err, pos0 + last);
@@ -1107,11 +1108,16 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(attn_paged_args a) {
     const int64_t rows = a.kv.ntok * a.n_head;
     const int64_t row = W == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     const int64_t tok = row / a.n_head;
+    const int at = W == 4 ? tid : lane;
+    // (what no part has written is loaded too, beside what says so, and not used;
+    // an unsound q_start may leave rows out)
+    const int64_t own = min(row, rows - 1);
+    const float2 part = a.stats[min(at, a.splits - 1) * rows + own];
+    const int parts = a.used[own];
     const bool in = row < rows && tok >= a.kv.q_start[0] && tok < a.kv.q_start[a.kv.n_seq];
     if (W == 4 && !in) return;
-    const int used = in ? max(1, min(a.used[row], a.splits)) : 0;   // (an unsound q_start may leave rows out)
-    const int at = W == 4 ? tid : lane;
-    const float2 st = at < used ? a.stats[at * rows + row] : make_float2(-INFINITY, 0.0f);
+    const int used = in ? max(1, min(parts, a.splits)) : 0;
+    const float2 st = at < used ? part : make_float2(-INFINITY, 0.0f);
     auto reduce = [&](float v, bool sum) {
         for (int d = 32; d; d >>= 1) {
             const float y = __shfl_xor(v, d);
