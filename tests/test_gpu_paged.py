@@ -294,6 +294,10 @@ ATTN = [
     ([257], [257], 64, 8, 2, 128, 129),
     ([300], [300], 16, 9, 3, 64, 0),
     ([520, 1, 90], [800, 50, 90], 32, 8, 2, 64, 0),
+    # more workgroups than CUs: four waves each
+    ([1] * 40, [1 + 37 * i for i in range(40)], 16, 32, 8, 64, 0),
+    ([1] * 40, [1 + 31 * i for i in range(40)], 64, 8, 8, 72, 0),
+    ([1] * 40, [2 + 29 * i for i in range(40)], 32, 16, 8, 128, 300),
 ]
 
 

@@ -478,8 +478,8 @@ __device__ __forceinline__ void load_q(const float *q, int d, int hd, bool vec, 
 }
 
 // Few rows a sequence (single tokens): a wave takes 16 rows and, of their
-// split's cells, every fourth block of 32; the four waves of a workgroup are
-// joined at the end.  Scores are formed transposed, S^T = K Q^T, with the cells
+// split's cells, every NW-th block of 32; the waves of a workgroup are joined at
+// the end.  Scores are formed transposed, S^T = K Q^T, with the cells
 // dealt to the rows of two 16 x 16 products so that a lane's eight scores are
 // eight neighbouring cells of one row: as such they are the operand of
 // O^T = V^T P^T, and both caches' layouts give a lane's share of K and V in
@@ -487,15 +487,17 @@ __device__ __forceinline__ void load_q(const float *q, int d, int hd, bool vec, 
 // this one's weights are formed, its values once this one's are decoded.
 // Bound by HBM where the cache is long: 64 sequences of 100 to 8000 cells, 32 heads of
 // 128 on 8, in 300 us, 3.7 TB/s of keys and values (a sum over memory reads 4.0); one of
-// 131072 cells in 125 us, 4.2 TB/s.  300 cells of 9 heads of 64 on 3 take 10.7 us: the
+// 131072 cells in 125 us, 4.2 TB/s.  300 cells of 9 heads of 64 on 3 take 9.4 us: the
 // loads of lengths, pages, keys and values wait for each other.
-template <int NB, bool FULL>   // 32-wide groups of head_dim; whether it fills them
-__global__ __launch_bounds__(256, NB <= 4 ? 3 : 1) void k_attn_paged(attn_paged_args a, unsigned long long *err) {
+template <int NB, bool FULL, int NW>   // 32-wide groups of head_dim; whether it fills them; waves
+__global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : NB <= 4 ? 3 : 1) void k_attn_paged(attn_paged_args a, unsigned long long *err) {
     const lnship_paged_kv &kv = a.kv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int rep = a.rep, kvh = blockIdx.y, split = blockIdx.z, hd = (int)kv.head_dim, page = (int)kv.page;
-    __shared__ float s_m[4][16], s_l[4][16], s_qs[16];
-    __shared__ float s_o[16][NB * 32 + 1];
+    constexpr int step = NW * 32;
+    constexpr int slots = NB <= 2 ? NW : NB <= 4 ? 4 : 2;   // waves that put their sums into LDS at once
+    __shared__ float s_m[NW][16], s_l[NW][16], s_qs[16];
+    __shared__ float s_o[slots][16][NB * 32 + 1];
     __shared__ uint4 s_q[2][NB][64];   // the queries' split halves, as the products' operands
 
     const row_tile T = find_tile(a, blockIdx.x, err);
@@ -558,10 +560,10 @@ __global__ __launch_bounds__(256, NB <= 4 ? 3 : 1) void k_attn_paged(attn_paged_
         kid = page_of(cb + kcell);
         vid = page_of(cb + vcell);
         load_k(cb, kid);
-        kid = page_of(cb + 128 + kcell);
+        kid = page_of(cb + step + kcell);
         sound_v(cb);
         load_v(cb, vid);
-        vid = page_of(cb + 128 + vcell);
+        vid = page_of(cb + step + vcell);
     }
     // the queries as halves, scaled by the row's largest to at most 2: by the
     // first wave, for all
@@ -592,7 +594,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 3 : 1) void k_attn_paged(attn_paged_
     }
     __syncthreads();
     const float qs = s_qs[n];
-    for (; cb < cend; cb += 128) {
+    for (; cb < cend; cb += step) {
         float4v sh[2], sx[2];
         sh[0] = sh[1] = sx[0] = sx[1] = float4v{0, 0, 0, 0};
 #pragma unroll
@@ -609,8 +611,8 @@ __global__ __launch_bounds__(256, NB <= 4 ? 3 : 1) void k_attn_paged(attn_paged_
                 sx[t] = mma(kh, ql, sx[t]);
             }
         }
-        load_k(cb + 128, kid);
-        kid = page_of(cb + 256 + kcell);
+        load_k(cb + step, kid);
+        kid = page_of(cb + 2 * step + kcell);
         float s[8], mb = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -646,9 +648,9 @@ __global__ __launch_bounds__(256, NB <= 4 ? 3 : 1) void k_attn_paged(attn_paged_
             o[i] = mma(vh, pl, o[i]);
             o[i] = mma(vl, pc, o[i]);
         }
-        sound_v(cb + 128);
-        load_v(cb + 128, vid);
-        vid = page_of(cb + 256 + vcell);
+        sound_v(cb + step);
+        load_v(cb + step, vid);
+        vid = page_of(cb + 2 * step + vcell);
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -659,32 +661,40 @@ __global__ __launch_bounds__(256, NB <= 4 ? 3 : 1) void k_attn_paged(attn_paged_
         s_l[wave][n] = l;
     }
     __syncthreads();
-    const float M = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
+    float M = s_m[0][n];
+#pragma unroll
+    for (int w = 1; w < NW; w++) M = fmaxf(M, s_m[w][n]);
     const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-    for (int w = 0; w < 4; w++) {
-        if (wave == w) {
+    for (int w = 0; w < NW; w += slots) {
+        if (wave >= w && wave < w + slots) {
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    float &x = s_o[n][i * 16 + g * 4 + j];
+                    float &x = s_o[wave - w][n][i * 16 + g * 4 + j];
                     x = (w ? x : 0.0f) + o[i][j] * f;
                 }
         }
         __syncthreads();
     }
-    // a row's elements, on 16 threads
-    const int rr = threadIdx.x >> 4, row2 = T.r0 + rr;
+    // a row's elements, on as many threads as there are for a row
+    constexpr int of = NW * 4;
+    const int rr = threadIdx.x / of, row2 = T.r0 + rr;
     if (row2 >= T.rows) return;
     const int tok2 = T.t0 + (int)((uint32_t)row2 / (uint32_t)rep), head2 = kvh * rep + (int)((uint32_t)row2 % (uint32_t)rep);
     float M2 = -INFINITY, L2 = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; w++) M2 = fmaxf(M2, s_m[w][rr]);
+    for (int w = 0; w < NW; w++) M2 = fmaxf(M2, s_m[w][rr]);
     if (M2 != -INFINITY)
 #pragma unroll
-        for (int w = 0; w < 4; w++) L2 += s_l[w][rr] * __builtin_amdgcn_exp2f(s_m[w][rr] - M2);
-    const row_out out = out_row(a, T, split, tok2, head2, M2, L2, (threadIdx.x & 15) == 0);
-    for (int d = threadIdx.x & 15; d < hd; d += 16) out.dst[d] = s_o[rr][d] * out.f;
+        for (int w = 0; w < NW; w++) L2 += s_l[w][rr] * __builtin_amdgcn_exp2f(s_m[w][rr] - M2);
+    const row_out out = out_row(a, T, split, tok2, head2, M2, L2, threadIdx.x % of == 0);
+    for (int d = threadIdx.x % of; d < hd; d += of) {
+        float x = s_o[0][rr][d];
+#pragma unroll
+        for (int w = 1; w < slots; w++) x += s_o[w][rr][d];
+        out.dst[d] = x * out.f;
+    }
 }
 
 // A barrier that waits for LDS alone: loads from memory stay in flight; and one
@@ -1217,7 +1227,7 @@ constexpr int k_decode_rows = 512;
 constexpr int64_t k_pre_bytes = (int64_t)1 << 30;   // of the workspace for decoded cells, at most
 // Waves of a workgroup.  Up to 64 dims four: three or four workgroups share a CU,
 // and uneven sequences leave smaller last tiles (a batch of 9 conversations of
-// 20 to 160 tokens 37 us, with eight waves 45).  Above, eight, which copy or decode a
+// 5 to 301 tokens 37 us, with eight waves 45).  Above, eight, which copy or decode a
 // cell once for 256 rows (one sequence of 4096 tokens, 32 heads of 128: 1043 us, with four
 // 1141) but where decoded cells meet less than 2048 rows a sequence (8 sequences of
 // 128 tokens over 2000 cells: 178, with four 157).
@@ -1290,8 +1300,18 @@ static int launch_attn(const attn_paged_args &m, const attn_plan &p, int cus, hi
         if (p.waves) return launch_chunk<NB, NB <= 2 ? 4 : 8>(m, chunks, s, err);
     }
     const dim3 grid((unsigned)p.tiles, (unsigned)m.kv.n_head_kv, (unsigned)p.splits);
-    if (m.kv.head_dim == NB * 32) hipLaunchKernelGGL((k_attn_paged<NB, true>), grid, dim3(256), 0, s, m, err);
-    else hipLaunchKernelGGL((k_attn_paged<NB, false>), grid, dim3(256), 0, s, m, err);
+    // A CU for each workgroup: eight waves, which go over their cells in half the steps
+    // (448 cells of 9 heads of 64 on 3 11.0 us, with four 12.0 and sixteen 12.3; 32 heads of
+    // 128 on 8 17.5 and 19.3; 64 sequences of 2000 cells of those 167 with eight, 130 with four).
+    if constexpr (NB <= 4)
+        if (p.tiles * m.kv.n_head_kv * p.splits <= cus) {
+            if (m.kv.head_dim == NB * 32) hipLaunchKernelGGL((k_attn_paged<NB, true, 8>), grid, dim3(512), 0, s, m, err);
+            else hipLaunchKernelGGL((k_attn_paged<NB, false, 8>), grid, dim3(512), 0, s, m, err);
+            LNSHIP_HIP(hipGetLastError());
+            return 0;
+        }
+    if (m.kv.head_dim == NB * 32) hipLaunchKernelGGL((k_attn_paged<NB, true, 4>), grid, dim3(256), 0, s, m, err);
+    else hipLaunchKernelGGL((k_attn_paged<NB, false, 4>), grid, dim3(256), 0, s, m, err);
     LNSHIP_HIP(hipGetLastError());
     return 0;
 }
