@@ -477,8 +477,7 @@ int64_t lnship16_attn_paged_work(const lnship_paged_kv *kv, int64_t n_head);
  * of additions; a weight is exact to 2^-32.  n_vocab up to 2^19.  A row whose
  * top_k is above 1024, or with thousands of equal logits at a limit, takes
  * several times as long as another.  No LNS arithmetic, and no counterpart in
- * the reference, which samples on the host.
- * work: lnship_sample_work bytes, as in lnship_paged_attn_args. */
+ * the reference, which samples on the host. */
 typedef struct lnship_sample_args {
     const float *logits;
     int64_t ld, n_rows, n_vocab;   /* ld 0: n_vocab */
@@ -487,11 +486,8 @@ typedef struct lnship_sample_args {
     const float *top_p, *min_p, *u;
     int32_t *tokens;
     float *probs;
-    void *work;
-    size_t work_bytes;
 } lnship_sample_args;
 int lnship_sample(const lnship_sample_args *a, void *stream);
-int64_t lnship_sample_work(int64_t n_rows, int64_t n_vocab);
 
 /* ggml views on the device (tensors in the ggml device buffer type): the
  * elements of a 4-D strided view (byte strides nb, as ggml_tensor::nb)

@@ -35,7 +35,7 @@ def attn(kv=None, **kw):
 
 def draw(**kw):
     a = dict(logits=P, ld=0, n_rows=2, n_vocab=100, temperature=None, top_k=None, top_p=None, min_p=None, u=P, tokens=P,
-             probs=None, work=P, work_bytes=1 << 40)
+             probs=None)
     a.update(kw)
     s = lnship.SampleArgs(*(a[f[0]] for f in lnship.SampleArgs._fields_))
     return lnship.lib().lnship_sample(ctypes.byref(s), None)
@@ -101,15 +101,13 @@ def test_empty_calls_need_no_pointers():
         kv = paged(**none, **e)
         assert store(kv, q=None, k=None, v=None, q_dst=None, cos_sin=None) == 0
         assert attn(kv, q=None, dst=None, work=None, work_bytes=0) == 0
-    assert draw(n_rows=0, logits=None, u=None, tokens=None, work=None, work_bytes=0) == 0
+    assert draw(n_rows=0, logits=None, u=None, tokens=None) == 0
 
 
 def test_workspace_sizes():
     L = lnship.lib()
     assert L.lnship16_attn_paged_work(ctypes.byref(paged(page=8)), 8) == EINVAL
     assert L.lnship16_attn_paged_work(ctypes.byref(paged()), 7) == EINVAL
-    assert L.lnship_sample_work(-1, 5) == EINVAL and L.lnship_sample_work(1, 1 << 20) == ERANGE
-    assert L.lnship_sample_work(4, 50000) >= 0
 
 
 def test_tensors_that_are_not_on_the_gpu_are_refused():

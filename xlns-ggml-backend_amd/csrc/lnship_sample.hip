@@ -792,22 +792,14 @@ using namespace lnship;
 
 extern "C" {
 
-int64_t lnship_sample_work(int64_t n_rows, int64_t n_vocab) {
-    if (n_rows < 0 || n_vocab < 0) return fail(LNSHIP_EINVAL, "sample: bad shape%s");
-    if (n_rows > 0x3fffff || n_vocab > k_draw_vocab) return fail(LNSHIP_ERANGE, "sample: too large%s");
-    return 0;
-}
-
 int lnship_sample(const lnship_sample_args *a, void *stream) {
     if (!a) return fail(LNSHIP_EINVAL, "sample: null arguments%s");
-    const int64_t need = lnship_sample_work(a->n_rows, a->n_vocab);
-    if (need < 0) return (int)need;
+    if (a->n_rows < 0 || a->n_vocab < 1) return fail(LNSHIP_EINVAL, "sample: bad shape%s");
+    if (a->n_rows > 0x3fffff || a->n_vocab > k_draw_vocab) return fail(LNSHIP_ERANGE, "sample: too large%s");
     const int64_t ld = a->ld ? a->ld : a->n_vocab;
-    if (a->n_vocab < 1 || ld < a->n_vocab) return fail(LNSHIP_EINVAL, "sample: bad shape%s");
+    if (ld < a->n_vocab) return fail(LNSHIP_EINVAL, "sample: bad shape%s");
     if (a->n_rows == 0) return 0;
     if (!a->logits || !a->u || !a->tokens) return fail(LNSHIP_EINVAL, "sample: null pointer%s");
-    if (need && (!a->work || a->work_bytes < (size_t)need || ((uintptr_t)a->work & 15)))
-        return fail(LNSHIP_EINVAL, "sample: work smaller than lnship_sample_work or not aligned%s");
     device_state *s = state();
     if (!s) return LNSHIP_ENOINIT;
     draw_args d{a->logits, ld, (int)a->n_vocab, a->temperature, a->top_k, a->top_p, a->min_p, a->u, a->tokens, a->probs};

@@ -85,8 +85,7 @@ class PagedAttnArgs(ctypes.Structure):
 
 class SampleArgs(ctypes.Structure):
     _fields_ = [("logits", c_p), ("ld", c_i64), ("n_rows", c_i64), ("n_vocab", c_i64), ("temperature", c_p),
-                ("top_k", c_p), ("top_p", c_p), ("min_p", c_p), ("u", c_p), ("tokens", c_p), ("probs", c_p),
-                ("work", c_p), ("work_bytes", ctypes.c_size_t)]
+                ("top_k", c_p), ("top_p", c_p), ("min_p", c_p), ("u", c_p), ("tokens", c_p), ("probs", c_p)]
 
 
 def attn_seqs(n_seq, seeds=(0, 0, 0)):
@@ -198,7 +197,6 @@ def lib():
         "lnship16_attn_paged": (ctypes.c_int, [ctypes.POINTER(PagedKV), ctypes.POINTER(PagedAttnArgs), c_p]),
         "lnship16_attn_paged_work": (c_i64, [ctypes.POINTER(PagedKV), c_i64]),
         "lnship_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), c_p]),
-        "lnship_sample_work": (c_i64, [c_i64, c_i64]),
         "lnship_causal_mask": (ctypes.c_int, [c_p, c_i64, c_i64, c_p, c_p]),
         "lnship_rope_table": (ctypes.c_int, [ctypes.c_float, ctypes.c_int, c_i64, c_p]),
     }
@@ -516,14 +514,10 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=
         raise LnshipError("sample: rows of logits must not overlap")
     tokens, probs = out if out is not None else (torch.empty(rows, dtype=i32, device=logits.device),
                                                  torch.empty(rows, dtype=f32, device=logits.device))
-    need = lib().lnship_sample_work(rows, vocab)
-    if need < 0:
-        check(need)
-    work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
     a = SampleArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
                    _row_values(temperature, rows, f32, "temperature", dev), _row_values(top_k, rows, i32, "top_k", dev),
                    _row_values(top_p, rows, f32, "top_p", dev), _row_values(min_p, rows, f32, "min_p", dev),
                    _row_values(u, rows, f32, "u", dev), _row_values(tokens, rows, i32, "tokens", dev),
-                   _row_values(probs, rows, f32, "probs", dev), _p(work), need)
+                   _row_values(probs, rows, f32, "probs", dev))
     check(lib().lnship_sample(byref(a), stream))
     return tokens, probs
