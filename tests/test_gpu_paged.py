@@ -373,6 +373,7 @@ def test_chunks_behind_a_table_of_many_pages(ln, q_len, kv_len, page, nh, nkv, h
     ([40, 90], [300, 90], 16, 4, 4, 24, 50), ([520, 1, 90], [800, 50, 90], 32, 8, 2, 64, 0), ([65], [65], 256, 2, 2, 8, 0),
     ([600], [900], 16, 1, 1, 32, 0), ([130, 3], [170, 9], 64, 18, 2, 128, 0), ([257], [300], 16, 28, 4, 80, 0),
     ([300, 1, 0, 180], [310, 5, 7, 900], 128, 32, 4, 96, 0), ([520], [530], 64, 8, 2, 128, 129), ([333], [999], 32, 3, 1, 64, 31),
+    ([65, 120], [66, 300], 16, 16, 8, 128, 0), ([64, 90, 130], [64, 900, 131], 32, 8, 2, 96, 77), ([75], [333], 64, 4, 1, 112, 0),
     ([1030], [1050], 16, 4, 2, 72, 0), ([519], [700], 32, 8, 2, 104, 0), ([2050], [2050], 64, 2, 2, 128, 700)])
 def test_chunks_behind_wide_tables(ln, q_len, kv_len, page, nh, nkv, hd, window):
     print(f"\n[attn] {q_len} {kv_len} page {page} {nh}/{nkv}x{hd} window {window}, wide", flush=True)

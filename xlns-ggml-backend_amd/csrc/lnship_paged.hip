@@ -723,11 +723,11 @@ struct tile_of {
 
 // A workgroup of NT threads that makes such tiles of the cells [.., cend) of one
 // sequence: a thread loads its units' codes ahead, then decodes them.  Unit u of
-// the keys: dims u / 64 * 8.., cell u % 64 of the tile (the same for all of a
+// the keys: dims u / C * 8.., cell u % C of the tile's C (the same for all of a
 // thread's); of the values: cells u / HD * 8.., dim u % HD.
-template <int NB, int NT>
+template <int NB, int NT, int C = 64>
 struct tile_maker {
-    static constexpr int HD = tile_of<NB>::HD, B = tile_of<NB>::B, U = 2 * B, UT = (U + NT - 1) / NT;
+    static constexpr int HD = tile_of<NB>::HD, B = tile_of<NB>::B, U = C / 32 * B, UT = (U + NT - 1) / NT;
     const int32_t *table;
     const uint16_t *kbase, *vbase;
     int64_t page_codes;
@@ -750,15 +750,15 @@ struct tile_maker {
     __device__ __forceinline__ int page_of(int c) const { return table[min(c, cend - 1) >> page_sh]; }
     __device__ __forceinline__ bool sound(int id) const { return (uint32_t)id < (uint32_t)n_pages; }
     __device__ __forceinline__ void pages(int cb) {
-        kid = page_of(cb + (tid & 63));
+        kid = page_of(cb + (tid & (C - 1)));
 #pragma unroll
         for (int i = 0; i < UT; i++) vid[i] = page_of(cb + (tid + i * NT) / HD * 8);
     }
     __device__ __forceinline__ void load(int cb) {
-        const uint16_t *k = kbase + (sound(kid) ? kid : 0) * page_codes + ((cb + (tid & 63)) & (page - 1)) * 8;
+        const uint16_t *k = kbase + (sound(kid) ? kid : 0) * page_codes + ((cb + (tid & (C - 1))) & (page - 1)) * 8;
 #pragma unroll
         for (int i = 0; i < UT; i++) {
-            const int d8 = (tid + i * NT) >> 6;
+            const int d8 = (tid + i * NT) / C;
             kc[i] = *reinterpret_cast<const uint4 *>(k + min(d8, hd / 8 - 1) * page * 8);
         }
 #pragma unroll
@@ -785,14 +785,14 @@ struct tile_maker {
     __device__ __forceinline__ void store(uint4 *s, uint32_t ok, uint8_t *oks) const {
         // the cell's row of its block's key product: a lane's 16 results are
         // then cells 8 h + 0..7 and 16 + 8 h + 0..7 of the block
-        const int cell = tid & 63, in = cell & 31;
+        const int cell = tid & (C - 1), in = cell & 31;
         const int row = 8 * ((in >> 4) * 2 + ((in >> 2) & 1)) + 4 * ((in >> 3) & 1) + (in & 3);
 #pragma unroll
         for (int i = 0; i < UT; i++) {
             frag hi, lo;
             decode8(kc[i], hi, lo);
             if (!has(i)) continue;
-            const int d8 = (tid + i * NT) >> 6;
+            const int d8 = (tid + i * NT) / C;
             uint4 *to = s + (cell >> 5) * 4 * B + (d8 >> 1) * 64 + (d8 & 1) * 32 + row;
             to[0] = hi.w;
             to[B] = lo.w;
@@ -817,15 +817,15 @@ struct tile_maker {
         pages(cb);
         load(cb);
         ok_next = sound_pages(cb);
-        pages(cb + 64);
+        pages(cb + C);
         next(cb, s, oks);
     }
     __device__ __forceinline__ void next(int cb, uint4 *s, uint8_t *oks) {
         if (cb >= cend) return;
         store(s, ok_next, oks);
-        load(cb + 64);   // (past the last tile: other cells of a page, not used)
-        ok_next = sound_pages(cb + 64);
-        pages(cb + 128);
+        load(cb + C);   // (past the last tile: other cells of a page, not used)
+        ok_next = sound_pages(cb + C);
+        pages(cb + 2 * C);
     }
 };
 
@@ -1038,16 +1038,16 @@ __global__ __launch_bounds__(NW * 64, NB <= 2 ? 3 : 2) void k_attn_tiles(attn_pa
 }
 
 // The same where a cell meets one tile or two of a sequence, or the tables' cells
-// are more than the workspace holds decoded: NW waves go over 64 cells at a time
+// are more than the workspace holds decoded: NW waves go over C cells at a time
 // and decode the codes themselves, each once a workgroup, by the thread that loaded
 // it a tile before, into the other of two LDS buffers.  Bound by the decoding and
 // the products in turn, and with few workgroups by the slowest: 9 conversations of 5
-// to 301 tokens behind up to 1777, 9 heads of 64 on 3, in 36 us with the join.
-template <int NB, int NW>   // 32-wide groups of head_dim; waves
-__global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsigned long long *err) {
-    constexpr int U = tile_of<NB>::U;
-    extern __shared__ uint4 s_cells[];         // [2][4 U]
-    __shared__ alignas(16) uint8_t s_ok[2][8];   // whether a tile's groups of eight cells lie in a page
+// to 301 tokens behind up to 1777, 9 heads of 64 on 3, in 34 us with the join.
+template <int NB, int NW, int C>   // 32-wide groups of head_dim; waves; cells of a tile
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void k_attn_chunk(attn_paged_args a, unsigned long long *err) {
+    constexpr int B = tile_of<NB>::B, buf_units = C / 32 * 4 * B;
+    extern __shared__ uint4 s_cells[];         // [2][buf_units]
+    __shared__ alignas(16) uint8_t s_ok[2][C / 8];   // whether a tile's groups of eight cells lie in a page
     const int wave = threadIdx.x >> 6, split = blockIdx.y;
     int kvh;
     const int tile = chunk_tile((int)a.kv.n_head_kv, kvh);
@@ -1055,14 +1055,14 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
     if (T.r0 < 0 || (split > 0 && split * T.per >= T.blocks)) return;
     const int cbeg = T.c0 + split * T.per * 64, cend = min(T.c1, cbeg + T.per * 64);
     const int tid = threadIdx.x;
-    auto cells = [&](int buf) { return s_cells + buf * 4 * U; };
+    auto cells = [&](int buf) { return s_cells + buf * buf_units; };
     chunk_rows<NB> r;
     auto blocks = [&](int cb, int buf) {
 #pragma unroll 1
-        for (int blk = 0; blk < 2; blk++) {
+        for (int blk = 0; blk < C / 32; blk++) {
             const uint32_t ok = (uint32_t)__builtin_amdgcn_readfirstlane(
                 (int)*reinterpret_cast<const uint32_t *>(&s_ok[buf][blk * 4]));
-            r.block(cells(buf) + blk * 2 * U, cb + blk * 32, ok, T.c1);
+            r.block(cells(buf) + blk * 4 * B, cb + blk * 32, ok, T.c1);
         }
     };
     if (NW == 8 && T.rows - T.r0 <= NW * 16) {
@@ -1070,12 +1070,12 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
         // to 27 tokens behind 640 to 5125 cells, 32 heads of 128 on 8: 249 us, all waves
         // decoding 284.)
         if (wave >= NW / 2) {
-            tile_maker<NB, NW * 32> maker(a.kv, T.sq, kvh, a.page_sh, cend, tid - NW * 32, err);
+            tile_maker<NB, NW * 32, C> maker(a.kv, T.sq, kvh, a.page_sh, cend, tid - NW * 32, err);
             maker.first(cbeg, cells(0), s_ok[0]);
             lds_barrier();
             int buf = 0;
-            for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
-                maker.next(cb + 64, cells(buf ^ 1), s_ok[buf ^ 1]);
+            for (int cb = cbeg; cb < cend; cb += C, buf ^= 1) {
+                maker.next(cb + C, cells(buf ^ 1), s_ok[buf ^ 1]);
                 lds_barrier();
             }
             return;
@@ -1084,22 +1084,22 @@ __global__ __launch_bounds__(NW * 64) void k_attn_chunk(attn_paged_args a, unsig
         r.load(a);
         lds_barrier();
         int buf = 0;
-        for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
+        for (int cb = cbeg; cb < cend; cb += C, buf ^= 1) {
             blocks(cb, buf);
             lds_barrier();
         }
         r.write(a, T, split);
         return;
     }
-    tile_maker<NB, NW * 64> maker(a.kv, T.sq, kvh, a.page_sh, cend, tid, err);
+    tile_maker<NB, NW * 64, C> maker(a.kv, T.sq, kvh, a.page_sh, cend, tid, err);
     maker.first(cbeg, cells(0), s_ok[0]);
     r.place(a, T, kvh, T.r0 + wave * 32);
     r.load(a);
     lds_barrier();
     int buf = 0;
-    for (int cb = cbeg; cb < cend; cb += 64, buf ^= 1) {
+    for (int cb = cbeg; cb < cend; cb += C, buf ^= 1) {
         blocks(cb, buf);
-        maker.next(cb + 64, cells(buf ^ 1), s_ok[buf ^ 1]);
+        maker.next(cb + C, cells(buf ^ 1), s_ok[buf ^ 1]);
         lds_barrier();
     }
     r.write(a, T, split);
@@ -1225,12 +1225,16 @@ constexpr double k_chunk_work = 268435456.0;    // rows x kv heads x cells of th
 // (128); of 64 tokens 37 and 35, 113 and 122; of 32 over 500 25 and 23, 43 and 35.
 constexpr int k_decode_rows = 512;
 constexpr int64_t k_pre_bytes = (int64_t)1 << 30;   // of the workspace for decoded cells, at most
-// Waves of a workgroup.  Up to 64 dims four: three or four workgroups share a CU,
+// Waves of a workgroup.  Up to 64 dims four: two or three workgroups share a CU,
 // and uneven sequences leave smaller last tiles (a batch of 9 conversations of
-// 5 to 301 tokens 37 us, with eight waves 45).  Above, eight, which copy or decode a
-// cell once for 256 rows (one sequence of 4096 tokens, 32 heads of 128: 1043 us, with four
-// 1141) but where decoded cells meet less than 2048 rows a sequence (8 sequences of
-// 128 tokens over 2000 cells: 178, with four 157).
+// 5 to 301 tokens 37 us, with eight waves 45).  Above, with cells decoded before, eight
+// from 2048 rows a sequence on, which copy a cell once for 256 rows (one sequence of
+// 4096 tokens, 32 heads of 128: 1043 us, with four 1141; 8 sequences of 128 tokens over 2000
+// cells: 178, with four 157).  Where each workgroup decodes, four, two workgroups
+// to a CU, above 128 rows a sequence (8 of 40 tokens over 2000 cells: 79 us, with eight
+// 101; of 64: 98 and 120), and eight up to there, of which half decode (32 of 16 over
+// 1000: 97 and 80), and for the many rows whose cells the workspace does not hold.
+constexpr int k_helped_rows = 128;
 constexpr int k_wide_rows = 2048;
 // Parts of a row's cells: as many workgroups as a CU runs at a time, a part at
 // least so many blocks of 64 cells (single tokens: 64 sequences of up to 8192 cells
@@ -1248,7 +1252,7 @@ static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
     p.pre = chunks && of_seq >= k_decode_rows && kv->n_seq * p.pre_tiles <= k_pre_bytes / tile_bytes;
     p.pre_bytes = p.pre ? kv->n_seq * p.pre_tiles * tile_bytes : 0;
     p.ok_bytes = p.pre ? (kv->n_seq * p.pre_tiles * 8 + 255) & ~(int64_t)255 : 0;
-    p.waves = !chunks ? 0 : kv->head_dim <= 64 || (p.pre && of_seq < k_wide_rows) ? 4 : 8;
+    p.waves = !chunks ? 0 : kv->head_dim <= 64 || (p.pre ? of_seq < k_wide_rows : of_seq > k_helped_rows && of_seq < k_decode_rows) ? 4 : 8;
     p.tile_rows = p.waves ? p.waves * 32 : 16;
     p.tiles = rows / p.tile_rows + kv->n_seq;
     const int64_t wgs = std::max<int64_t>(1, p.tiles * kv->n_head_kv);
@@ -1271,12 +1275,12 @@ static int allow_lds(const void *kernel, int lds, std::atomic<uint64_t> &done) {
     return 0;
 }
 
-template <int NB, int NW>
+template <int NB, int NW, int C>
 static int launch_chunk(const attn_paged_args &m, const dim3 &grid, hipStream_t s, unsigned long long *err) {
-    constexpr int lds = 2 * 4 * tile_of<NB>::U * 16;
+    constexpr int lds = 2 * C / 32 * 4 * tile_of<NB>::B * 16;
     static std::atomic<uint64_t> done{0};
-    if (int rc = allow_lds(reinterpret_cast<const void *>(k_attn_chunk<NB, NW>), lds, done)) return rc;
-    hipLaunchKernelGGL((k_attn_chunk<NB, NW>), grid, dim3(NW * 64), lds, s, m, err);
+    if (int rc = allow_lds(reinterpret_cast<const void *>(k_attn_chunk<NB, NW, C>), lds, done)) return rc;
+    hipLaunchKernelGGL((k_attn_chunk<NB, NW, C>), grid, dim3(NW * 64), lds, s, m, err);
     LNSHIP_HIP(hipGetLastError());
     return 0;
 }
@@ -1297,7 +1301,9 @@ static int launch_attn(const attn_paged_args &m, const attn_plan &p, int cus, hi
             LNSHIP_HIP(hipGetLastError());
             return 0;
         }
-        if (p.waves) return launch_chunk<NB, NB <= 2 ? 4 : 8>(m, chunks, s, err);
+        if (p.waves == 4) return launch_chunk<NB, 4, NB <= 2 ? 64 : 32>(m, chunks, s, err);
+        if constexpr (NB > 2)
+            if (p.waves == 8) return launch_chunk<NB, 8, 64>(m, chunks, s, err);
     }
     const dim3 grid((unsigned)p.tiles, (unsigned)m.kv.n_head_kv, (unsigned)p.splits);
     // A CU for each workgroup: eight waves, which go over their cells in half the steps
