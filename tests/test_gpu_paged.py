@@ -535,6 +535,16 @@ def test_long_cache_of_one_token(ln):
         check_attn(got, q, [1], [n], keys, vals)
 
 
+@pytest.mark.parametrize("window", [1, 63, 64, 65, 500, 513, 1000, 5000, 1 << 40])
+def test_windows_of_single_tokens(ln, window):
+    """Parts are as many as a window may need: windows of any length behind long caches."""
+    rng = np.random.default_rng(23)
+    kv_len = [4096, 3000, 1, 77]
+    q, c, table, keys, vals = attn_case(rng, [1] * 4, kv_len, 16, 8, 2, 64)
+    got = run_attn(ln, q, c, table, [1] * 4, kv_len, window).cpu().numpy()
+    check_attn(got, q, [1] * 4, kv_len, keys, vals, window)
+
+
 # ---- together ----------------------------------------------------------------------------
 
 def test_chunks_and_single_tokens_agree(ln):

@@ -1241,7 +1241,8 @@ constexpr int k_wide_rows = 2048;
 // 302 us with 16 a CU, 340 with 4; conversations 37 us with parts of 4 blocks, 40 with 8
 // and 55 with 2, of which the join reads more).
 constexpr int k_few_wgs = 16, k_few_part = 8, k_many_wgs = 2, k_many_part = 4;
-static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
+// window: 0, or fewer parts for it (the workspace's size is that without).
+static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus, int64_t window) {
     attn_plan p;
     const int64_t rows = kv->ntok * rep, of_seq = kv->n_seq ? rows / kv->n_seq : 0;
     const int64_t n_head = rep * kv->n_head_kv, tile_bytes = kv->n_head_kv * 64 * ((kv->head_dim + 31) & ~(int64_t)31) * 8;
@@ -1257,7 +1258,9 @@ static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus) {
     p.tiles = rows / p.tile_rows + kv->n_seq;
     const int64_t wgs = std::max<int64_t>(1, p.tiles * kv->n_head_kv);
     p.min_per = p.waves ? k_many_part : k_few_part;
-    const int64_t most = (cells / 64 + p.min_per - 1) / p.min_per;
+    // blocks of 64 cells that a tile sees at most
+    const int64_t seen = window > 0 ? std::min(cells, std::min(window, cells) + p.tile_rows / rep + 128) : cells;
+    const int64_t most = (seen / 64 + p.min_per - 1) / p.min_per;
     const int64_t want = p.waves ? k_many_wgs : k_few_wgs;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want * cus + wgs - 1) / wgs, most, 256}));
     p.parts_bytes = p.splits > 1 ? (kv->ntok * n_head * (p.splits * (kv->head_dim + 2) + 1) * 4 + 255) & ~(int64_t)255 : 0;
@@ -1377,7 +1380,7 @@ int64_t lnship16_attn_paged_work(const lnship_paged_kv *kv, int64_t n_head) {
         return fail(LNSHIP_EINVAL, "attn_paged: n_head not a multiple of n_head_kv%s");
     device_state *st = state();
     if (!st) return LNSHIP_ENOINIT;
-    const attn_plan p = plan_attn(kv, n_head / kv->n_head_kv, st->cus);
+    const attn_plan p = plan_attn(kv, n_head / kv->n_head_kv, st->cus, 0);
     return p.parts_bytes + p.pre_bytes + p.ok_bytes;
 }
 
@@ -1393,7 +1396,7 @@ int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args 
     device_state *st = state();
     if (!st) return LNSHIP_ENOINIT;
     const int64_t rep = a->n_head / kv->n_head_kv;
-    const attn_plan p = plan_attn(kv, rep, st->cus);
+    const attn_plan p = plan_attn(kv, rep, st->cus, a->window);
     const int64_t need = p.parts_bytes + p.pre_bytes + p.ok_bytes;
     if (need && (!a->work || a->work_bytes < (size_t)need || ((uintptr_t)a->work & 15)))
         return fail(LNSHIP_EINVAL, "attn_paged: work smaller than lnship16_attn_paged_work or not aligned%s");
