@@ -110,6 +110,16 @@ def test_workspace_sizes():
     assert L.lnship16_attn_paged_work(ctypes.byref(paged()), 7) == EINVAL
 
 
+@pytest.mark.parametrize("packer,cls", [("_KV", "PagedKV"), ("_STORE", "PagedStoreArgs"), ("_ATTN", "PagedAttnArgs")])
+def test_packed_arguments_are_the_structures(packer, cls):
+    import lnship.paged
+    cls, packer = getattr(lnship, cls), getattr(lnship.paged, packer)
+    n = len(cls._fields_)
+    want = [i + 1 + (i << 33) if ctypes.sizeof(t) == 8 else i + 1 for i, (_, t) in enumerate(cls._fields_)]
+    a = cls.from_buffer_copy(packer.pack(*want))
+    assert packer.size == ctypes.sizeof(cls) and [getattr(a, f[0]) for f in cls._fields_] == want and n == len(want)
+
+
 def test_tensors_that_are_not_on_the_gpu_are_refused():
     import lnship.paged
     import torch

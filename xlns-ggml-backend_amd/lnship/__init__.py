@@ -193,9 +193,9 @@ def lib():
                                          c_p]),
         "lnship32_store_kv": (ctypes.c_int, [c_p, c_i64, c_p, c_i64, c_i64, c_i64, ctypes.c_int, c_p, c_p, c_i64,
                                              c_i64, ctypes.c_int, c_p, c_i64, c_p]),
-        "lnship16_rope_store_kv_paged": (ctypes.c_int, [ctypes.POINTER(PagedKV), ctypes.POINTER(PagedStoreArgs), c_p]),
-        "lnship16_attn_paged": (ctypes.c_int, [ctypes.POINTER(PagedKV), ctypes.POINTER(PagedAttnArgs), c_p]),
-        "lnship16_attn_paged_work": (c_i64, [ctypes.POINTER(PagedKV), c_i64]),
+        "lnship16_rope_store_kv_paged": (ctypes.c_int, [c_p, c_p, c_p]),   # (PagedKV, PagedStoreArgs, or their bytes)
+        "lnship16_attn_paged": (ctypes.c_int, [c_p, c_p, c_p]),   # (PagedKV, PagedAttnArgs)
+        "lnship16_attn_paged_work": (c_i64, [c_p, c_i64]),
         "lnship_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), c_p]),
         "lnship_causal_mask": (ctypes.c_int, [c_p, c_i64, c_i64, c_p, c_p]),
         "lnship_rope_table": (ctypes.c_int, [ctypes.c_float, ctypes.c_int, c_i64, c_p]),
@@ -246,7 +246,7 @@ def current_stream(dev):
     current one; uploads the tables to it at its first use.  For entry points
     that are called once a token: it costs a tenth of init() and _stream()."""
     import torch
-    if dev < 0 or dev != torch.cuda.current_device():
+    if dev < 0 or dev != (torch._C._cuda_getDevice() if _ready else torch.cuda.current_device()):
         raise LnshipError("tensors must be on the current device (they are on %s)" %
                           ("the CPU" if dev < 0 else "cuda:%d" % dev))
     if dev not in _ready:

@@ -7,9 +7,15 @@ replays with other lengths and pages: q_start [n_seq + 1] (rows q_start[s] to
 q_start[s+1] - 1 are sequence s's new tokens), kv_len [n_seq] (its cells, the
 new tokens' included) and table [n_seq, pages a sequence may have].
 """
+import struct
+
 import torch
 
-from . import LnshipError, PagedAttnArgs, PagedKV, PagedStoreArgs, byref, check, current_stream, lib
+from . import LnshipError, check, current_stream, lib
+
+# The fields of PagedKV, PagedStoreArgs and PagedAttnArgs, packed: a tenth of
+# the time that the structures take, of calls that every layer of a step makes.
+_KV, _STORE, _ATTN = (struct.Struct(f) for f in ("PPqqqqPqqqPP", "PPPqqqqiiPqPq", "PPqqqfqPN"))
 
 _I16, _I32, _F32 = torch.int16, torch.int32, torch.float32
 
@@ -25,20 +31,21 @@ def _no(what):
 
 
 def _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok):
-    """lnship_paged_kv of the tensors, checked; and the device that all must be on, the current one."""
+    """lnship_paged_kv of the tensors, checked, as bytes; the device that all must be on, the current one;
+    n_head_kv and head_dim."""
     dev = k_pages.get_device()
     shape = k_pages.shape
-    if k_pages.dtype != _I16 or k_pages.dim() != 3 or not k_pages.is_contiguous():
+    if k_pages.dtype is not _I16 or k_pages.dim() != 3 or not k_pages.is_contiguous():
         _no("k_pages must be contiguous int16 [n_pages, n_head_kv, page * head_dim]")
-    if v_pages.dtype != _I16 or v_pages.shape != shape or not v_pages.is_contiguous() or v_pages.get_device() != dev:
+    if v_pages.dtype is not _I16 or v_pages.shape != shape or not v_pages.is_contiguous() or v_pages.get_device() != dev:
         _no("v_pages must be as k_pages")
     n_seq = kv_len.numel()
-    if kv_len.dtype != _I32 or kv_len.dim() != 1 or not kv_len.is_contiguous() or kv_len.get_device() != dev:
+    if kv_len.dtype is not _I32 or kv_len.dim() != 1 or not kv_len.is_contiguous() or kv_len.get_device() != dev:
         _no("kv_len must be contiguous int32 [n_seq] on the pages' device")
-    if q_start.dtype != _I32 or q_start.shape != (n_seq + 1,) or not q_start.is_contiguous() or \
+    if q_start.dtype is not _I32 or q_start.shape != (n_seq + 1,) or not q_start.is_contiguous() or \
             q_start.get_device() != dev:
         _no("q_start must be contiguous int32 [n_seq + 1] on the pages' device")
-    if table.dtype != _I32 or table.dim() != 2 or not table.is_contiguous() or table.get_device() != dev:
+    if table.dtype is not _I32 or table.dim() != 2 or not table.is_contiguous() or table.get_device() != dev:
         _no("table must be contiguous int32 [n_seq, pages] on the pages' device")
     rows, width = table.shape
     n_pages, n_head_kv, codes = shape
@@ -46,13 +53,14 @@ def _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok):
         _no("table must have a row for every sequence")
     if page < 1 or codes % page:
         _no("pages of %d codes a head hold no %d cells" % (codes, page))
-    return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, n_head_kv, codes // page, table.data_ptr(),
-                   width, ntok, n_seq, q_start.data_ptr(), kv_len.data_ptr()), dev
+    hd = codes // page
+    return _KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, n_head_kv, hd, table.data_ptr(), width, ntok,
+                    n_seq, q_start.data_ptr(), kv_len.data_ptr()), dev, n_head_kv, hd
 
 
 def _ld(t, name, ntok, heads, dim, dev):
     """The row stride of a [ntok, heads, dim] float32 tensor whose heads lie behind each other."""
-    if t.dtype != _F32 or t.shape != (ntok, heads, dim) or t.get_device() != dev:
+    if t.dtype is not _F32 or t.shape != (ntok, heads, dim) or t.get_device() != dev:
         _no("%s must be float32 [%d, %d, %d] on the pages' device" % (name, ntok, heads, dim))
     s0, s1, s2 = t.stride()
     if s2 != 1 or (s1 != dim and heads > 1):
@@ -69,14 +77,13 @@ def rope_store_kv(q, k, v, k_pages, v_pages, page, table, q_start, kv_len, cos_s
     q|k|v product's rows; cos_sin [n_pos, n_dims / 2, 2] float32 (None with
     n_dims 0: nothing is rotated).  Returns the rotated queries."""
     ntok = k.shape[0]
-    kv, dev = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
+    kv, dev, nkv, hd = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
     stream = current_stream(dev)
-    hd, nkv = kv.head_dim, kv.n_head_kv
     if n_dims is None:
         n_dims = hd if cos_sin is not None else 0
     cs = n_pos = 0
     if n_dims:
-        if cos_sin is None or cos_sin.dtype != _F32 or cos_sin.dim() != 3 or not cos_sin.is_contiguous() or \
+        if cos_sin is None or cos_sin.dtype is not _F32 or cos_sin.dim() != 3 or not cos_sin.is_contiguous() or \
                 cos_sin.get_device() != dev or cos_sin.shape[1:] != (n_dims // 2, 2):
             _no("cos_sin must be contiguous float32 [n_pos, n_dims / 2, 2] on the pages' device")
         cs, n_pos = cos_sin.data_ptr(), cos_sin.shape[0]
@@ -87,9 +94,9 @@ def rope_store_kv(q, k, v, k_pages, v_pages, page, table, q_start, kv_len, cos_s
             out = torch.empty((ntok, nh, hd), dtype=_F32, device=k_pages.device)
         q_ld, out_ld = _ld(q, "q", ntok, nh, hd, dev), _ld(out, "out", ntok, nh, hd, dev)
         q_at, out_at = q.data_ptr(), out.data_ptr()
-    a = PagedStoreArgs(q_at, k.data_ptr(), v.data_ptr(), q_ld, _ld(k, "k", ntok, nkv, hd, dev),
-                       _ld(v, "v", ntok, nkv, hd, dev), nh, n_dims, neox, cs, n_pos, out_at, out_ld)
-    check(lib().lnship16_rope_store_kv_paged(byref(kv), byref(a), stream))
+    a = _STORE.pack(q_at, k.data_ptr(), v.data_ptr(), q_ld, _ld(k, "k", ntok, nkv, hd, dev),
+                    _ld(v, "v", ntok, nkv, hd, dev), nh, n_dims, neox, cs, n_pos, out_at, out_ld)
+    check(lib().lnship16_rope_store_kv_paged(kv, a, stream))
     return out
 
 
@@ -99,18 +106,17 @@ def attention(q, k_pages, v_pages, page, table, q_start, kv_len, scale, window=0
     and, with window > 0, no further than window - 1 before it.  Returns out,
     [ntok, n_head, head_dim] float32."""
     ntok, nh = q.shape[:2]
-    kv, dev = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
+    kv, dev, _, hd = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
     stream = current_stream(dev)
-    hd = kv.head_dim
     if out is None:
         out = torch.empty((ntok, nh, hd), dtype=_F32, device=k_pages.device)
     q_ld, out_ld = _ld(q, "q", ntok, nh, hd, dev), _ld(out, "out", ntok, nh, hd, dev)
-    L, ref = lib(), byref(kv)
-    need = L.lnship16_attn_paged_work(ref, nh)
+    L = lib()
+    need = L.lnship16_attn_paged_work(kv, nh)
     if need < 0:
         check(need)
     # (of torch's allocator: the stream's own, a captured graph's own)
     work = torch.empty(need, dtype=torch.uint8, device=k_pages.device) if need else None
-    a = PagedAttnArgs(q.data_ptr(), out.data_ptr(), q_ld, out_ld, nh, scale, window, work.data_ptr() if need else 0, need)
-    check(L.lnship16_attn_paged(ref, byref(a), stream))
+    a = _ATTN.pack(q.data_ptr(), out.data_ptr(), q_ld, out_ld, nh, scale, window, work.data_ptr() if need else 0, need)
+    check(L.lnship16_attn_paged(kv, a, stream))
     return out
