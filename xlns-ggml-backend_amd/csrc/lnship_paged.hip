@@ -1108,7 +1108,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void k_attn_chunk(attn_pa
 // The splits' parts of a row joined, in a fixed order, by one wave (four rows a
 // workgroup) or, many parts, by the workgroup's four: head_dim / 4 lanes read a
 // part, the others other parts beside it.  Bound by the launch and one read of the
-// parts: 7.5 us for the rows of 9 conversations, 9 heads of 64.
+// parts: 6.6 us for the rows of 9 conversations, 9 heads of 64.
 template <int W>   // waves of a row
 __global__ __launch_bounds__(256) void k_attn_paged_join(attn_paged_args a) {
     constexpr int S = W == 4 ? 256 : 64;   // parts at most
