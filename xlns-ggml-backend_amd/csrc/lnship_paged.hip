@@ -163,8 +163,9 @@ constexpr int k_store_rows = 8;   // rows of a workgroup at most
 // is a gather that costs a cache line a lane.  A row's cosines and sines are
 // converted once for all heads.  Bound by the arithmetic of the codes, some 40
 // instructions a pair and 60 for its conversions, and by the scattered stores:
-// 11414 rows of 32 heads of 64 on 8 in 77 us, 3.4 TB/s of what is read and written
-// (with rows spread over all XCDs 94: the caches' lines are then written in parts).
+// 11414 rows of 32 heads of 64 on 8 in 75 us, 3.4 TB/s of what is read and written
+// (with rows spread over all XCDs 94: the caches' lines are then written in parts;
+// with registers for six waves a SIMD in place of eight 80).
 template <bool NEOX>
 __global__ __launch_bounds__(k_block, 8) void k_store_paged_rows(store_args s, int row_sh, dev_tables T,
                                                               unsigned long long *err) {
