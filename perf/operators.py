@@ -21,7 +21,6 @@ own = False
 
 DEV = "cuda"
 THETA = 10000.0
-PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xlns-ggml-backend_amd")
 
 
 def listed():
@@ -173,8 +172,9 @@ def prepare(case, seed):
 # ---- the framework's calls -----------------------------------------------------------------------
 
 def _package():
-    if PACKAGE not in sys.path:
-        sys.path.insert(0, PACKAGE)
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xlns-ggml-backend_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
     import lnship
     import lnship.paged
     return lnship
