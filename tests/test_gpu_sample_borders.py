@@ -1,0 +1,55 @@
+"""Token draws that one histogram does not resolve, with a min_p at or above the largest token's own
+weight: the first token by rank is kept always, and every row's token and probability are written."""
+import numpy as np
+import pytest
+
+from test_gpu_sample import check, dev
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ln():
+    import lnship
+    lnship.init()
+    return lnship
+
+
+def draws(ln, x, u, T=None, k=None, p=None, m=None):
+    """The draw into outputs that hold what no draw gives."""
+    rows = len(x)
+    out = (torch.full((rows,), -77, dtype=torch.int32, device="cuda"), torch.full((rows,), -7.0, device="cuda"))
+    ln.sample(dev(x, np.float32), dev(u, np.float32), dev(T, np.float32), dev(k, np.int32), dev(p, np.float32),
+              dev(m, np.float32), out=out)
+    return out[0].cpu().numpy(), out[1].cpu().numpy()
+
+
+@pytest.mark.parametrize("vocab", [2500, 40000])
+@pytest.mark.parametrize("min_p", [0.25, 0.99999994, 1.0])
+@pytest.mark.parametrize("what", ["large top_k", "cold", "infinitely hot", "all alike", "ties at the top", "tied border"])
+def test_min_p_up_to_the_largest_weight(ln, what, min_p, vocab):
+    print(f"\n[draw] {what} min_p {min_p} vocab {vocab}", flush=True)
+    rng = np.random.default_rng(vocab)
+    rows = 6
+    x = (rng.standard_normal((rows, vocab)) * 2).astype(np.float32)
+    x[:, 7] = 9.0                     # the largest, alone
+    u = np.array([0.0, 0.1, 0.4, 0.5, 0.8, 0.9999999])
+    m = np.full(rows, min_p)
+    T = k = p = None
+    if what == "large top_k":
+        k = np.full(rows, 2000)
+    elif what == "cold":
+        T = np.full(rows, 1e-6)
+    elif what == "infinitely hot":
+        T = np.full(rows, np.inf)
+    elif what == "all alike":
+        x[:] = -3.0
+        p = np.array([0.0, 0.3, 0.5, 0.9, 0.999, 0.9999999])
+    elif what == "ties at the top":
+        x[:, 5:2400:3] = 9.0
+        k = np.full(rows, 1500)
+    else:
+        x = np.round(x).astype(np.float32)
+        p = np.array([0.0, 0.3, 0.5, 0.9, 0.999, 0.9999999])
+    check(draws(ln, x, u, T, k, p, m), x, u, T, k, p, m)

@@ -210,7 +210,8 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
     auto W = [&](float v) { return sharp ? (uint64_t)(v == d0.xmax) << k_w_sh : any(v); };
     const int top_k = d0.top_k;
     const float top_p = d0.top_p;
-    const uint64_t wmin = least_weight(d0.min_p, (uint64_t)1 << k_w_sh);   // (the largest logit weighs 2^40 units)
+    // (the largest logit's own weight, which power() leaves 44 units below 2^40)
+    const uint64_t wmin = least_weight(d0.min_p, W(d0.xmax));
     __syncthreads();   // (what lay in s_w and s_u64 is read)
     // the border key and how many of its ties are kept
     uint32_t bkey = k_key_ninf + 1, bties = 0xffffffffu;
