@@ -26,7 +26,7 @@ def draws(ln, x, u, T=None, k=None, p=None, m=None):
 
 
 @pytest.mark.parametrize("vocab", [2500, 40000])
-@pytest.mark.parametrize("min_p", [0.25, 0.99999994, 1.0])
+@pytest.mark.parametrize("min_p", [0.25, 0.99999994, 1.0, 1.0000001, 5.0, float("inf")])
 @pytest.mark.parametrize("what", ["large top_k", "cold", "infinitely hot", "all alike", "ties at the top", "tied border"])
 def test_min_p_up_to_the_largest_weight(ln, what, min_p, vocab):
     print(f"\n[draw] {what} min_p {min_p} vocab {vocab}", flush=True)
@@ -53,3 +53,20 @@ def test_min_p_up_to_the_largest_weight(ln, what, min_p, vocab):
         x = np.round(x).astype(np.float32)
         p = np.array([0.0, 0.3, 0.5, 0.9, 0.999, 0.9999999])
     check(draws(ln, x, u, T, k, p, m), x, u, T, k, p, m)
+
+
+@pytest.mark.parametrize("vocab", [100, 30000, 60000])
+def test_a_min_p_above_one_leaves_the_first_token(ln, vocab):
+    """Of equal largest logits too, whichever limits stand beside it."""
+    rng = np.random.default_rng(vocab)
+    rows = 5
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    first = np.array([0, 3, 50, 98, 99])
+    for r, f in enumerate(first):
+        x[r, f:] = 8.0
+    u = np.full(rows, 0.75)
+    for kw in ({}, {"T": 0.7}, {"k": 40}, {"k": 5000}, {"p": 0.9}, {"k": 40, "p": 0.9}):
+        kw = {n: np.full(rows, y) for n, y in kw.items()}
+        for m in (1.5, float("inf")):
+            tok, prob = draws(ln, x, u, **kw, m=np.full(rows, m))
+            assert np.array_equal(tok, first) and (prob == 1.0).all(), (kw, m)

@@ -147,9 +147,9 @@ struct draw_row {   // what a row asks for
     float top_p, min_p;
 };
 
-// the least weight that min_p keeps
+// the least weight that min_p, up to 1, keeps
 __device__ __forceinline__ uint64_t least_weight(float min_p, uint64_t largest) {
-    return min_p > 0.0f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * (double)largest) : 0;
+    return min_p > 0.0f ? (uint64_t)ceil((double)min_p * (double)largest) : 0;
 }
 
 // the unit of the total that u names
@@ -438,7 +438,6 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
     };
 
     const float T = uniform(a.temperature ? a.temperature[r] : 1.0f);
-    const bool greedy = !(T > 0.0f);
     draw_row D;
     D.f = uniform(1.4426950408889634 / (double)T);
     D.top_k = uniform(a.top_k ? a.top_k[r] : 0);
@@ -446,6 +445,8 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
     D.top_p = uniform(a.top_p ? a.top_p[r] : 1.0f);
     if (!(D.top_p < 1.0f)) D.top_p = 1.0f;
     D.min_p = uniform(a.min_p ? a.min_p[r] : 0.0f);
+    // (a min_p above 1 leaves the first token by rank, which is kept always)
+    const bool greedy = !(T > 0.0f) || D.min_p > 1.0f;
 
     auto easy = [&]() -> bool {
         // Bins of a logit's distance from ref, which lies no more than k_head bins
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
             return read_lane(row_scan(s[lane & (k_draw_waves - 1)], max_u64()), k_draw_waves - 1);
         };
 
-        // the largest logit, the first index that has it for greedy, and the bins
+        // the largest logit, the first index that has it if that one is taken, and the bins
         float mx = -INFINITY;
         int at = 0x7fffffff;
         if (greedy) {
@@ -607,7 +608,7 @@ __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
                 if (wmin) {
                     // min_p's border above top_p's: that one alone counts; at or below the
                     // list's first bin: what lies above the list is above it too
-                    const int at = (int)(place_of(D.xmax) - log2f(fminf(D.min_p, 1.0f)) * k_bins_binade);
+                    const int at = (int)(place_of(D.xmax) - log2f(D.min_p) * k_bins_binade);
                     cut = at + 1 >= s_bin[0];
                     lo = max(min(lo, at - 1), 0);
                 }
