@@ -405,7 +405,7 @@ typedef struct lnship_paged_kv {
  * (lnship_rope_table's layout, n_pos positions).  A position below 0, past the
  * table's cells or (rotating) not below n_pos, and a page outside
  * [0, n_pages), is recorded (lnship_index_error) and its row, or what it has
- * in that page, is skipped.  Two rows of one call never have the same cell
+ * in that page, is skipped.  q_dst may be q (with q_dst_ld = q_ld).  Two rows of one call never have the same cell
  * unless the table names a page twice; then which of them stays is not said. */
 typedef struct lnship_paged_store_args {
     const float *q, *k, *v;

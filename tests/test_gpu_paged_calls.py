@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import paged_reference as R
-from test_gpu_paged import attn_case, check_attn, dev, index_error, positions, run_attn, starts
+from test_gpu_paged import attn_case, check_attn, dev, index_error, positions, rope_table, run_attn, starts
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -18,39 +18,32 @@ def ln():
     return lnship
 
 
-# ---- pages behind a window ---------------------------------------------------------------
+# ---- rotation in place -------------------------------------------------------------------
 
-FREED = [
-    # q_len, kv_len, page, heads, kv heads, dim, window, cells of the table
-    ([1], [1000], 16, 12, 4, 64, 33, 0),
-    ([1, 1, 1], [1000, 517, 40], 32, 8, 2, 128, 100, 0),
-    ([1] * 40, [300 + 29 * i for i in range(40)], 16, 16, 8, 128, 65, 0),
-    ([9, 3], [700, 400], 16, 4, 2, 200, 50, 0),
-    ([40, 90], [300, 400], 16, 4, 2, 64, 17, 1 << 14),
-    ([70], [700], 32, 8, 2, 128, 111, 1 << 14),
-    ([520], [900], 16, 8, 2, 64, 200, 1 << 13),
-    ([600, 300], [1200, 1111], 32, 4, 2, 128, 77, 1 << 13),
-]
-
-
-@pytest.mark.parametrize("q_len,kv_len,page,nh,nkv,hd,window,cells", FREED)
-def test_pages_behind_the_window_may_be_freed(ln, q_len, kv_len, page, nh, nkv, hd, window, cells):
-    """A page whose cells no new token sees is not looked at: its number may be -1, and is no error."""
-    print(f"\n[attn] {q_len} {kv_len} page {page} {nh}/{nkv}x{hd} window {window} freed", flush=True)
-    rng = np.random.default_rng(window)
-    q, c, table, keys, vals = attn_case(rng, q_len, kv_len, page, nh, nkv, hd)
-    want = run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells).cpu().numpy()
-    first = [max(0, m - n - window + 1) // page for n, m in zip(q_len, kv_len)]
-    assert any(first)
-    for s, f in enumerate(first):
-        table[s, :f] = -1
-    index_error(ln)
-    got = run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells).cpu().numpy()
-    assert index_error(ln)[0] == 0
-    assert np.array_equal(got, want)
-    check_attn(got, q, q_len, kv_len, keys, vals, window)
-    # the first page that is seen counts
-    s = int(np.argmax(first))
-    table[s, first[s]] = -5
-    run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells)
-    assert index_error(ln) == (1, -5)
+@pytest.mark.parametrize("neox", [False, True])
+@pytest.mark.parametrize("T,nh,nkv,hd,nd", [
+    (1, 1, 1, 8, 8), (3, 9, 3, 64, 64), (5, 4, 2, 80, 80), (7, 6, 2, 96, 96), (20, 32, 8, 128, 128), (9, 3, 3, 256, 256),
+    (6, 5, 1, 72, 18), (11, 3, 1, 136, 64), (4, 2, 2, 24, 0), (300, 3, 1, 256, 250),
+    # 2^19 values and more: the other kernel
+    (700, 4, 2, 128, 128), (1500, 4, 2, 80, 64)])
+def test_queries_rotated_in_place(ln, T, nh, nkv, hd, nd, neox):
+    """out = q, of its own or within the rows of a fused product: queries and cells bit for bit, and
+    nothing else written."""
+    print(f"\n[store] in place {T} x {nh}/{nkv}x{hd} rot {nd} neox {neox}", flush=True)
+    rng = np.random.default_rng(hd + T)
+    page = 32
+    x = rng.standard_normal((T, nh + 2 * nkv, hd)).astype(np.float32)
+    cs = rope_table(ln, T + 3, nd) if nd else None
+    table, n_pages = R.tables(rng, [T + 3], page)
+    batch = (page, dev(table), dev(starts([T])), dev(np.int32([T + 3])), dev(cs) if nd else None)
+    rot = R.rope(x[:, :nh + nkv], cs[3:], neox, nd) if nd else x[:, :nh + nkv]
+    c = R.Cache(n_pages, page, nkv, hd, fill=0)
+    c.put(table[0], np.arange(3, T + 3), R.store_codes(rot[:, nh:]), R.store_codes(x[:, nh + nkv:]))
+    for fused in (True, False):
+        xd = dev(x)
+        q = xd[:, :nh] if fused else xd[:, :nh].contiguous()
+        k, v = ln.paged.alloc_pages(n_pages, page, nkv, hd)
+        got = ln.paged.rope_store_kv(q, xd[:, nh:nh + nkv], xd[:, nh + nkv:], k, v, *batch, n_dims=nd, neox=neox, out=q)
+        assert got is q and np.array_equal(q.cpu().numpy().view(np.uint32), rot[:, :nh].view(np.uint32))
+        assert np.array_equal(xd[:, nh:].cpu().numpy(), x[:, nh:])
+        assert np.array_equal(k.cpu().numpy().view(np.uint16), c.k) and np.array_equal(v.cpu().numpy().view(np.uint16), c.v)

@@ -51,9 +51,9 @@ struct store_args {
     int page_sh;
 };
 
-// One thread per element of a row's heads (query, key, value heads in turn);
-// what a thread reads and converts alone is as in lnship16_rope and
-// lnship16_store_kv.
+// One thread per rotated pair, or other element, of a row's heads (query, key,
+// value heads in turn), as in lnship16_rope and lnship16_store_kv: a thread
+// writes what it alone has read, so that q_dst may be q.
 __global__ __launch_bounds__(k_block) void k_store_paged(store_args s, dev_tables T, unsigned long long *err) {
     const fmt16 F{T};
     const lnship_paged_kv &kv = s.kv;
@@ -72,32 +72,37 @@ __global__ __launch_bounds__(k_block) void k_store_paged(store_args s, dev_table
     const bool paged = id >= 0 && id < kv.n_pages;
     if (!paged && blockIdx.y == 0 && threadIdx.x == 0) index_fault(err, id);
     const float *cs = nd > 0 ? a.cos_sin + p * nd : nullptr;
-    const int64_t nq = a.n_head * hd, nk = kv.n_head_kv * hd;
-    for (int64_t i = (int64_t)blockIdx.y * k_block + threadIdx.x; i < nq + 2 * nk; i += (int64_t)gridDim.y * k_block) {
+    const int64_t pairs = nd / 2, of_head = hd - pairs;   // items of a query or key head
+    const int64_t nq = a.n_head * of_head, nk = kv.n_head_kv * of_head, nv = kv.n_head_kv * hd;
+    for (int64_t i = (int64_t)blockIdx.y * k_block + threadIdx.x; i < nq + nk + nv; i += (int64_t)gridDim.y * k_block) {
         const int part = i < nq ? 0 : i < nq + nk ? 1 : 2;
-        const int64_t e = part == 0 ? i : part == 1 ? i - nq : i - nq - nk;
-        const int64_t h = e / hd, d = e - h * hd;
+        const int64_t e = part == 0 ? i : part == 1 ? i - nq : i - nq - nk, items = part < 2 ? of_head : hd;
+        const int64_t h = e / items, j = e - h * items;
         const float *x = part == 0 ? a.q + t * a.q_ld : part == 1 ? a.k + t * a.k_ld : a.v + t * a.v_ld;
         x += h * hd;
-        float v = x[d];
-        if (part < 2 && nd > 0) {
-            if (d < nd) {
-                const int64_t half = nd / 2, j = a.neox ? d % half : d / 2;
-                int64_t i0, i1;
-                uint32_t r0, r1;
-                rope_pair(F, x, j, nd, a.neox, cs, i0, i1, r0, r1);
-                v = F.to(d == i0 ? r0 : r1);
-            } else {
-                v = F.to(F.from(v));
-            }
+        // the thread's element, or pair (all loads before the stores)
+        const bool pair = part < 2 && j < pairs;
+        int64_t d0 = part < 2 ? j + pairs : j, d1 = d0;
+        float v0, v1;
+        if (pair) {
+            uint32_t r0, r1;
+            rope_pair(F, x, j, nd, a.neox, cs, d0, d1, r0, r1);
+            v0 = F.to(r0);
+            v1 = F.to(r1);
+        } else {
+            v0 = v1 = part < 2 && nd > 0 ? F.to(F.from(x[d0])) : x[d0];
         }
         if (part == 0) {
-            a.q_dst[t * a.q_dst_ld + e] = v;
+            float *o = a.q_dst + t * a.q_dst_ld + h * hd;
+            o[d0] = v0;
+            if (pair) o[d1] = v1;
         } else if (paged) {
-            const int64_t base = (id * kv.n_head_kv + h) * kv.page * hd;
-            uint16_t *o = part == 1 ? kv.k_pages + base + ((d >> 3) * kv.page + c) * 8 + (d & 7)
-                                    : kv.v_pages + base + ((c >> 3) * hd + d) * 8 + (c & 7);
-            *o = (uint16_t)F.from(__half2float(__float2half_rn(v)));
+            const uint16_t c0 = (uint16_t)F.from(__half2float(__float2half_rn(v0)));
+            const uint16_t c1 = (uint16_t)F.from(__half2float(__float2half_rn(v1)));
+            uint16_t *o = (part == 1 ? kv.k_pages : kv.v_pages) + (id * kv.n_head_kv + h) * kv.page * hd;
+            auto at = [&](int64_t d) { return part == 1 ? ((d >> 3) * kv.page + c) * 8 + (d & 7) : ((c >> 3) * hd + d) * 8 + (c & 7); };
+            o[at(d0)] = c0;
+            if (pair) o[at(d1)] = c1;
         }
     }
 }
@@ -1368,7 +1373,8 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
         LNSHIP_HIP(hipGetLastError());
         return 0;
     }
-    const int64_t y = std::min<int64_t>((nq + 2 * nk + k_block - 1) / k_block, 65535);
+    const int64_t items = (a->n_head + kv->n_head_kv) * (kv->head_dim - a->rope_n_dims / 2) + nk;
+    const int64_t y = std::min<int64_t>((items + k_block - 1) / k_block, 65535);
     hipLaunchKernelGGL(k_store_paged, dim3((unsigned)kv->ntok, (unsigned)y), dim3(k_block), 0, (hipStream_t)stream, s,
                        st->T, st->index_err);
     LNSHIP_HIP(hipGetLastError());

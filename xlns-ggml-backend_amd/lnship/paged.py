@@ -75,7 +75,7 @@ def rope_store_kv(q, k, v, k_pages, v_pages, page, table, q_start, kv_len, cos_s
     values into the pages (in place).  q [ntok, n_head, head_dim] (or None), k,
     v [ntok, n_head_kv, head_dim] float32: arrays, or the parts of a fused
     q|k|v product's rows; cos_sin [n_pos, n_dims / 2, 2] float32 (None with
-    n_dims 0: nothing is rotated).  Returns the rotated queries."""
+    n_dims 0: nothing is rotated).  Returns the rotated queries.  out may be q."""
     ntok = k.shape[0]
     kv, dev, nkv, hd = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
     stream = current_stream(dev)
