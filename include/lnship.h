@@ -432,7 +432,8 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
  * as pairs of IEEE halves on the matrix cores, 22 bits of each operand; the
  * relative error is about 1e-6.
  * Cells of a page outside [0, n_pages) or past the table's end count as
- * hidden and are recorded (lnship_index_error).  dst may be q.
+ * hidden and, if a row's window holds them, are recorded (lnship_index_error):
+ * pages that lie behind every new token's window may be freed.  dst may be q.
  * work: lnship16_attn_paged_work bytes of device memory, 16-byte aligned,
  * that nothing else uses until the call has run (calls on two streams, or
  * graphs that may replay side by side, need one each); it may be null where

@@ -47,3 +47,40 @@ def test_queries_rotated_in_place(ln, T, nh, nkv, hd, nd, neox):
         assert got is q and np.array_equal(q.cpu().numpy().view(np.uint32), rot[:, :nh].view(np.uint32))
         assert np.array_equal(xd[:, nh:].cpu().numpy(), x[:, nh:])
         assert np.array_equal(k.cpu().numpy().view(np.uint16), c.k) and np.array_equal(v.cpu().numpy().view(np.uint16), c.v)
+
+# ---- pages behind a window ---------------------------------------------------------------
+
+FREED = [
+    # q_len, kv_len, page, heads, kv heads, dim, window, cells of the table
+    ([1], [1000], 16, 12, 4, 64, 33, 0),
+    ([1, 1, 1], [1000, 517, 40], 32, 8, 2, 128, 100, 0),
+    ([1] * 40, [300 + 29 * i for i in range(40)], 16, 16, 8, 128, 65, 0),
+    ([9, 3], [700, 400], 16, 4, 2, 200, 50, 0),
+    ([40, 90], [300, 400], 16, 4, 2, 64, 17, 1 << 14),
+    ([70], [700], 32, 8, 2, 128, 111, 1 << 14),
+    ([520], [900], 16, 8, 2, 64, 200, 1 << 13),
+    ([600, 300], [1200, 1111], 32, 4, 2, 128, 77, 1 << 13),
+]
+
+
+@pytest.mark.parametrize("q_len,kv_len,page,nh,nkv,hd,window,cells", FREED)
+def test_pages_behind_the_window_may_be_freed(ln, q_len, kv_len, page, nh, nkv, hd, window, cells):
+    """A page whose cells no new token sees is not looked at: its number may be -1, and is no error."""
+    print(f"\n[attn] {q_len} {kv_len} page {page} {nh}/{nkv}x{hd} window {window} freed", flush=True)
+    rng = np.random.default_rng(window)
+    q, c, table, keys, vals = attn_case(rng, q_len, kv_len, page, nh, nkv, hd)
+    want = run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells).cpu().numpy()
+    first = [max(0, m - n - window + 1) // page for n, m in zip(q_len, kv_len)]
+    assert any(first)
+    for s, f in enumerate(first):
+        table[s, :f] = -1
+    index_error(ln)
+    got = run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells).cpu().numpy()
+    assert index_error(ln)[0] == 0
+    assert np.array_equal(got, want)
+    check_attn(got, q, q_len, kv_len, keys, vals, window)
+    # the first page that is seen counts
+    s = int(np.argmax(first))
+    table[s, first[s]] = -5
+    run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells)
+    assert index_error(ln) == (1, -5)

@@ -422,6 +422,7 @@ struct row_tile {
     int sq, t0, rows, r0;   // its sequence, that one's first token and rows, the tile's first row
     int pos0;               // position of token t0
     int c0, c1;             // cells [c0, c1) may be seen, c0 a multiple of 64
+    int seen;               // the first cell that is (c1: none): pages before it may be any
     int blocks, per;        // blocks of 64 of them, and of a split
 };
 // r0 < 0: the tile has no rows.
@@ -444,7 +445,8 @@ __device__ __forceinline__ row_tile find_tile(const attn_paged_args &a, int tile
     if (err && pos0 + last >= cells && threadIdx.x == 0) index_fault(err, pos0 + last);
     t.pos0 = (int)min(pos0, ((int64_t)1 << 31) - 1 - t.rows);
     t.c1 = (int)max(min((int64_t)t.pos0 + last + 1, cells), (int64_t)0);
-    t.c0 = a.window > 0 ? max(0, min(t.pos0 + first - a.window + 1, t.c1)) & ~63 : 0;
+    t.seen = a.window > 0 ? max(0, min(t.pos0 + first - a.window + 1, t.c1)) : 0;
+    t.c0 = t.seen & ~63;
     t.blocks = (t.c1 - t.c0 + 63) >> 6;
     t.per = max((t.blocks + a.splits - 1) / a.splits, a.min_per);
     return t;
@@ -560,7 +562,10 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : NB <= 4 ? 3 : 1) void k_attn
     bool vok = false;
     auto sound_v = [&](int cb) {
         vok = cb + vcell < cend && sound(vid);
-        if (cb + vcell < cend && !vok) index_fault(err, vid);
+        if (cb + vcell < cend && !vok) {
+            asm volatile("");   // (few blocks need the rest)
+            if (cb + vcell + 7 >= T.seen) index_fault(err, vid);
+        }
     };
     if (cb < cend) {
         kid = page_of(cb + kcell);
@@ -728,7 +733,7 @@ struct tile_of {
 };
 
 // A workgroup of NT threads that makes such tiles of the cells [.., cend) of one
-// sequence: a thread loads its units' codes ahead, then decodes them.  Unit u of
+// sequence, of which those before `seen` are seen by no row: a thread loads its units' codes ahead, then decodes them.  Unit u of
 // the keys: dims u / C * 8.., cell u % C of the tile's C (the same for all of a
 // thread's); of the values: cells u / HD * 8.., dim u % HD.
 template <int NB, int NT, int C = 64>
@@ -737,14 +742,14 @@ struct tile_maker {
     const int32_t *table;
     const uint16_t *kbase, *vbase;
     int64_t page_codes;
-    int cend, page_sh, page, hd, n_pages, tid;
+    int seen, cend, page_sh, page, hd, n_pages, tid;
     unsigned long long *err;
     uint4 kc[UT], vc[UT];
     int kid, vid[UT];   // the pages of the next units to load
 
-    __device__ __forceinline__ tile_maker(const lnship_paged_kv &kv, int sq, int kvh, int sh, int end, int thread,
+    __device__ __forceinline__ tile_maker(const lnship_paged_kv &kv, int sq, int kvh, int sh, int first_seen, int end, int thread,
                                           unsigned long long *e)
-        : table(kv.table + (int64_t)sq * kv.table_ld), cend(end), page_sh(sh), page((int)kv.page), hd((int)kv.head_dim),
+        : table(kv.table + (int64_t)sq * kv.table_ld), seen(first_seen), cend(end), page_sh(sh), page((int)kv.page), hd((int)kv.head_dim),
           n_pages((int)kv.n_pages), tid(thread), err(e) {
         const int64_t head_codes = (int64_t)page * hd;
         page_codes = kv.n_head_kv * head_codes;
@@ -781,9 +786,13 @@ struct tile_maker {
         uint32_t ok = 0;
 #pragma unroll
         for (int i = 0; i < UT; i++) {
-            const bool in = has(i) && cb + (tid + i * NT) / HD * 8 < cend;
+            const int c = cb + (tid + i * NT) / HD * 8;
+            const bool in = has(i) && c < cend;
             if (in && sound(vid[i])) ok |= 1u << i;
-            else if (in) index_fault(err, vid[i]);
+            else if (in) {
+                asm volatile("");   // (few tiles need the rest)
+                if (c + 7 >= seen) index_fault(err, vid[i]);
+            }
         }
         return ok;
     }
@@ -848,9 +857,9 @@ __global__ __launch_bounds__(256) void k_attn_decode(attn_paged_args a, unsigned
         if (end <= start) continue;
         // the first cell that the sequence's first token sees
         const int64_t first = kv.kv_len[sq] - (end - start) - a.window + 1;
-        const int lo = a.window > 0 ? (int)(min(max(first, (int64_t)0), (int64_t)cend) >> 6) : 0;
-        tile_maker<NB, 256> t(kv, sq, kvh, a.page_sh, cend, threadIdx.x, err);
-        for (int i = lo + (int)blockIdx.x; i * 64 < cend; i += (int)gridDim.x) {
+        const int seen = a.window > 0 ? (int)min(max(first, (int64_t)0), (int64_t)cend) : 0;
+        tile_maker<NB, 256> t(kv, sq, kvh, a.page_sh, seen, cend, threadIdx.x, err);
+        for (int i = (seen >> 6) + (int)blockIdx.x; i * 64 < cend; i += (int)gridDim.x) {
             t.pages(i * 64);
             t.load(i * 64);
             const uint32_t ok = t.sound_pages(i * 64);
@@ -1076,7 +1085,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void k_attn_chunk(attn_pa
         // to 27 tokens behind 640 to 5125 cells, 32 heads of 128 on 8: 249 us, all waves
         // decoding 284.)
         if (wave >= NW / 2) {
-            tile_maker<NB, NW * 32, C> maker(a.kv, T.sq, kvh, a.page_sh, cend, tid - NW * 32, err);
+            tile_maker<NB, NW * 32, C> maker(a.kv, T.sq, kvh, a.page_sh, T.seen, cend, tid - NW * 32, err);
             maker.first(cbeg, cells(0), s_ok[0]);
             lds_barrier();
             int buf = 0;
@@ -1097,7 +1106,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void k_attn_chunk(attn_pa
         r.write(a, T, split);
         return;
     }
-    tile_maker<NB, NW * 64, C> maker(a.kv, T.sq, kvh, a.page_sh, cend, tid, err);
+    tile_maker<NB, NW * 64, C> maker(a.kv, T.sq, kvh, a.page_sh, T.seen, cend, tid, err);
     maker.first(cbeg, cells(0), s_ok[0]);
     r.place(a, T, kvh, T.r0 + wave * 32);
     r.load(a);
