@@ -405,7 +405,8 @@ typedef struct lnship_paged_kv {
  * (lnship_rope_table's layout, n_pos positions).  A position below 0, past the
  * table's cells or (rotating) not below n_pos, and a page outside
  * [0, n_pages), is recorded (lnship_index_error) and its row, or what it has
- * in that page, is skipped.  q_dst may be q (with q_dst_ld = q_ld).  Two rows of one call never have the same cell
+ * in that page, is skipped.  q_dst may be q (with q_dst_ld = q_ld);
+ * otherwise it shares no memory with q (refused), k or v.  Two rows of one call never have the same cell
  * unless the table names a page twice; then which of them stays is not said. */
 typedef struct lnship_paged_store_args {
     const float *q, *k, *v;
@@ -433,7 +434,8 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
  * relative error is about 1e-6.
  * Cells of a page outside [0, n_pages) or past the table's end count as
  * hidden and, if a row's window holds them, are recorded (lnship_index_error):
- * pages that lie behind every new token's window may be freed.  dst may be q.
+ * pages that lie behind every new token's window may be freed.
+ * dst may be q (with dst_ld = q_ld); other overlap is refused.
  * work: lnship16_attn_paged_work bytes of device memory, 16-byte aligned,
  * that nothing else uses until the call has run (calls on two streams, or
  * graphs that may replay side by side, need one each); it may be null where

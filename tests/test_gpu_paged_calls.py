@@ -48,6 +48,31 @@ def test_queries_rotated_in_place(ln, T, nh, nkv, hd, nd, neox):
         assert np.array_equal(xd[:, nh:].cpu().numpy(), x[:, nh:])
         assert np.array_equal(k.cpu().numpy().view(np.uint16), c.k) and np.array_equal(v.cpu().numpy().view(np.uint16), c.v)
 
+def test_outputs_that_overlap_inputs_are_refused(ln):
+    """Shifted or otherwise strided views of q, and k or v, as out; nothing is written."""
+    T, nh, nkv, hd = 3, 2, 1, 32
+    k, v = ln.paged.alloc_pages(2, 16, nkv, hd)
+    batch = (16, dev(np.int32([[0, 1]])), dev(np.int32([0, T])), dev(np.int32([T])))
+    buf = torch.ones(T * 5 * hd + 64, device="cuda")
+    q = torch.as_strided(buf, (T, nh, hd), (4 * hd, hd, 1), 0)
+    x = torch.ones((T, 2 * nkv, hd), device="cuda")
+    for out in (torch.as_strided(buf, (T, nh, hd), (4 * hd, hd, 1), hd), torch.as_strided(buf, (T, nh, hd), (5 * hd, hd, 1), 0)):
+        with pytest.raises(ln.LnshipError, match="overlaps q"):
+            ln.paged.rope_store_kv(q, x[:, :1], x[:, 1:], k, v, *batch, None, n_dims=0, out=out)
+        with pytest.raises(ln.LnshipError, match="overlaps q"):
+            ln.paged.attention(q, k, v, *batch, 1.0, out=out)
+    wide = torch.ones((T, nh + 2 * nkv, hd), device="cuda")
+    for at in (1, 2):
+        with pytest.raises(ln.LnshipError, match="overlaps k or v"):
+            ln.paged.rope_store_kv(q, wide[:, 2:3], wide[:, 3:], k, v, *batch, None, n_dims=0, out=wide[:, at:at + nh])
+    torch.cuda.synchronize()
+    assert (buf == 1).all() and (wide == 1).all() and not k.any() and not v.any()
+    # in the gaps of q's rows, and of the fused rows
+    gap = torch.as_strided(buf, (T, nh, hd), (4 * hd, hd, 1), 2 * hd)
+    ln.paged.attention(q, k, v, *batch, 1.0, out=gap)
+    assert (gap == 0).all() and (q == 1).all()
+
+
 # ---- pages behind a window ---------------------------------------------------------------
 
 FREED = [

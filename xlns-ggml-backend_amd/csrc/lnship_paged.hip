@@ -1210,6 +1210,17 @@ static int check_paged(const lnship_paged_kv *kv, bool ptrs) {
     return 0;
 }
 
+// Whether out's rows (n of w floats, out_ld apart) are x's, or share no memory with
+// them: of rows equally far apart, one may lie in the gaps of the other.
+static bool same_or_apart(const float *x, int64_t x_ld, const float *out, int64_t out_ld, int64_t w, int64_t n) {
+    if (x == out && (x_ld == out_ld || n == 1)) return true;
+    const int64_t a = (int64_t)(uintptr_t)x, b = (int64_t)(uintptr_t)out, bytes = w * 4;
+    if (a + (n - 1) * x_ld * 4 + bytes <= b || b + (n - 1) * out_ld * 4 + bytes <= a) return true;
+    if (x_ld != out_ld) return false;
+    const int64_t step = x_ld * 4, d = ((b - a) % step + step) % step;
+    return d >= bytes && step - d >= bytes;
+}
+
 static int log2_of(int64_t page) {
     int sh = 0;
     while ((int64_t)1 << sh < page) sh++;
@@ -1358,6 +1369,8 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
     if (kv->ntok == 0 || kv->n_seq == 0) return 0;
     if (!a->k || !a->v || (a->n_head && (!a->q || !a->q_dst)) || (a->rope_n_dims && a->n_pos && !a->cos_sin))
         return fail(LNSHIP_EINVAL, "rope_store_kv_paged: null pointer%s");
+    if (a->n_head && !same_or_apart(a->q, a->q_ld, a->q_dst, s.a.q_dst_ld, nq, kv->ntok))
+        return fail(LNSHIP_EINVAL, "rope_store_kv_paged: q_dst overlaps q%s");
     device_state *st = state();
     if (!st) return LNSHIP_ENOINIT;
     // 16-byte loads and stores, and eight dims a thread
@@ -1409,6 +1422,8 @@ int lnship16_attn_paged(const lnship_paged_kv *kv, const lnship_paged_attn_args 
     if (q_ld < nq || dst_ld < nq) return fail(LNSHIP_EINVAL, "attn_paged: bad shape%s");
     if (kv->ntok == 0 || kv->n_seq == 0) return 0;
     if (!a->q || !a->dst) return fail(LNSHIP_EINVAL, "attn_paged: null pointer%s");
+    if (!same_or_apart(a->q, q_ld, a->dst, dst_ld, nq, kv->ntok))
+        return fail(LNSHIP_EINVAL, "attn_paged: dst overlaps q%s");
     device_state *st = state();
     if (!st) return LNSHIP_ENOINIT;
     const int64_t rep = a->n_head / kv->n_head_kv;

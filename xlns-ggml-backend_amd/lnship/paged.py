@@ -70,6 +70,15 @@ def _ld(t, name, ntok, heads, dim, dev):
     return s0 if ntok > 1 else max(s0, heads * dim)
 
 
+def _apart(a, a_ld, a_w, b, b_ld, b_w, n):
+    """Whether n rows of a_w floats from address a on, a_ld floats apart, share no memory with n of b's: of
+    rows equally far apart, one may lie in the gaps of the other."""
+    if a + ((n - 1) * a_ld + a_w) * 4 <= b or b + ((n - 1) * b_ld + b_w) * 4 <= a:
+        return True
+    d = (b - a) % (a_ld * 4)
+    return a_ld == b_ld and a_w * 4 <= d <= (a_ld - b_w) * 4
+
+
 def rope_store_kv(q, k, v, k_pages, v_pages, page, table, q_start, kv_len, cos_sin, n_dims=None, neox=False, out=None):
     """Rotates the new tokens' queries and keys and stores their keys and
     values into the pages (in place).  q [ntok, n_head, head_dim] (or None), k,
@@ -88,14 +97,18 @@ def rope_store_kv(q, k, v, k_pages, v_pages, page, table, q_start, kv_len, cos_s
             _no("cos_sin must be contiguous float32 [n_pos, n_dims / 2, 2] on the pages' device")
         cs, n_pos = cos_sin.data_ptr(), cos_sin.shape[0]
     nh = q_ld = out_ld = q_at = out_at = 0
+    k_at, v_at, k_ld, v_ld = k.data_ptr(), v.data_ptr(), _ld(k, "k", ntok, nkv, hd, dev), _ld(v, "v", ntok, nkv, hd, dev)
     if q is not None:
         nh = q.shape[1]
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty((ntok, nh, hd), dtype=_F32, device=k_pages.device)
         q_ld, out_ld = _ld(q, "q", ntok, nh, hd, dev), _ld(out, "out", ntok, nh, hd, dev)
         q_at, out_at = q.data_ptr(), out.data_ptr()
-    a = _STORE.pack(q_at, k.data_ptr(), v.data_ptr(), q_ld, _ld(k, "k", ntok, nkv, hd, dev),
-                    _ld(v, "v", ntok, nkv, hd, dev), nh, n_dims, neox, cs, n_pos, out_at, out_ld)
+        if given and ntok and not (_apart(out_at, out_ld, nh * hd, k_at, k_ld, nkv * hd, ntok) and
+                                   _apart(out_at, out_ld, nh * hd, v_at, v_ld, nkv * hd, ntok)):
+            _no("out overlaps k or v")
+    a = _STORE.pack(q_at, k_at, v_at, q_ld, k_ld, v_ld, nh, n_dims, neox, cs, n_pos, out_at, out_ld)
     check(lib().lnship16_rope_store_kv_paged(kv, a, stream))
     return out
 
