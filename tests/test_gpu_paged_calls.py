@@ -109,3 +109,66 @@ def test_pages_behind_the_window_may_be_freed(ln, q_len, kv_len, page, nh, nkv, 
     table[s, first[s]] = -5
     run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells)
     assert index_error(ln) == (1, -5)
+
+
+# ---- many sequences ----------------------------------------------------------------------
+
+def many(rng, n_seq, most, past):
+    """Lengths of n_seq sequences, some without new tokens, those beside multiples of 64 and 79 among them."""
+    q_len = rng.integers(0, most + 1, n_seq)
+    for at in (0, 63, 64, 65, 79, 128, 4095, 4096, n_seq - 1):
+        q_len[min(at, n_seq - 1)] = at % 2
+    q_len[n_seq // 2] = most
+    return q_len.tolist(), (q_len + rng.integers(0, past, n_seq)).tolist()
+
+
+def check_some(got, q, q_len, kv_len, keys, vals, rng, window=0):
+    """check_attn of sequences drawn at random and of those at the ends of a search's rounds."""
+    n_seq, at = len(q_len), np.concatenate([[0], np.cumsum(q_len)])
+    some = set(rng.choice(n_seq, min(n_seq, 60), replace=False).tolist())
+    some |= {s for b in (0, 64, 79, 128, 4096, n_seq) for s in (b - 1, b, b + 1) if 0 <= s < n_seq}
+    for s in some:
+        check_attn(got[at[s]:at[s + 1]], q[at[s]:at[s + 1]], [q_len[s]], [kv_len[s]], [keys[s]], [vals[s]], window)
+
+
+@pytest.mark.parametrize("n_seq,most,nh,nkv,hd,cells", [
+    (64, 3, 4, 2, 64, 0), (65, 3, 4, 2, 64, 0), (129, 3, 4, 2, 128, 0), (300, 1, 32, 8, 64, 0), (5000, 2, 2, 1, 8, 0),
+    # chunks: each workgroup decodes; decoded before
+    (65, 20, 8, 1, 16, 1 << 13), (130, 10, 32, 2, 72, 1 << 11), (4200, 2, 128, 1, 8, 1 << 9),
+    (70, 20, 64, 1, 8, 1 << 10), (129, 16, 64, 1, 40, 1 << 10)])
+def test_attention_of_many_sequences(ln, n_seq, most, nh, nkv, hd, cells):
+    print(f"\n[attn] {n_seq} sequences of up to {most} tokens, {nh}/{nkv}x{hd}, {cells} cells", flush=True)
+    rng = np.random.default_rng(n_seq + hd)
+    q_len, kv_len = many(rng, n_seq, most, 60)
+    q, c, table, keys, vals = attn_case(rng, q_len, kv_len, 16, nh, nkv, hd)
+    for window in (0, 21):
+        got = run_attn(ln, q, c, table, q_len, kv_len, window, cells=cells).cpu().numpy()
+        assert np.isfinite(got).all()
+        check_some(got, q, q_len, kv_len, keys, vals, rng, window)
+
+
+@pytest.mark.parametrize("n_seq,hd", [(64, 8), (65, 8), (129, 64), (1000, 16), (5000, 8)])
+def test_stores_of_many_sequences(ln, n_seq, hd):
+    """Fewer than 2^19 values: the kernel that looks a row's sequence up with a wave."""
+    print(f"\n[store] {n_seq} sequences x {hd}", flush=True)
+    rng = np.random.default_rng(n_seq)
+    q_len, kv_len = many(rng, n_seq, 3, 40)
+    T, page = sum(q_len), 16
+    assert T * 3 * hd < 1 << 19
+    x = rng.standard_normal((T, 3, hd)).astype(np.float32)
+    cs = rope_table(ln, max(kv_len) + 1, hd)
+    table, n_pages = R.tables(rng, kv_len, page)
+    k, v = ln.paged.alloc_pages(n_pages, page, 1, hd)
+    xd = dev(x)
+    out = ln.paged.rope_store_kv(xd[:, :1], xd[:, 1:2], xd[:, 2:], k, v, page, dev(table), dev(starts(q_len)),
+                                 dev(np.int32(kv_len)), dev(cs))
+    pos = positions(q_len, kv_len)
+    rot = R.rope(x[:, :2], cs[np.concatenate(pos)], False, hd)
+    kc, vc = R.store_codes(rot[:, 1:]), R.store_codes(x[:, 2:])
+    c = R.Cache(n_pages, page, 1, hd, fill=0)
+    at = 0
+    for s, p in enumerate(pos):
+        c.put(table[s], p, kc[at:at + len(p)], vc[at:at + len(p)])
+        at += len(p)
+    assert np.array_equal(out.cpu().numpy().view(np.uint32), rot[:, :1].view(np.uint32))
+    assert np.array_equal(k.cpu().numpy().view(np.uint16), c.k) and np.array_equal(v.cpu().numpy().view(np.uint16), c.v)

@@ -70,3 +70,27 @@ def test_a_min_p_above_one_leaves_the_first_token(ln, vocab):
         for m in (1.5, float("inf")):
             tok, prob = draws(ln, x, u, **kw, m=np.full(rows, m))
             assert np.array_equal(tok, first) and (prob == 1.0).all(), (kw, m)
+
+
+@pytest.mark.parametrize("vocab", [262145, (1 << 19) - 1, 1 << 19])
+@pytest.mark.parametrize("kind", ["smooth", "flat", "alike", "two levels"])
+def test_the_largest_vocabularies(ln, vocab, kind):
+    """Up to 512 segments, the fewest bits of a bin's weight and its sums' largest."""
+    print(f"\n[draw] {vocab} {kind}", flush=True)
+    rng = np.random.default_rng(vocab)
+    rows = 10
+    x = rng.standard_normal((rows, vocab))
+    x = {"smooth": x * 2.5, "flat": x * 0.01, "alike": x * 0 - 3, "two levels": np.where(x > 2, 6.0, 0.0) + x * 1e-4}[kind]
+    x = x.astype(np.float32)
+    u = np.concatenate([[0.0, 0.9999999], rng.random(rows - 2)])
+    p = np.concatenate([[1e-7, 0.9999999, 1.0], rng.random(rows - 3)])
+    m = np.where(np.arange(rows) % 4 == 3, 0.02, 0.0)
+    k = np.where(np.arange(rows) % 3 == 0, 50, 0)
+    check(draws(ln, x, u, None, None, p, m), x, u, None, None, p, m)
+    check(draws(ln, x, u, None, k, p, m), x, u, None, k, p, m)
+    check(draws(ln, x, u), x, u, None, None, None, None)
+
+
+def test_a_larger_vocabulary_is_refused(ln):
+    with pytest.raises(ln.LnshipError, match="too large"):
+        ln.sample(torch.zeros((1, (1 << 19) + 1), device="cuda"), torch.zeros(1, device="cuda"))
