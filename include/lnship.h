@@ -429,9 +429,13 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
  * 2^(2047/128)); q and dst are F32, and every sum is a sum of real numbers in
  * 32 bits, not a chain of LNS additions: such a chain takes two dependent
  * steps a cell (lnship16_attn_decode runs them), which a long cache cannot
- * afford, and its result is what the chain rounds.  Keys and values are read
- * as pairs of IEEE halves on the matrix cores, 22 bits of each operand; the
- * relative error is about 1e-6.
+ * afford, and its result is what the chain rounds.  Keys, values, queries
+ * and weights go through the matrix cores as pairs of IEEE halves, 22 bits of
+ * each, and the relative error is about 1e-6.  A half's steps have an end: a
+ * key or value is off by up to 2^-36 (so less exact below 2^-14), a query by
+ * as much of its head's largest, a weight by up to 2^-34 of its row's
+ * largest.  Where one cell outweighs all others by 2^20 and its value is near
+ * zero, what the others add up to is therefore less exact than F32 sums.
  * Cells of a page outside [0, n_pages) or past the table's end count as
  * hidden and, if a row's window holds them, are recorded (lnship_index_error):
  * pages that lie behind every new token's window may be freed.
