@@ -94,3 +94,19 @@ def test_the_largest_vocabularies(ln, vocab, kind):
 def test_a_larger_vocabulary_is_refused(ln):
     with pytest.raises(ln.LnshipError, match="too large"):
         ln.sample(torch.zeros((1, (1 << 19) + 1), device="cuda"), torch.zeros(1, device="cuda"))
+
+
+@pytest.mark.parametrize("vocab", [40000, 131075])
+@pytest.mark.parametrize("first", [-np.inf, np.nan, -300.0, 300.0])
+def test_rows_whose_first_logits_are_unlike_the_rest(ln, vocab, first):
+    """A long row's bins are counted from the largest of its first 16384 logits; here none of those is a
+    number, or all lie far from the rest."""
+    rng = np.random.default_rng(vocab)
+    rows = 8
+    x = (rng.standard_normal((rows, vocab)) * 2.5).astype(np.float32)
+    x[:, :17000] = first
+    x[::2, 123::5000] = first        # in the rest too
+    u = rng.random(rows)
+    for kw in ({"p": 0.9}, {"k": 40}, {"k": 40, "p": 0.7}, {"p": 0.99, "m": 0.01}, {"k": 3000}):
+        a = [np.full(rows, kw[n]) if n in kw else None for n in ("T", "k", "p", "m")]
+        check(draws(ln, x, u, *a), x, u, *a)
