@@ -469,21 +469,22 @@ int64_t lnship16_attn_paged_work(const lnship_paged_kv *kv, int64_t n_head);
  * For each of n_rows rows of n_vocab F32 logits (row r at logits + r * ld) one
  * token, from the uniform random number u[r] in [0, 1).  With x_max the row's
  * largest logit and T its temperature, token i weighs e^((x_i - x_max) / T).
- * Tokens are ranked by logit, equal ones by index.  Kept are: the first
- * top_k; of these the shortest beginning whose weights sum to at least top_p
- * of theirs all; of these the ones that weigh at least min_p; the first token
- * always.  Drawn is the first token, by index, at which the running sum of the
- * kept weights exceeds u times their sum; probs (optional) receives its weight
- * over that sum.  T not above 0: the first token by rank, with probability 1.
- * temperature, top_k, top_p, min_p: n_rows values on the device, or null (1,
- * and no limits); top_k <= 0, top_p >= 1, min_p <= 0 and NaN set no limit.  u
- * outside [0, 1) counts as the nearer end, NaN as 0.  A NaN logit is never
- * drawn; with an infinite largest logit only its equals weigh anything; a row
- * without any logit above -inf gets token -1 and probability 0.  Weights are
- * summed as integers (units of 2^-40), so the draw does not depend on an order
- * of additions; a weight is exact to 2^-32.  n_vocab up to 2^19.  A row whose
- * top_k is above 1024, or with thousands of equal logits at a limit, takes
- * several times as long as another.  No LNS arithmetic, and no counterpart in
+ * Tokens are ranked by logit, equal ones by index.  Kept are: the first top_k;
+ * of these the shortest beginning whose weights sum to at least top_p of
+ * theirs all; of these the ones that weigh at least min_p; the first token
+ * always (a min_p above 1 leaves that one alone).  Drawn is the first token,
+ * by index, at which the running sum of the kept weights exceeds u times their
+ * sum; probs (optional) receives its weight over that sum.  T not above 0: the
+ * first token by rank, with probability 1. temperature, top_k, top_p, min_p:
+ * n_rows values on the device, or null (1, and no limits); top_k <= 0, top_p
+ * >= 1, min_p <= 0 and NaN set no limit.  u outside [0, 1) counts as the
+ * nearer end, NaN as 0.  A NaN logit is never drawn; with an infinite largest
+ * logit only its equals weigh anything; a row without any logit above -inf
+ * gets token -1 and probability 0.  Weights are summed as integers (units of
+ * 2^-40), so the draw does not depend on an order of additions; a weight is
+ * exact to 2^-32.  n_vocab up to 2^19.  A row whose top_k is above 1024, or
+ * with thousands of equal logits at a limit, takes ten to twenty times as long
+ * as another.  No LNS arithmetic, and no counterpart in
  * the reference, which samples on the host. */
 typedef struct lnship_sample_args {
     const float *logits;
@@ -539,8 +540,9 @@ int lnship_set_rows(const float *src, const int64_t src_ne[4], const int64_t src
                     int ids_i64, const int64_t ids_ne[3], const int64_t ids_nb[3], void *dst, int dst_type,
                     const int64_t dst_ne[4], const int64_t dst_nb[4], void *stream);
 /* Waits for stream, then returns 1 (and one offending index in *bad_index)
- * if a get_rows / set_rows on this device met an index out of range since
- * the last call, else 0; clears the record.  The reference asserts on such
+ * if a call on this device (get_rows, set_rows, a KV store, a paged-cache
+ * operator) met an index, position or page out of range since the last call,
+ * else 0; clears the record.  The reference asserts on such
  * an index (src/lns-ops.cpp:1024). */
 int lnship_index_error(int64_t *bad_index, void *stream);
 

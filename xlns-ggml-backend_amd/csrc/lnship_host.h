@@ -32,7 +32,7 @@ struct device_state {
     size_t scratch_size = 0;
     std::vector<void *> retired;   // outgrown scratch blocks, kept for captured graphs
     void *fixed_scratch = nullptr;  // this device's copy of `scratch` (below), from hipGetSymbolAddress
-    // index check of get_rows / set_rows: [0] set to 1 by the first
+    // index check (rows, positions, pages): [0] set to 1 by the first
     // out-of-range index since the last lnship_index_error, [1] that index
     unsigned long long *index_err = nullptr;
 };

@@ -166,11 +166,13 @@ constexpr int k_store_rows = 8;   // rows of a workgroup at most
 // one item, whose cells then fill cache lines in one store.  The conversions, the
 // Gaussian logs and the decoded values come from tables in LDS: from memory each
 // is a gather that costs a cache line a lane.  A row's cosines and sines are
-// converted once for all heads.  Bound by the arithmetic of the codes, some 40
-// instructions a pair and 60 for its conversions, and by the scattered stores:
-// 11414 rows of 32 heads of 64 on 8 in 75 us, 3.4 TB/s of what is read and written
-// (with rows spread over all XCDs 94: the caches' lines are then written in parts;
-// with registers for six waves a SIMD in place of eight 80).
+// converted once for all heads.  Bound by VALU issue, 137 instructions a pair with
+// its conversions, its value or cell and its share of the values' stores (counted:
+// 69 % of the kernel's cycles, 87 % of those in which a CU has work; the rest are the
+// tables and the end): 11414 rows of 32 heads of 64 on 8 in 70 us, 3.7 TB/s of what is
+// read and written.  With rows spread over all XCDs it took 1.2 times as long (the
+// caches' lines are then written in parts), with registers for six waves a SIMD in
+// place of eight 1.04 times.
 template <bool NEOX>
 __global__ __launch_bounds__(k_block, 8) void k_store_paged_rows(store_args s, int row_sh, dev_tables T,
                                                               unsigned long long *err) {
@@ -1089,8 +1091,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void k_attn_chunk(attn_pa
     };
     if (NW == 8 && T.rows - T.r0 <= NW * 16) {
         // Rows for half of the waves: the others decode meanwhile.  (33 sequences of 6
-        // to 27 tokens behind 640 to 5125 cells, 32 heads of 128 on 8: 249 us, all waves
-        // decoding 284.)
+        // to 27 tokens behind 640 to 5125 cells, 32 heads of 128 on 8: 244 to 259 us, all
+        // waves decoding 283 to 296.)
         if (wave >= NW / 2) {
             tile_maker<NB, NW * 32, C> maker(a.kv, T.sq, kvh, a.page_sh, T.seen, cend, tid - NW * 32, err);
             maker.first(cbeg, cells(0), s_ok[0]);
@@ -1243,36 +1245,47 @@ struct attn_plan {
     // the workspace: bytes of the splits' parts, of the decoded tiles, of their flags
     int64_t parts_bytes, pre_bytes, ok_bytes, pre_tiles;
 };
+// The rules go by what the host knows, the rows of all sequences and the tables'
+// cells, so that a captured graph runs the same kernels whatever its lengths.  They
+// were measured on batches of sequences that are alike, behind tables as wide as the
+// longest.  What they cost elsewhere: one kernel serves single tokens and a chunk in
+// one call (32 heads of 128 on 8, 64 tokens over 4000 cells and a chunk behind 4000: of
+// 512 tokens 579 us, apart 232 and 146; of 4096 1675, apart 230 and 1021), and a wide
+// table stands for long caches (one token over 300 cells, 9 heads of 64 on 3, behind a
+// table of 131072 14.4 us, of 304 9.2).
+//
 // Few rows a sequence, or little work: k_attn_paged, whose tiles are 16 rows and
 // whose loads go straight to registers.  Otherwise the chunks' kernels, which
 // read a cell once for 128 or 256 rows but take longer to start.  Measured with
 // 16-row tiles and chunks (us): 8 sequences of 8 tokens over 500 cells, 32 heads
-// of 128 on 8: 21.8 and 30; of 32 tokens (2^29 below): 46.5 and 34.5; 32 of 16 over
-// 1000: 123 and 92; 9 heads of 64 on 3, 8 of 64 over 500: 19.4 and 24.0, over 2000
-// (2^29): 44.9 and 34.6; below 64 rows 32 of 8 over 1000: 78.8 and 82.6.
+// of 128 on 8: 20.0 and 24.3; of 32 tokens (2^29 below): 45.5 and 31.5; 32 of 16 over
+// 1000: 126 and 81; 9 heads of 64 on 3, 8 of 64 over 500: 19.1 and 22.2, over 2000
+// (2^29): 45.3 and 32.4; below 64 rows 32 of 8 over 1000: 76.5 and 71.0.
 constexpr int k_chunk_rows = 64;                // rows of a sequence on average, at least
 constexpr double k_chunk_work = 268435456.0;    // rows x kv heads x cells of the tables x head_dim, at least
 // From two tiles of a sequence on the cells are decoded once for all tiles,
 // while they fit the workspace.  Measured decoded before and in each workgroup
-// (us): 8 sequences of 512 tokens over 2000 cells 98 and 125 (64 dims), 369 and 376
-// (128); of 64 tokens 37 and 35, 113 and 122; of 32 over 500 25 and 23, 43 and 35.
+// (us), 32 heads of 64 and of 128 on 8: 8 sequences of 512 tokens over 2000 cells 214
+// and 250, 371 and 430; of 128 tokens (512 rows) 105 and 94, 156 and 149; of 64 tokens
+// 69 and 62, 112 and 96; of 32 over 500 32 and 23, 42 and 31.
 constexpr int k_decode_rows = 512;
 constexpr int64_t k_pre_bytes = (int64_t)1 << 30;   // of the workspace for decoded cells, at most
 // Waves of a workgroup.  Up to 64 dims four: two or three workgroups share a CU,
 // and uneven sequences leave smaller last tiles (a batch of 9 conversations of
-// 5 to 301 tokens 37 us, with eight waves 45).  Above, with cells decoded before, eight
-// from 2048 rows a sequence on, which copy a cell once for 256 rows (one sequence of
-// 4096 tokens, 32 heads of 128: 1043 us, with four 1141; 8 sequences of 128 tokens over 2000
-// cells: 178, with four 157).  Where each workgroup decodes, four, two workgroups
-// to a CU, above 128 rows a sequence (8 of 40 tokens over 2000 cells: 79 us, with eight
-// 101; of 64: 98 and 120), and eight up to there, of which half decode (32 of 16 over
-// 1000: 97 and 80), and for the many rows whose cells the workspace does not hold.
+// 5 to 301 tokens 37 us, with eight waves 45, before parts were smaller).  Above, with
+// cells decoded before, eight from 2048 rows a sequence on, which copy a cell once for
+// 256 rows (one sequence of 4096 tokens behind 4096, 32 heads of 128: 1053 us, with four
+// 1104; of 512 rows, 8 of 128 tokens over 2000 cells, 179, with four 157; at the border,
+// 4 of 512 tokens, 225 and 200).  Where each workgroup decodes, four, two workgroups
+// to a CU, above 128 rows a sequence (8 of 40 tokens over 2000 cells: 77 us, with eight
+// 100; of 64: 97 and 122), and eight up to there, of which half decode (32 of 16 over
+// 1000: 96 and 76), and for the many rows whose cells the workspace does not hold.
 constexpr int k_helped_rows = 128;
 constexpr int k_wide_rows = 2048;
 // Parts of a row's cells: as many workgroups as a CU runs at a time, a part at
 // least so many blocks of 64 cells (single tokens: 64 sequences of up to 8192 cells
-// 302 us with 16 a CU, 340 with 4; conversations 37 us with parts of 4 blocks, 40 with 8
-// and 55 with 2, of which the join reads more).
+// 297 us with 16 a CU, 326 with 4; conversations 33.5 us with parts of 4 blocks, 37.1 with 8
+// and 33.1 with 2, of which the join reads more).
 constexpr int k_few_wgs = 16, k_few_part = 8, k_many_wgs = 2, k_many_part = 4;
 // window: 0, or fewer parts for it (the workspace's size is that without).
 static attn_plan plan_attn(const lnship_paged_kv *kv, int64_t rep, int cus, int64_t window) {
@@ -1343,8 +1356,8 @@ static int launch_attn(const attn_paged_args &m, const attn_plan &p, int cus, hi
     }
     const dim3 grid((unsigned)p.tiles, (unsigned)m.kv.n_head_kv, (unsigned)p.splits);
     // A CU for each workgroup: eight waves, which go over their cells in half the steps
-    // (448 cells of 9 heads of 64 on 3 11.0 us, with four 12.0 and sixteen 12.3; 32 heads of
-    // 128 on 8 17.5 and 19.3; 64 sequences of 2000 cells of those 167 with eight, 130 with four).
+    // (448 cells of 9 heads of 64 on 3 11.0 us, with four 12.1; 32 heads of 128 on 8 17.4
+    // and 18.9; 64 sequences of 2000 cells of those 167 with eight, 129 with four).
     if constexpr (NB <= 4)
         if (p.tiles * m.kv.n_head_kv * p.splits <= cus) {
             if (m.kv.head_dim == NB * 32) hipLaunchKernelGGL((k_attn_paged<NB, true, 8>), grid, dim3(512), 0, s, m, err);
@@ -1384,14 +1397,14 @@ int lnship16_rope_store_kv_paged(const lnship_paged_kv *kv, const lnship_paged_s
     const bool vec = a->rope_n_dims > 0 && a->rope_n_dims % 8 == 0 &&
                      (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->cos_sin | (uintptr_t)a->q_dst) & 15) == 0 &&
                      ((a->q_ld | a->k_ld | s.a.q_dst_ld) & 3) == 0;
-    // (its tables take 4 us to lay out: 64 rows of 32 heads of 128 on 8 6.7 us without,
-    // 8.4 so, 128 rows 9.6 and 8.6; 128 of 9 heads of 64 on 3 4.9 and 8.3)
+    // (its tables take 4 us to lay out: 64 rows of 32 heads of 128 on 8 6.3 us without,
+    // 8.5 so, 128 rows 8.5 and 8.9, 256 13.8 and 10.2; 128 of 9 heads of 64 on 3 4.9 and 8.4)
     if (vec && nq <= 1 << 26 && kv->ntok * (nq + 2 * nk) >= 1 << 19) {
         // Eight rows of a prompt together, as their cells share cache lines (8 prompts
-        // of 511 to 2047 tokens, 32 heads of 64 on 8: 77 us, by single rows 85); single
+        // of 1400 tokens, 32 heads of 64 on 8: 68 us, by single rows 80); single
         // tokens' rows, and few, by themselves (4096 sequences' tokens, heads of 128: 75,
         // by eight 83).  Workgroups: 16 a CU, if there is an item for each thread (256
-        // tokens 10.3 us, a workgroup a row 13).
+        // tokens 10.2 us, a workgroup a row 13.2).
         const int sh = kv->ntok >= 1024 && kv->ntok >= 8 * kv->n_seq ? 3 : 0;
         const int64_t x = (((kv->ntok + (1 << sh) - 1) >> sh) + 7) / 8 * 8;   // (all of every XCD's share)
         const int64_t items = (nq / 8 + nk / 8 + nk / 4) << sh;

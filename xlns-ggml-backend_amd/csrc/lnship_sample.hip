@@ -372,8 +372,9 @@ __device__ __forceinline__ void draw_by_digits(const draw_args &a, const draw_ro
 //   too many tokens are) the row takes draw_by_digits.
 // - The segment that holds u's share is gone through again.
 // Bound by a row's passes on one CU: one of loads, and one of weights (above).
-// 256 rows of 131075: 22 us greedy (6 TB/s), 45 with a top_k, 53 with neither and
-// 74 with a top_p (with an exact histogram of 64-bit weights for its border 106).
+// 256 rows of 131075: 22 us greedy (6 TB/s), 45 with a top_k, 52 without limits and
+// 75 with a top_p (with an exact histogram of 64-bit weights for its border 106); by
+// digits 606 with a top_k of 5000, 904 with a top_p too.
 template <int R, bool MORE>
 __global__ __launch_bounds__(k_draw_block) void k_draw(draw_args a) {
     typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));   // rows need no alignment
@@ -810,8 +811,8 @@ int lnship_sample(const lnship_sample_args *a, void *stream) {
     const int rounds = (int)((a->n_vocab + k_seg * k_draw_waves - 1) / (k_seg * k_draw_waves));
     // Up to two segments a wave stay in registers; of longer rows one, and the
     // others are read for each pass, which costs less than the registers' spills
-    // (32000 logits 23.4 us in registers, 24.7 so; 49152: 22.1 so, 27.3 with three
-    // in registers; 131075: 75 so, 78 with two).
+    // (61 rows of 32000 logits 24.7 us in registers, 25.2 so; of 49152 31.2 so, 34.3 with
+    // three in registers, one row 17.9 and 17.2; 256 of 131075 75.4 so, 76.9 with two).
     if (rounds == 1) hipLaunchKernelGGL((k_draw<1, false>), grid, block, 0, st, d);
     else if (rounds == 2) hipLaunchKernelGGL((k_draw<2, false>), grid, block, 0, st, d);
     else hipLaunchKernelGGL((k_draw<1, true>), grid, block, 0, st, d);
