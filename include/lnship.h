@@ -484,8 +484,8 @@ int64_t lnship16_attn_paged_work(const lnship_paged_kv *kv, int64_t n_head);
  * 2^-40), so the draw does not depend on an order of additions; a weight is
  * exact to 2^-32.  n_vocab up to 2^19.  A row whose top_k is above 1024, or
  * with thousands of equal logits at a limit, takes ten to twenty times as long
- * as another.  No LNS arithmetic, and no counterpart in
- * the reference, which samples on the host. */
+ * as another.  No LNS arithmetic, and no counterpart in the reference, which
+ * samples on the host. */
 typedef struct lnship_sample_args {
     const float *logits;
     int64_t ld, n_rows, n_vocab;   /* ld 0: n_vocab */

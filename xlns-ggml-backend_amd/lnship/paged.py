@@ -116,9 +116,10 @@ def rope_store_kv(q, k, v, k_pages, v_pages, page, table, q_start, kv_len, cos_s
 def attention(q, k_pages, v_pages, page, table, q_start, kv_len, scale, window=0, out=None):
     """Attention of the new tokens q [ntok, n_head, head_dim] float32 over
     their sequences' cells in the pages: those up to each token's own position
-    and, with window > 0, no further than window - 1 before it.  Returns out,
-    [ntok, n_head, head_dim] float32.  Its workspace, up to 1 GiB for prompts,
-    comes from torch's allocator."""
+    and, with window > 0, no further than window - 1 before it (pages behind
+    every new token's window are not looked at, and may be freed).  Returns
+    out, [ntok, n_head, head_dim] float32, which may be q.  Its workspace, up
+    to 1 GiB for prompts, comes from torch's allocator."""
     ntok, nh = q.shape[:2]
     kv, dev, _, hd = _kv(k_pages, v_pages, page, table, q_start, kv_len, ntok)
     stream = current_stream(dev)
